@@ -644,6 +644,74 @@ int orca_hip_relu_bw_colsum(orca_hip_ctx* ctx, const float* grad, const float* p
 int orca_hip_relu_bw_colsum_noalloc(orca_hip_ctx* ctx, const float* grad, const float* pre, size_t rows,
                                     size_t cols, float* dpre, float* colsum);
 
+/* ---------------- Linear with activation and residual; 8-bit activation checkpoints ----------------
+ * No counterpart in the reference, whose Linear, activations and additions are ops of their own
+ * (python/orca/nn/linear.py:77-86, activation.py) and which keeps every activation in 32 bits.
+ *
+ * Products here read fp32 and give fp32 precision (each operand is taken apart into three bf16
+ * terms that add up to it; sums are fp32), on the bf16 matrix instructions.  Their sums run in
+ * another order than orca_hip_gemm's.  Infinities and NaN come out as from fp32 products.
+ * Sizes are below 2^31 each and may be 0; leading dimensions count elements; fp32 operands
+ * need no alignment beyond a float's.  A call may not write what it reads, or overlap two results,
+ * except as said below.  Work is enqueued on the context stream; workspaces come from the
+ * context's allocator, so these calls fail while launches go to the side stream, and under
+ * stream capture unless a call of the same sizes ran before. */
+#define ORCA_HIP_ACT_NONE 0
+#define ORCA_HIP_ACT_RELU 1      /* z > 0 ? z : 0 */
+#define ORCA_HIP_ACT_GELU 2      /* z * (1 + erf(z / sqrt 2)) / 2 */
+#define ORCA_HIP_ACT_GELU_TANH 3 /* z * (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+#define ORCA_HIP_ACT_SILU 4      /* z / (1 + exp(-z)) */
+
+/* An 8-bit checkpoint holds a matrix [rows][cols] as codes of 8 bits with one power-of-two step for
+ * each 32 columns of a row (the last group of a row may be shorter), in one 16-byte aligned buffer
+ * of *bytes: int8 codes [rows][cols], then at *scales_offset (optional) the step bytes
+ * [ceil(cols / 32)][rows in multiples of 16].  A value is code * 2^(byte - 133), exact in bf16 and
+ * f32.  Codes lie in -127 .. 127 and are rounded to nearest, ties to even; a group's byte is the
+ * least of 7 .. 254 with which no code passes 127, so a value is off by at most half a step and by
+ * 2^-7 of the group's largest magnitude (values above 127.5 * 2^121 become 127 * 2^121, groups below
+ * 2^-127 become zeros).  A group that holds an infinity or a NaN is stored as NaN as a whole
+ * (byte 255).  Bytes between the codes and the step bytes, and behind a group's last row, are not
+ * written and mean nothing. */
+int orca_hip_act8_size(size_t rows, size_t cols, size_t* bytes, size_t* scales_offset);
+int orca_hip_act8_pack(orca_hip_ctx* ctx, const float* x, size_t rows, size_t cols, size_t ldx, void* packed);
+/* dtype: ORCA_HIP_F32 or ORCA_HIP_BF16, of out [rows][ldo]. */
+int orca_hip_act8_unpack(orca_hip_ctx* ctx, const void* packed, size_t rows, size_t cols, int dtype, void* out,
+                         size_t ldo);
+
+typedef struct {
+  int act;               /* ORCA_HIP_ACT_* */
+  const float* bias;     /* [N], or NULL */
+  const float* residual; /* [M][ldr] added after the activation, or NULL; may be Y itself (ldr = ldy) */
+  size_t ldr;
+  float* pre;            /* [M][ldpre]: receives z = X W + bias, or NULL */
+  size_t ldpre;
+  void* pre8;            /* receives the checkpoint of z [M][N], or NULL */
+  void* y8;              /* receives the checkpoint of Y [M][N] (the next layer's input), or NULL */
+} orca_hip_linear_epilogue;
+/* Y[M][N] = act(X[M][K] W[K][N] + bias) + residual (epi NULL: Y = X W). */
+int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const float* X, size_t ldx, const float* W,
+                        size_t ldw, float* Y, size_t ldy, const orca_hip_linear_epilogue* epi);
+
+/* What a forward kept for its backward. */
+typedef struct {
+  int act;             /* ORCA_HIP_ACT_* */
+  const float* z;      /* [M][ldz] the pre-activation, or */
+  size_t ldz;
+  const void* z8;      /* its checkpoint: exactly one of the two (neither is read for ORCA_HIP_ACT_NONE).  With a
+                          checkpoint ReLU's gradient goes by the stored value: one that rounds to 0 counts as 0 */
+  const float* x;      /* [M][ldx] the input, or */
+  size_t ldx;
+  const void* x8;      /* its checkpoint: exactly one of the two, for dW */
+  const float* dx_add; /* [M][ldadd] added to dX (the gradient that came past the layer), or NULL;
+                          may be dX itself (ldadd = lddx) */
+  size_t ldadd;
+} orca_hip_linear_saved;
+/* dz = dY * act'(z); dX[M][K] = dz W^T + dx_add, dW[K][N] = X^T dz, db[N] = the column sums of dz, each
+ * optional.  The residual's gradient is dY itself. */
+int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const float* dY, size_t lddy,
+                                 const float* W, size_t ldw, const orca_hip_linear_saved* saved, float* dX,
+                                 size_t lddx, float* dW, size_t lddw, float* db);
+
 /* One AdamW step over flat buffers, same f32 op order as
  * python/orca/optim/adamw.py:71-94 with the f64 scalars rounded to f32 as
  * PyO3 does (orca-python/src/lib.rs:12-16).  t is the step count after

@@ -10,7 +10,7 @@ use std::fs;
 use std::path::{Path, PathBuf};
 use std::process::Command;
 
-const SOURCES: [&str; 9] = [
+const SOURCES: [&str; 11] = [
     "runtime_host.cpp",
     "storage.cpp",
     "runtime.hip",
@@ -20,6 +20,8 @@ const SOURCES: [&str; 9] = [
     "head.hip",
     "mlp.hip",
     "ewprog.hip",
+    "act8.hip",
+    "linear_act.hip",
 ];
 
 fn run(cmd: &mut Command) {

@@ -32,6 +32,8 @@ F32, F64, F16, BF16, I32, I64, U8, BOOL = range(8)
 VIEW_CONTIGUOUS = 0
 VIEW_TRANSPOSED = 1
 
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+
 EPI_NONE, EPI_BIAS, EPI_BIAS_RELU, EPI_RELU_MASK, EPI_BIAS_RELU_PRE, EPI_RELU_MASK_PRE = range(6)
 
 # Elementwise program opcodes and interpreter limits (include/orca_hip.h ORCA_HIP_EW_*).
@@ -68,6 +70,20 @@ class Epilogue(ctypes.Structure):
         ("pre", ctypes.c_void_p),
         ("done", ctypes.POINTER(ctypes.c_void_p)),
     ]
+
+
+class LinearEpilogue(ctypes.Structure):
+    """orca_hip_linear_epilogue."""
+    _fields_ = [("act", ctypes.c_int), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("ldr", ctypes.c_size_t), ("pre", ctypes.c_void_p), ("ldpre", ctypes.c_size_t),
+                ("pre8", ctypes.c_void_p), ("y8", ctypes.c_void_p)]
+
+
+class LinearSaved(ctypes.Structure):
+    """orca_hip_linear_saved."""
+    _fields_ = [("act", ctypes.c_int), ("z", ctypes.c_void_p), ("ldz", ctypes.c_size_t), ("z8", ctypes.c_void_p),
+                ("x", ctypes.c_void_p), ("ldx", ctypes.c_size_t), ("x8", ctypes.c_void_p),
+                ("dx_add", ctypes.c_void_p), ("ldadd", ctypes.c_size_t)]
 
 
 class Optim(ctypes.Structure):
@@ -231,6 +247,12 @@ SIGNATURES = {
     "orca_hip_max_to_shape_backward": [_P, _P, _P, _P, _SZP, _SZ, _SZP, _SZ, _I, _PP],
     "orca_hip_has_nan_or_inf": [_P, _P, _SZ, _I, ctypes.POINTER(_I)],
     "orca_hip_gemm": [_P, _I, _I, _SZ, _SZ, _SZ, _P, _SZ, _P, _SZ, _P, _SZ, ctypes.POINTER(Epilogue)],
+    "orca_hip_act8_size": [_SZ, _SZ, _SZP, _SZP],
+    "orca_hip_act8_pack": [_P, _P, _SZ, _SZ, _SZ, _P],
+    "orca_hip_act8_unpack": [_P, _P, _SZ, _SZ, _I, _P, _SZ],
+    "orca_hip_linear_act": [_P, _SZ, _SZ, _SZ, _P, _SZ, _P, _SZ, _P, _SZ, ctypes.POINTER(LinearEpilogue)],
+    "orca_hip_linear_act_backward": [_P, _SZ, _SZ, _SZ, _P, _SZ, _P, _SZ, ctypes.POINTER(LinearSaved), _P, _SZ, _P,
+                                     _SZ, _P],
     "orca_hip_narrow_linear_backward": [_P, _P, _SZ, _SZ, _P, _SZ, _P, _P, _P, _P, _P, _P, _PP],
     "orca_hip_softmax_ce": [_P, _P, _SZ, _SZ, _P, _P, _P, _P, _P, _P],
     "orca_hip_head_forward_ce": [_P, _P, _SZ, _SZ, _P, _P, _SZ, _P, _P, _P, _P, _P, _P, _P],
