@@ -609,6 +609,78 @@ class Linear(Module):
         return out
 
 
+class LinearAct(Linear):
+    """A Linear with its activation and a residual in the product's epilogue:
+    y = act(x @ W + bias) + residual, one tape node whose backward gives the gradients of x, W,
+    bias and the residual (no counterpart in the reference, where each is an op of its own and
+    gelu and silu do not exist; orca_hip_linear_act).  activation: "none", "relu", "gelu",
+    "gelu_tanh" or "silu".
+
+    checkpoint=True keeps what the backward reads (x and the pre-activation) as 8-bit
+    checkpoints instead of in 32 bits: 33/32 bytes a value in place of 4, and a weight gradient at half the
+    matrix work, with gradients that see x and the pre-activation to about 2^-8 of the largest
+    magnitude among 32 neighbours.  The output then carries its own checkpoint, which a
+    LinearAct(checkpoint=True) above takes as its input's."""
+
+    def __init__(self, ad: Autodiff, weight: np.ndarray, bias: np.ndarray | None, activation: str = "none",
+                 checkpoint: bool = False):
+        super().__init__(ad, weight, bias)
+        if not hasattr(ad.inner, "linear_act"):
+            raise OrcaError("LinearAct needs a backend with linear_act")
+        if activation not in ad.inner.ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ad.inner.ACTIVATIONS)}")
+        self.activation, self.checkpoint = activation, checkpoint
+
+    def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
+        K, N = self.in_features, self.out_features
+        if len(x.shape) < 2 or x.shape[-1] != K:
+            raise OrcaError(f"Shape mismatch during linear_act: expected [..., {K}], got {list(x.shape)}")
+        out_shape = x.shape[:-1] + (N,)
+        if residual is not None and residual.shape != out_shape:
+            raise OrcaError(f"Shape mismatch during linear_act: expected {list(out_shape)}, got {list(residual.shape)}")
+        ad, be, act = x.ad, x.ad.inner, self.activation
+        tensors = [x, self.weight.tensor] + ([self.bias.tensor] if self.bias is not None else []) \
+            + ([residual] if residual is not None else [])
+        if any(t.ad is not ad for t in tensors):
+            raise OrcaError("Device mismatch: tensors must be on the same device")
+        M = _numel(x.shape[:-1])
+        w, b = self.weight.tensor.storage, self.bias.tensor.storage if self.bias is not None else None
+        r = residual.storage if residual is not None else None
+        ids = [s.node_id if s is not None else None for s in (x.storage, w, b, r)]
+        record = ad.grad_enabled and any(i is not None for i in ids)
+        want_z = record and act != "none" and any(i is not None for i in ids[:3])
+        keep = ()
+        if want_z:
+            keep += ("z8",) if self.checkpoint else ("z",)
+        if record and self.checkpoint:
+            keep += ("y8",)
+        y, kept = be.linear_act(x.storage.primal, w.primal, b.primal if b else None, r.primal if r else None, M, N, K,
+                                act, keep)
+        saved_x = None
+        if record and ids[1] is not None:
+            saved_x = x.storage.primal
+            if self.checkpoint:
+                saved_x = x.checkpoint if getattr(x, "checkpoint", None) is not None else be.act8_pack(saved_x, M, K)
+        z, wp = kept.get("z8", kept.get("z")), w.primal
+        want = tuple(k for k, i in zip(("dx", "dw", "db"), ids[:3]) if i is not None)
+        same = ids[3] is not None and ids[3] == ids[0]  # y = act(x W) + x: both gradients in one product
+        has_bias, has_residual = b is not None, r is not None  # the node holds no more of them than that
+
+        def backward(g, be):
+            out = be.linear_act_backward(g, wp, M, N, K, act, z=z, x=saved_x, dx_add=g if same else None,
+                                         want=want) if want else {}
+            grads = [out.get("dx"), out.get("dw")]
+            if has_bias:
+                grads.append(out.get("db"))
+            if has_residual:
+                grads.append(None if same else g)
+            return grads
+        t = Tensor(ad, ad.custom(y, [s for s in (x.storage, w, b, r) if s is not None], backward), out_shape)
+        if "y8" in kept:
+            t.checkpoint = kept["y8"]
+        return t
+
+
 class ReLU(Module):
     """python/orca/nn/activation.py:5-21."""
 
@@ -980,5 +1052,5 @@ def argmax_rows(logits: np.ndarray) -> np.ndarray:
     return out
 
 
-__all__ = ["Autodiff", "Tensor", "Tape", "no_grad", "Linear", "ReLU", "Sequential", "CrossEntropyLoss", "MSELoss",
+__all__ = ["Autodiff", "Tensor", "Tape", "no_grad", "Linear", "LinearAct", "ReLU", "Sequential", "CrossEntropyLoss", "MSELoss",
            "SGD", "AdamW", "Parameter", "Module", "build_mlp", "argmax_rows", "OrcaError", "math"]

@@ -112,6 +112,22 @@ class HipStorage:
         self.h = None
 
 
+class Act8:
+    """An 8-bit checkpoint of a matrix [rows, cols] (include/orca_hip.h, orca_hip_act8_size): the
+    codes and steps in a device storage of 33/32 bytes a value."""
+
+    __slots__ = ("storage", "rows", "cols")
+
+    def __init__(self, storage: HipStorage, rows: int, cols: int):
+        self.storage, self.rows, self.cols = storage, rows, cols
+
+    @property
+    def nbytes(self) -> int:
+        b = ctypes.c_size_t()
+        _lib.call("orca_hip_act8_size", self.rows, self.cols, ctypes.byref(b), None)
+        return b.value
+
+
 class HipBackend:
     """Drop-in for `GpuBackend` (orca-backend-gpu/src/backend.rs:45-50): an `orca_hip_backend`
     on a context.  The switches select the library's planning (include/orca_hip.h
@@ -361,6 +377,105 @@ class HipBackend:
     def sgd_step_(self, p: HipStorage, g: HipStorage, n: int, lr: float) -> None:
         """In place on p (orca_hip_be_sgd_step)."""
         _lib.call("orca_hip_be_sgd_step", self.handle, p.h, g.h, n, lr)
+
+    # ---- Linear with activation and residual; 8-bit activation checkpoints ----
+    ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU,
+                   "gelu_tanh": _lib.ACT_GELU_TANH, "silu": _lib.ACT_SILU}
+
+    def _act(self, name: str) -> int:
+        if name not in self.ACTIVATIONS:
+            raise ValueError(f"unknown activation {name!r}: one of {', '.join(self.ACTIVATIONS)}")
+        return self.ACTIVATIONS[name]
+
+    def _operand(self, s: HipStorage | None, n: int, what: str):
+        """(address, storage to hold until the call) of a contiguous storage of n values."""
+        if s is None:
+            return None, None
+        if s.be.ctx is not self.ctx:
+            raise ValueError(f"Device mismatch: {what} is on another context")
+        if s.n != n:
+            raise ValueError(f"Shape mismatch during {what}: expected {n} elements, got {s.n}")
+        if s.transposed:
+            s = self.clone(s)
+        return s.ptr, s
+
+    def _checkpoint(self, rows: int, cols: int) -> Act8:
+        c = Act8(None, rows, cols)
+        c.storage = self.arena(-(-c.nbytes // 4))
+        return c
+
+    def _checkpoint_ptr(self, c: Act8 | None, rows: int, cols: int, what: str):
+        if c is None:
+            return None
+        if c.storage.be.ctx is not self.ctx:
+            raise ValueError(f"Device mismatch: {what} is on another context")
+        if (c.rows, c.cols) != (rows, cols):
+            raise ValueError(f"Shape mismatch during {what}: expected {[rows, cols]}, got {[c.rows, c.cols]}")
+        return c.storage.ptr
+
+    def act8_pack(self, s: HipStorage, rows: int, cols: int) -> Act8:
+        """The 8-bit checkpoint of a matrix (orca_hip_act8_pack)."""
+        p, hold = self._operand(s, rows * cols, "act8_pack")  # noqa: F841
+        c = self._checkpoint(rows, cols)
+        _lib.call("orca_hip_act8_pack", self.ctx.handle, p, rows, cols, cols, c.storage.ptr)
+        return c
+
+    def act8_unpack(self, c: Act8) -> HipStorage:
+        """The values a checkpoint stands for, in f32 (orca_hip_act8_unpack)."""
+        p = self._checkpoint_ptr(c, c.rows, c.cols, "act8_unpack")
+        out = self.arena(c.rows * c.cols)
+        _lib.call("orca_hip_act8_unpack", self.ctx.handle, p, c.rows, c.cols, _lib.F32, out.ptr, c.cols)
+        return out
+
+    def linear_act(self, x: HipStorage, w: HipStorage, bias: HipStorage | None, residual: HipStorage | None, M: int,
+                   N: int, K: int, act: str = "none", keep: tuple = ()):
+        """y = act(x w + bias) + residual of [M, K] x [K, N] in one product (orca_hip_linear_act).
+        Returns y and what `keep` names besides: "z" the pre-activation, "z8" and "y8" checkpoints
+        of the pre-activation and of y, as a dict."""
+        act = self._act(act)
+        if not set(keep) <= {"z", "z8", "y8"}:
+            raise ValueError(f"linear_act cannot keep {sorted(set(keep) - {'z', 'z8', 'y8'})}")
+        xp, hx = self._operand(x, M * K, "linear_act (x)")
+        wp, hw = self._operand(w, K * N, "linear_act (weight)")
+        bp, hb = self._operand(bias, N, "linear_act (bias)")
+        rp, hr = self._operand(residual, M * N, "linear_act (residual)")
+        y = self.arena(M * N)
+        kept = {k: self.arena(M * N) if k == "z" else self._checkpoint(M, N) for k in keep}
+        e = _lib.LinearEpilogue(act=act, bias=bp, residual=rp, ldr=N, pre=kept["z"].ptr if "z" in kept else None,
+                                ldpre=N, pre8=kept["z8"].storage.ptr if "z8" in kept else None,
+                                y8=kept["y8"].storage.ptr if "y8" in kept else None)
+        _lib.call("orca_hip_linear_act", self.ctx.handle, M, N, K, xp, K, wp, N, y.ptr, N, ctypes.byref(e))
+        del hx, hw, hb, hr
+        return y, kept
+
+    def linear_act_backward(self, dy: HipStorage, w: HipStorage, M: int, N: int, K: int, act: str = "none",
+                            z: HipStorage | Act8 | None = None, x: HipStorage | Act8 | None = None,
+                            dx_add: HipStorage | None = None, want: tuple = ("dx", "dw", "db")) -> dict:
+        """The gradients that `want` names (orca_hip_linear_act_backward); z and x are what the
+        forward kept, in f32 or as checkpoints."""
+        act = self._act(act)
+        if not set(want) <= {"dx", "dw", "db"}:
+            raise ValueError(f"linear_act_backward cannot give {sorted(set(want) - {'dx', 'dw', 'db'})}")
+        dyp, hdy = self._operand(dy, M * N, "linear_act_backward (dy)")
+        wp, hw = self._operand(w, K * N, "linear_act_backward (weight)")
+        ap, ha = self._operand(dx_add, M * K, "linear_act_backward (dx_add)")
+        held = {}
+
+        def kept(t, cols, what):
+            if isinstance(t, Act8):
+                return None, self._checkpoint_ptr(t, M, cols, what)
+            p, held[what] = self._operand(t, M * cols, what)
+            return p, None
+
+        zp, z8 = kept(z if act != _lib.ACT_NONE else None, N, "linear_act_backward (z)")
+        xp, x8 = kept(x if "dw" in want else None, K, "linear_act_backward (x)")
+        out = {k: self.arena({"dx": M * K, "dw": K * N, "db": N}[k]) for k in want}
+        s = _lib.LinearSaved(act=act, z=zp, ldz=N, z8=z8, x=xp, ldx=K, x8=x8, dx_add=ap, ldadd=K)
+        p = {k: t.ptr for k, t in out.items()}
+        _lib.call("orca_hip_linear_act_backward", self.ctx.handle, M, N, K, dyp, N, wp, N, ctypes.byref(s),
+                  p.get("dx"), K, p.get("dw"), N, p.get("db"))
+        del hdy, hw, ha
+        return out
 
     # ---- flat arenas and one-launch optimizer passes ----
     def arena(self, n: int, fill: float | None = None) -> HipStorage:
