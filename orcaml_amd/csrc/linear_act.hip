@@ -69,154 +69,236 @@ __device__ __forceinline__ void store_codes(int8_t* p, int have, floatx4 v, uint
   for (int j = 0; j < 3; ++j)
     if (j < have) p[j] = (int8_t)(w >> (8 * j));
 }
+__device__ __forceinline__ floatx4 load_codes(const int8_t* p, int have) {
+  uint32_t w = 0;
+  if (have == 4) {
+    typedef uint32_t word_u __attribute__((aligned(1)));
+    w = *reinterpret_cast<const word_u*>(p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < have) w |= (uint32_t)(uint8_t)p[j] << (8 * j);
+  }
+  return floatx4{(float)(int8_t)w, (float)(int8_t)(w >> 8), (float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24)};
+}
 __device__ __forceinline__ uint32_t quad_top(floatx4 v, int have) {
   uint32_t t = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) t = max(t, j < have ? act8_magnitude(v[j]) : 0u);
   return t;
 }
-__device__ __forceinline__ floatx4 activate(int act, floatx4 z) {
+// The epilogue of four neighbouring columns of row m (`have` of them exist; none in a row past M).
+// Eight neighbouring lanes hold a checkpoint's group of 32 columns.
+__device__ __forceinline__ void quad_out(const LinearOut& o, floatx4 z, floatx4 bias, floatx4 residual, int64_t m,
+                                         int64_t c, int have) {
+  z = z + bias;
   floatx4 y;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = activation(act, z[j]);
-  return y;
-}
-
-// A lane's part of a 32 x 32 block: row m, columns n + 8 q .. + 3 for q = 0 .. 3 (n past the half
-// wave's four).  The other half wave holds the row's other 16 columns.
-__device__ __forceinline__ void block_out(const LinearOut& o, const acc32& acc, int64_t m, int64_t n, int64_t M,
-                                          int64_t N) {
-  const bool row = m < M;
-  uint32_t ztop = 0, ytop = 0;
-  floatx4 z[4], y[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int64_t c = n + 8 * q;
-    const int have = row ? (int)max((int64_t)0, min((int64_t)4, N - c)) : 0;
-    z[q] = floatx4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-    if (o.bias) z[q] = z[q] + load_quad(o.bias + c, have);
-    y[q] = activate(o.act, z[q]);
-    if (o.residual) y[q] = y[q] + load_quad(o.residual + m * o.ldr + c, have);
-    ztop = max(ztop, quad_top(z[q], have));
-    ytop = max(ytop, quad_top(y[q], have));
-  }
-  uint32_t zb = 0, yb = 0;
-  if (o.pre8.codes) zb = act8_byte(max(ztop, (uint32_t)__shfl_xor((int)ztop, 32)));
-  if (o.y8.codes) yb = act8_byte(max(ytop, (uint32_t)__shfl_xor((int)ytop, 32)));
-  if (!row) return;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int64_t c = n + 8 * q;
-    const int have = (int)max((int64_t)0, min((int64_t)4, N - c));
-    if (o.pre) store_quad(o.pre + m * o.ldpre + c, have, z[q]);
-    store_quad(o.y + m * o.ldy + c, have, y[q]);
-    if (o.pre8.codes) store_codes(o.pre8.codes + m * o.pre8.cols + c, have, z[q], zb);
-    if (o.y8.codes) store_codes(o.y8.codes + m * o.y8.cols + c, have, y[q], yb);
-  }
-  if (n % 32 == 0 && n < N) {
-    if (o.pre8.codes) o.pre8.scales[n / 32 * o.pre8.ld + m] = (uint8_t)zb;
-    if (o.y8.codes) o.y8.scales[n / 32 * o.y8.ld + m] = (uint8_t)yb;
-  }
-}
-
-template <class T, template <int, int, int> class LoadA, template <int, int, int> class LoadB>
-__global__ void __launch_bounds__(T::THREADS, T::OCC* T::THREADS / 256) split_product_kernel(ProductArgs p) {
-  using LA = LoadA<T::BM, T::BK, T::THREADS>;
-  using LB = LoadB<T::BN, T::BK, T::THREADS>;
-  __shared__ u32x4 smem[2 * (LA::UNITS + LB::UNITS)];
-  // Consecutive blocks go to the 8 XCDs in turn: each XCD takes a run of tiles, eight tile rows
-  // by column, so that its blocks share the operand panels in its L2.
-  const int nb = gridDim.x, x = blockIdx.x % 8, lin = x * (nb / 8) + min(x, nb % 8) + blockIdx.x / 8;
-  const int tiles = p.tiles_m * p.tiles_n, split = lin / tiles, tile = lin % tiles;
-  const int width = 8 * p.tiles_n, first = tile / width * 8, rows = min(8, p.tiles_m - first);
-  const int m0 = (first + tile % width % rows) * T::BM, n0 = tile % width / rows * T::BN;
-  acc32 acc[T::FM][T::FN];
-  product<T, LA, LB>(p.A, p.B, m0, n0, split * p.chunk, min(p.K, (split + 1) * p.chunk), smem, acc);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t m = m0 + wave / T::WN * (T::FM * 32) + (lane & 31);
-  const int64_t n = n0 + wave % T::WN * (T::FN * 32) + (lane >> 5) * 4;
-#pragma unroll
-  for (int i = 0; i < T::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < T::FN; ++j) {
-      if (p.splits == 1) {
-        block_out(p.out, acc[i][j], m + 32 * i, n + 32 * j, p.M, p.N);
-        continue;
-      }
-      if (m + 32 * i >= p.M) continue;
-      float* w = p.ws + ((int64_t)split * p.M + m + 32 * i) * p.N;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t c = n + 32 * j + 8 * q;
-        store_quad(w + c, (int)max((int64_t)0, min((int64_t)4, p.N - c)),
-                   floatx4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
-      }
-    }
-}
-
-// The splits' partial products, added in split order, and the epilogue.  A lane takes four columns,
-// eight lanes a checkpoint's group of 32.
-__global__ void __launch_bounds__(256) split_product_finish_kernel(ProductArgs p) {
-  const int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t c = (int64_t)blockIdx.y * 256 + (threadIdx.x & 63) * 4;
-  if (m >= p.M) return;  // a whole wave
-  const LinearOut& o = p.out;
-  const int have = (int)max((int64_t)0, min((int64_t)4, p.N - c));
-  floatx4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.splits; ++s) z = z + load_quad(p.ws + ((int64_t)s * p.M + m) * p.N + c, have);
-  if (o.bias) z = z + load_quad(o.bias + c, have);
-  floatx4 y = activate(o.act, z);
-  if (o.residual) y = y + load_quad(o.residual + m * o.ldr + c, have);
+  activations<4>(o.act, z, y);
+  y = y + residual;
   auto group = [](uint32_t top) {
+#pragma unroll
     for (int d = 1; d < 8; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
     return act8_byte(top);
   };
   uint32_t zb = 0, yb = 0;
   if (o.pre8.codes) zb = group(quad_top(z, have));
   if (o.y8.codes) yb = group(quad_top(y, have));
+  if (have == 0) return;
   if (o.pre) store_quad(o.pre + m * o.ldpre + c, have, z);
   store_quad(o.y + m * o.ldy + c, have, y);
-  const bool lead = (threadIdx.x & 7) == 0 && c < p.N;
   if (o.pre8.codes) {
     store_codes(o.pre8.codes + m * o.pre8.cols + c, have, z, zb);
-    if (lead) o.pre8.scales[c / 32 * o.pre8.ld + m] = (uint8_t)zb;
+    if (c % 32 == 0) o.pre8.scales[c / 32 * o.pre8.ld + m] = (uint8_t)zb;
   }
   if (o.y8.codes) {
     store_codes(o.y8.codes + m * o.y8.cols + c, have, y, yb);
-    if (lead) o.y8.scales[c / 32 * o.y8.ld + m] = (uint8_t)yb;
+    if (c % 32 == 0) o.y8.scales[c / 32 * o.y8.ld + m] = (uint8_t)yb;
+  }
+}
+__device__ __forceinline__ floatx4 bias_quad(const LinearOut& o, int64_t c, int have) {
+  return o.bias ? load_quad(o.bias + c, have) : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+__device__ __forceinline__ floatx4 residual_quad(const LinearOut& o, int64_t m, int64_t c, int have) {
+  return o.residual ? load_quad(o.residual + m * o.ldr + c, have) : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+template <class T, template <int, int, int> class LoadA, template <int, int, int> class LoadB>
+constexpr int tile_units() {
+  return 2 * (LoadA<T::BM, T::BK, T::THREADS>::UNITS + LoadB<T::BN, T::BK, T::THREADS>::UNITS);
+}
+
+// Block `block` of `blocks` of one product.
+template <class T, template <int, int, int> class LoadA, template <int, int, int> class LoadB>
+__device__ __forceinline__ void tile_product(const ProductArgs& p, int block, int blocks, u32x4* __restrict__ smem) {
+  using LA = LoadA<T::BM, T::BK, T::THREADS>;
+  using LB = LoadB<T::BN, T::BK, T::THREADS>;
+  // Consecutive blocks go to the 8 XCDs in turn: each XCD takes a run of tiles, eight tile rows
+  // by column, so that its blocks share the operand panels in its L2.
+  const int x = block % 8, lin = x * (blocks / 8) + min(x, blocks % 8) + block / 8;
+  const int tiles = p.tiles_m * p.tiles_n, split = lin / tiles, tile = lin % tiles;
+  const int width = 8 * p.tiles_n, first = tile / width * 8, rows = min(8, p.tiles_m - first);
+  const int m0 = (first + tile % width % rows) * T::BM, n0 = tile % width / rows * T::BN;
+  acc32 acc[T::FM][T::FN];
+  product<T, LA, LB>(p.A, p.B, m0, n0, split * p.chunk, min(p.K, (split + 1) * p.chunk), smem, acc);
+  // The tile leaves through LDS, a 32 x 32 block of each wave at a time: a lane's four rows of four
+  // columns lie along the rows then (whole lines to and from memory, and a checkpoint's group in eight
+  // lanes), and the epilogue is one piece of code instead of one per block.
+  constexpr int PITCH = 36;
+  static_assert(T::THREADS / 64 * 32 * PITCH / 4 <= tile_units<T, LoadA, LoadB>(), "the waves' blocks fit the stages");
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float* stage = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
+#pragma unroll 1
+  for (int b = 0; b < T::FM * T::FN; ++b) {
+#pragma unroll
+    for (int i = 0; i < T::FM * T::FN; ++i)
+      if (i == b) {
+        const acc32& v = acc[i / T::FN][i % T::FN];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<floatx4*>(stage + (lane & 31) * PITCH + 8 * q + (lane >> 5) * 4) =
+              floatx4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+      }
+    const int64_t m = m0 + wave / T::WN * (T::FM * 32) + b / T::FN * 32 + lane / 8;
+    const int64_t c = n0 + wave % T::WN * (T::FN * 32) + b % T::FN * 32 + lane % 8 * 4;
+    const int cols = (int)max((int64_t)0, min((int64_t)4, p.N - c));
+    floatx4 bias = {0.0f, 0.0f, 0.0f, 0.0f}, res[4];
+    if (p.splits == 1) {
+      bias = bias_quad(p.out, c, cols);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) res[q] = residual_quad(p.out, m + 8 * q, c, m + 8 * q < p.M ? cols : 0);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t r = m + 8 * q;
+      const int have = r < p.M ? cols : 0;
+      const floatx4 z = *reinterpret_cast<const floatx4*>(stage + (lane / 8 + 8 * q) * PITCH + lane % 8 * 4);
+      if (p.splits == 1)
+        quad_out(p.out, z, bias, res[q], r, c, have);
+      else if (have)
+        store_quad(p.ws + ((int64_t)split * p.M + r) * p.N + c, have, z);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
 }
 
-// dz = dy * act'(z) (z in fp32, or its checkpoint) and, per block of 64 rows, the column sums of dz.
-// A thread takes four columns of 16 rows.
-constexpr int kSlopeRows = 64;
+template <class T>
+__global__ void __launch_bounds__(T::THREADS, T::OCC* T::THREADS / 256) linear_act_kernel(ProductArgs p) {
+  __shared__ u32x4 smem[tile_units<T, LoadKFast, LoadKSlow>()];
+  tile_product<T, LoadKFast, LoadKSlow>(p, blockIdx.x, gridDim.x, smem);
+}
+
+// The backward's two products and the last step of the bias gradient, each a run of blocks.
+struct BackwardArgs {
+  ProductArgs dx, dw;
+  int dx_blocks, dw_blocks;  // the rest: db
+  const float* partial;      // [partials][N]
+  int64_t partials, N;
+  float* db;
+};
+
+// db[n] = the sum of the slope kernel's column sums: RUNS runs of blocks, each in order, then the runs in order.
+template <int RUNS>
+__device__ __forceinline__ void finish_bias(const BackwardArgs& p, int block, float* __restrict__ sums) {
+  const int64_t n = (int64_t)block * 32 + (threadIdx.x & 31);
+  const int run = threadIdx.x >> 5;
+  const int64_t per = (p.partials + RUNS - 1) / RUNS, end = min(p.partials, (run + 1) * per);
+  float s = 0.0f;
+  if (n < p.N)
+    for (int64_t b = run * per; b < end; ++b) s = s + p.partial[b * p.N + n];
+  sums[threadIdx.x] = s;
+  __syncthreads();
+  if (run == 0 && n < p.N) {
+    for (int i = 1; i < RUNS; ++i) s = s + sums[32 * i + threadIdx.x];
+    p.db[n] = s;
+  }
+}
+
+template <class T, template <int, int, int> class LoadX>
+__global__ void __launch_bounds__(T::THREADS, T::OCC* T::THREADS / 256) linear_act_backward_kernel(BackwardArgs p) {
+  __shared__ u32x4 smem[tile_units<T, LoadKFast, LoadKFast>()];  // the larger of the two products'
+  const int block = blockIdx.x;
+  if (block < p.dx_blocks)
+    tile_product<T, LoadKFast, LoadKFast>(p.dx, block, p.dx_blocks, smem);
+  else if (block < p.dx_blocks + p.dw_blocks)
+    tile_product<T, LoadX, LoadKSlow>(p.dw, block - p.dx_blocks, p.dw_blocks, smem);
+  else
+    finish_bias<T::THREADS / 32>(p, block - p.dx_blocks - p.dw_blocks, reinterpret_cast<float*>(smem));
+}
+
+// The splits' partial products of up to two products, added in split order, and the epilogue.  A
+// lane takes four columns, eight lanes a checkpoint's group of 32; a block 4 rows of 256 columns.
+struct FinishArgs {
+  ProductArgs p[2];
+  int64_t blocks[2];
+};
+__global__ void __launch_bounds__(256) split_finish_kernel(FinishArgs a) {
+  int64_t block = blockIdx.x;
+  const bool second = block >= a.blocks[0];
+  if (second) block -= a.blocks[0];
+  const ProductArgs& p = a.p[second];
+  const int64_t groups = (p.N + 255) / 256;
+  const int64_t m = block / groups * 4 + (threadIdx.x >> 6);
+  const int64_t c = block % groups * 256 + (threadIdx.x & 63) * 4;
+  if (m >= p.M) return;  // a whole wave
+  const int have = (int)max((int64_t)0, min((int64_t)4, p.N - c));
+  const floatx4 bias = bias_quad(p.out, c, have), residual = residual_quad(p.out, m, c, have);
+  floatx4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float* w = p.ws + m * p.N + c;
+  const int64_t step = p.M * p.N;
+  int s = 0;
+  for (; s + 8 <= p.splits; s += 8) {  // eight loads ahead of their additions
+    floatx4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = load_quad(w + (s + i) * step, have);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z = z + v[i];
+  }
+  for (; s < p.splits; ++s) z = z + load_quad(w + s * step, have);
+  quad_out(p.out, z, bias, residual, m, c, have);
+}
+
+// dz = dy * act'(z) (z in fp32, or its checkpoint) and, per block of 4 R rows, the column sums of dz.
+// A thread takes four columns of R rows, four rows' loads at a time.
+template <int R>
 __global__ void __launch_bounds__(256) slope_kernel(const float* __restrict__ dy, int64_t lddy, int act,
                                                     const float* __restrict__ z, int64_t ldz, Act8 z8,
                                                     float* __restrict__ dz, float* __restrict__ partial, int64_t M,
                                                     int64_t N) {
   __shared__ floatx4 sums[4][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t c = (int64_t)blockIdx.y * 256 + lane * 4, r0 = (int64_t)blockIdx.x * kSlopeRows + wave * 16;
+  const int64_t c = (int64_t)blockIdx.y * 256 + lane * 4, r0 = (int64_t)blockIdx.x * (4 * R) + wave * R;
   const int have = (int)max((int64_t)0, min((int64_t)4, N - c));
   floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int r = 0; r < 16; ++r) {
-    const int64_t m = r0 + r;
-    if (m >= M || have == 0) break;
-    floatx4 g = load_quad(dy + m * lddy + c, have);
-    if (act != ORCA_HIP_ACT_NONE) {
-      floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int r = 0; r < R && r0 + r < M; r += 4) {
+    const int rows = (int)min((int64_t)4, M - r0 - r);
+    floatx4 g[4], v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t m = r0 + r + min(i, rows - 1);
+      g[i] = load_quad(dy + m * lddy + c, have);
+      v[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (act == ORCA_HIP_ACT_NONE || have == 0) continue;
       if (z8.codes) {
         const float step = act8_step(z8.scales[c / 32 * z8.ld + m]);
-        for (int j = 0; j < 4; ++j)
-          if (j < have) v[j] = (float)z8.codes[m * z8.cols + c + j] * step;
+        v[i] = load_codes(z8.codes + m * z8.cols + c, have) * step;
       } else {
-        v = load_quad(z + m * ldz + c, have);
+        v[i] = load_quad(z + m * ldz + c, have);
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) g[j] = g[j] * activation_slope(act, v[j]);
-      store_quad(dz + m * N + c, have, g);
     }
-    sum = sum + g;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i >= rows) break;
+      if (act != ORCA_HIP_ACT_NONE) {
+        activation_slopes<4>(act, v[i], g[i]);
+        store_quad(dz + (r0 + r + i) * N + c, have, g[i]);
+      }
+      sum = sum + g[i];
+    }
   }
   if (!partial) return;
   sums[wave][lane] = sum;
@@ -225,81 +307,104 @@ __global__ void __launch_bounds__(256) slope_kernel(const float* __restrict__ dy
     store_quad(partial + (int64_t)blockIdx.x * N + c, have, sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]);
 }
 
-// db[n] = the sum of the blocks' column sums: 8 runs of blocks, each in order, then the runs in order.
-__global__ void __launch_bounds__(256) slope_finish_kernel(const float* __restrict__ partial, int64_t blocks, int64_t N,
-                                                           float* __restrict__ db) {
-  __shared__ float sums[8][32];
-  const int64_t n = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-  const int run = threadIdx.x >> 5;
-  const int64_t per = (blocks + 7) / 8, end = min(blocks, (run + 1) * per);
-  float s = 0.0f;
-  if (n < N)
-    for (int64_t b = run * per; b < end; ++b) s = s + partial[b * N + n];
-  sums[run][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (run == 0 && n < N) {
-    for (int i = 1; i < 8; ++i) s = s + sums[i][threadIdx.x];
-    db[n] = s;
-  }
-}
-
-
 dim3 quad_grid(int64_t rows, int64_t per, int64_t cols, const char* op) {
   const int64_t gx = (rows + per - 1) / per, gy = (cols + 255) / 256;
   if (gx > 0x7fffffff || gy > 65535) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
   return dim3((unsigned)gx, (unsigned)gy);
 }
 
-enum class Load { kFast, kSlow, kCodes };
+// 256: eight waves of 128 x 64, the least LDS traffic for a matrix instruction; at 8192 x 4096 x 4096 228 TFLOP/s
+// (of fp32 work; 128: 201, 64: 154).  128 and 64 for products with too few tiles of 256.
+using Tile256 = ProductTile<256, 256, 2, 4, 16, 1>;
+using Tile128 = ProductTile<128, 128, 2, 4, 32, 1>;
+using Tile64 = ProductTile<64, 64, 2, 2, 32, 3>;
 
-using Tile128 = ProductTile<128, 128, 2, 2, 16, 2>;
+struct Plan {
+  int tile = 0;       // 0: nothing to do
+  int64_t blocks = 0;
+  size_t ws = 0;      // floats of partial products
+};
 
-template <class T>
-void launch_tile(orca_hip_ctx* ctx, Load a, Load b, unsigned grid, const ProductArgs& p) {
-  const dim3 threads(T::THREADS);
-  if (a == Load::kFast && b == Load::kSlow)
-    hipLaunchKernelGGL((split_product_kernel<T, LoadKFast, LoadKSlow>), dim3(grid), threads, 0, ctx->stream, p);
-  else if (a == Load::kFast && b == Load::kFast)
-    hipLaunchKernelGGL((split_product_kernel<T, LoadKFast, LoadKFast>), dim3(grid), threads, 0, ctx->stream, p);
-  else if (a == Load::kSlow)
-    hipLaunchKernelGGL((split_product_kernel<T, LoadKSlow, LoadKSlow>), dim3(grid), threads, 0, ctx->stream, p);
-  else
-    hipLaunchKernelGGL((split_product_kernel<T, LoadCodes, LoadKSlow>), dim3(grid), threads, 0, ctx->stream, p);
+// Microseconds of a product on a tile with its k range split, on an otherwise idle GPU of 256 CUs:
+// fitted to 7700 products of 1 .. 8192 x 16 .. 4096 x 16 .. 4096, each timed with every tile and split
+// (8 % rms near the best ones; the choice by it takes 1.7 % longer than the best, 11 % in one case of
+// twenty).  A launch; then the CU with the most blocks, `together` of them at a time: a stage's chain of
+// waits, or its throughput; with splits the second launch, which reads and writes them.
+struct TileCost {
+  int tile, bk, together;
+  double launch, chain, block, stage, each, finish, bytes_per_us;
+};
+constexpr TileCost kTileCosts[2][3] = {
+    {{64, 32, 3, 5.5, 0.584, 0.0, 0.432, 0.97, 3.2, 6.0e6},
+     {128, 32, 1, 5.5, 1.159, 2.65, 1.159, 2.65, 1.6, 2.9e6},
+     {256, 16, 1, 8.0, 1.783, 7.44, 1.783, 7.44, 0.0, 3.5e6}},
+    // the row operand is a checkpoint: half the matrix instructions
+    {{64, 32, 3, 5.0, 0.495, 0.97, 0.305, 1.43, 3.5, 8.0e6},
+     {128, 32, 1, 5.4, 0.765, 2.93, 0.819, 1.42, 2.2, 3.2e6},
+     {256, 16, 1, 9.7, 1.031, 8.29, 1.031, 8.29, 0.0, 4.3e6}}};
+
+// Tiles and splits of `p`'s product.
+Plan plan_product(orca_hip_ctx* ctx, ProductArgs& p, bool codes, const char* op) {
+  Plan best;
+  double best_us = 0.0;
+  for (const TileCost& c : kTileCosts[codes]) {
+    const int64_t tm = (p.M + c.tile - 1) / c.tile, tn = (p.N + c.tile - 1) / c.tile;
+    if (tm > 0x3fffffff / tn) continue;
+    for (int64_t splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (splits > 1 && (p.K < 48 * splits || tm * tn * splits > 8 * ctx->num_cus)) break;
+      // even runs of a multiple of every stage's k values
+      const int64_t chunk = std::max<int64_t>(64, ((p.K + splits - 1) / splits + 63) / 64 * 64);
+      const int64_t n = std::max<int64_t>(1, (p.K + chunk - 1) / chunk);
+      if (splits > 1 && n == 1) continue;
+      const int64_t per_cu = (tm * tn * n + ctx->num_cus - 1) / ctx->num_cus;
+      const double stages = (double)((std::min(chunk, p.K) + c.bk - 1) / c.bk);
+      double us = c.launch + std::max((double)((per_cu + c.together - 1) / c.together) * (stages * c.chain + c.block),
+                                      (double)per_cu * (stages * c.stage + c.each));
+      if (n > 1) us += c.finish + 4.0 * (double)(n + 1) * (double)p.M * (double)p.N / c.bytes_per_us;
+      if (best.tile && us >= best_us) continue;
+      best_us = us;
+      best.tile = c.tile;
+      best.blocks = tm * tn * n;
+      best.ws = n > 1 ? (size_t)n * p.M * p.N : 0;
+      p.tiles_m = (int)tm;
+      p.tiles_n = (int)tn;
+      p.splits = (int)n;
+      p.chunk = chunk;
+    }
+  }
+  if (!best.tile) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
+  return best;
+}
+
+int64_t finish_blocks(const ProductArgs& p, const Plan& q) {
+  return q.ws ? (p.M + 3) / 4 * ((p.N + 255) / 256) : 0;
+}
+void launch_finish(orca_hip_ctx* ctx, const ProductArgs& a, const Plan& qa, const ProductArgs& b, const Plan& qb,
+                   const char* op) {
+  FinishArgs f{{a, b}, {finish_blocks(a, qa), finish_blocks(b, qb)}};
+  const int64_t grid = f.blocks[0] + f.blocks[1];
+  if (!grid) return;
+  if (grid > 0x7fffffff) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
+  hipLaunchKernelGGL(split_finish_kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, f);
   ORCA_HIP_CHECK(hipGetLastError());
 }
 
-// out = the product of A [M][K] and B [N][K] with its epilogue.
-void product(orca_hip_ctx* ctx, const char* name, Load la, const ProductOperand& A, Load lb, const ProductOperand& B,
-             int64_t M, int64_t N, int64_t K, const LinearOut& out) {
-  ProductArgs p{};
-  p.A = A;
-  p.B = B;
-  p.M = M;
-  p.N = N;
-  p.K = K;
-  p.out = out;
-  const int64_t tm = (M + 127) / 128, tn = (N + 127) / 128;
-  if (tm > 0x7fffffff / tn / 64) fail(ORCA_HIP_ERR_INTERNAL, std::string(name) + ": matrix too large");
-  p.tiles_m = (int)tm;
-  p.tiles_n = (int)tn;
-  // too few tiles for the CUs: k in even runs of at least 64 values
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>({2 * ctx->num_cus / (tm * tn), K / 64, 64}));
-  p.chunk = std::max<int64_t>(64, ((K + splits - 1) / splits + 63) / 64 * 64);
-  p.splits = (int)std::max<int64_t>(1, (K + p.chunk - 1) / p.chunk);
-  std::unique_ptr<Scratch> ws;
-  if (p.splits > 1) {
-    ws.reset(new Scratch(ctx, sizeof(float) * (size_t)p.splits * M * N));
-    p.ws = ws->as<float>();
-  }
-  std::string pname;
-  if (ctx->prof.enabled)
-    pname = std::string(name) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
-  ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K, 4.0 * ((double)M * K + (double)K * N + (double)M * N));
-  launch_tile<Tile128>(ctx, la, lb, (unsigned)(tm * tn * p.splits), p);
-  if (p.splits > 1) {
-    hipLaunchKernelGGL(split_product_finish_kernel, quad_grid(M, 4, N, name), dim3(256), 0, ctx->stream, p);
-    ORCA_HIP_CHECK(hipGetLastError());
-  }
+template <class T>
+void launch_backward(orca_hip_ctx* ctx, bool codes, unsigned grid, const BackwardArgs& b) {
+  if (codes)
+    hipLaunchKernelGGL((linear_act_backward_kernel<T, LoadCodes>), dim3(grid), dim3(T::THREADS), 0, ctx->stream, b);
+  else
+    hipLaunchKernelGGL((linear_act_backward_kernel<T, LoadKSlow>), dim3(grid), dim3(T::THREADS), 0, ctx->stream, b);
+  ORCA_HIP_CHECK(hipGetLastError());
+}
+void launch_backward(orca_hip_ctx* ctx, int tile, bool codes, const BackwardArgs& b) {
+  const unsigned grid = (unsigned)(b.dx_blocks + b.dw_blocks + (b.db ? (b.N + 31) / 32 : 0));
+  if (tile == 256)
+    launch_backward<Tile256>(ctx, codes, grid, b);
+  else if (tile == 128)
+    launch_backward<Tile128>(ctx, codes, grid, b);
+  else
+    launch_backward<Tile64>(ctx, codes, grid, b);
 }
 
 void check_ld(const char* what, size_t ld, size_t cols) {
@@ -379,8 +484,32 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
     o.ldy = (int64_t)ldy;
     o.pre8 = act8_at(e.pre8, M, N);
     o.y8 = act8_at(e.y8, M, N);
-    product(ctx, op, Load::kFast, ProductOperand{X, (int64_t)ldx, (int)M, nullptr, 0}, Load::kSlow,
-            ProductOperand{W, (int64_t)ldw, (int)N, nullptr, 0}, (int64_t)M, (int64_t)N, (int64_t)K, o);
+    ProductArgs p{};
+    p.A = ProductOperand{X, (int64_t)ldx, (int)M, nullptr, 0};
+    p.B = ProductOperand{W, (int64_t)ldw, (int)N, nullptr, 0};
+    p.M = (int64_t)M;
+    p.N = (int64_t)N;
+    p.K = (int64_t)K;
+    p.out = o;
+    const Plan q = plan_product(ctx, p, false, op);
+    std::unique_ptr<Scratch> ws;
+    if (q.ws) {
+      ws.reset(new Scratch(ctx, sizeof(float) * q.ws));
+      p.ws = ws->as<float>();
+    }
+    std::string pname;
+    if (ctx->prof.enabled)
+      pname = std::string(op) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
+    ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K, 4.0 * ((double)M * K + (double)K * N + (double)M * N));
+    const dim3 grid((unsigned)q.blocks);
+    if (q.tile == 256)
+      hipLaunchKernelGGL(linear_act_kernel<Tile256>, grid, dim3(Tile256::THREADS), 0, ctx->stream, p);
+    else if (q.tile == 128)
+      hipLaunchKernelGGL(linear_act_kernel<Tile128>, grid, dim3(Tile128::THREADS), 0, ctx->stream, p);
+    else
+      hipLaunchKernelGGL(linear_act_kernel<Tile64>, grid, dim3(Tile64::THREADS), 0, ctx->stream, p);
+    ORCA_HIP_CHECK(hipGetLastError());
+    launch_finish(ctx, p, q, p, Plan(), op);
   });
 }
 
@@ -436,7 +565,9 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     const float* dz = dY;
     int64_t lddz = (int64_t)lddy;
     std::unique_ptr<Scratch> dzs, partial;
-    const int64_t blocks = ((int64_t)M + kSlopeRows - 1) / kSlopeRows;
+    // 64 rows a block, 16 where that leaves CUs without one
+    const bool tall = ((int64_t)M + 63) / 64 * (((int64_t)N + 255) / 256) >= ctx->num_cus;
+    const int64_t rows = tall ? 64 : 16, blocks = ((int64_t)M + rows - 1) / rows;
     if (N && (want_db || (slope && (want_dx || want_dw)))) {
       if (slope && M) {
         dzs.reset(new Scratch(ctx, sizeof(float) * M * N));
@@ -444,41 +575,76 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
         lddz = (int64_t)N;
       }
       if (want_db && M) partial.reset(new Scratch(ctx, sizeof(float) * (size_t)blocks * N));
-      ProfScope prof(ctx, "linear_act_slope", 0.0, (slope ? 12.0 : 4.0) * M * N);
       if (M) {
-        hipLaunchKernelGGL(slope_kernel, quad_grid((int64_t)M, kSlopeRows, (int64_t)N, op), dim3(256), 0, ctx->stream,
-                           dY, (int64_t)lddy, s.act, static_cast<const float*>(z.p), (int64_t)s.ldz,
-                           act8_at(const_cast<void*>(z8.p), M, N), dzs ? dzs->as<float>() : nullptr,
+        ProfScope prof(ctx, "linear_act_slope", 0.0, (slope ? 12.0 : 4.0) * M * N);
+        hipLaunchKernelGGL(tall ? slope_kernel<16> : slope_kernel<4>, quad_grid((int64_t)M, rows, (int64_t)N, op),
+                           dim3(256), 0, ctx->stream, dY, (int64_t)lddy, s.act, static_cast<const float*>(z.p),
+                           (int64_t)s.ldz, act8_at(const_cast<void*>(z8.p), M, N), dzs ? dzs->as<float>() : nullptr,
                            partial ? partial->as<float>() : nullptr, (int64_t)M, (int64_t)N);
         ORCA_HIP_CHECK(hipGetLastError());
       }
-      if (want_db) {
-        hipLaunchKernelGGL(slope_finish_kernel, dim3((unsigned)((N + 31) / 32)), dim3(256), 0, ctx->stream,
-                           partial ? partial->as<float>() : nullptr, M ? blocks : 0, (int64_t)N, db);
-        ORCA_HIP_CHECK(hipGetLastError());
-      }
     }
+    BackwardArgs b{};
+    b.N = (int64_t)N;
+    if (want_db) {
+      b.db = db;
+      b.partial = partial ? partial->as<float>() : nullptr;
+      b.partials = M ? blocks : 0;
+    }
+    Plan qx, qw;
     if (want_dx) {
-      LinearOut o;
-      o.residual = s.dx_add;
-      o.ldr = (int64_t)s.ldadd;
-      o.y = dX;
-      o.ldy = (int64_t)lddx;
-      product(ctx, "linear_act_dx", Load::kFast, ProductOperand{dz, lddz, (int)M, nullptr, 0}, Load::kFast,
-              ProductOperand{W, (int64_t)ldw, (int)K, nullptr, 0}, (int64_t)M, (int64_t)K, (int64_t)N, o);
+      b.dx.A = ProductOperand{dz, lddz, (int)M, nullptr, 0};
+      b.dx.B = ProductOperand{W, (int64_t)ldw, (int)K, nullptr, 0};
+      b.dx.M = (int64_t)M;
+      b.dx.N = (int64_t)K;
+      b.dx.K = (int64_t)N;
+      b.dx.out.residual = s.dx_add;
+      b.dx.out.ldr = (int64_t)s.ldadd;
+      b.dx.out.y = dX;
+      b.dx.out.ldy = (int64_t)lddx;
+      qx = plan_product(ctx, b.dx, false, op);
     }
     if (want_dw) {
-      LinearOut o;
-      o.y = dW;
-      o.ldy = (int64_t)lddw;
-      ProductOperand a{s.x, (int64_t)s.ldx, (int)K, nullptr, 0};
+      b.dw.A = ProductOperand{s.x, (int64_t)s.ldx, (int)K, nullptr, 0};
       if (s.x8) {
         const Act8 q = act8_at(const_cast<void*>(s.x8), M, K);
-        a = ProductOperand{q.codes, q.cols, (int)K, q.scales, q.ld};
+        b.dw.A = ProductOperand{q.codes, q.cols, (int)K, q.scales, q.ld};
       }
-      product(ctx, "linear_act_dw", s.x8 ? Load::kCodes : Load::kSlow, a, Load::kSlow,
-              ProductOperand{dz, lddz, (int)N, nullptr, 0}, (int64_t)K, (int64_t)N, (int64_t)M, o);
+      b.dw.B = ProductOperand{dz, lddz, (int)N, nullptr, 0};
+      b.dw.M = (int64_t)K;
+      b.dw.N = (int64_t)N;
+      b.dw.K = (int64_t)M;
+      b.dw.out.y = dW;
+      b.dw.out.ldy = (int64_t)lddw;
+      qw = plan_product(ctx, b.dw, s.x8 != nullptr, op);
     }
+    std::unique_ptr<Scratch> ws;
+    if (qx.ws + qw.ws) {
+      ws.reset(new Scratch(ctx, sizeof(float) * (qx.ws + qw.ws)));
+      b.dx.ws = ws->as<float>();
+      b.dw.ws = ws->as<float>() + qx.ws;
+    }
+    if (!qx.tile && !qw.tile && !b.db) return;
+    std::string pname;
+    if (ctx->prof.enabled)
+      pname = std::string(op) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
+    ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K * (want_dx + want_dw),
+                   4.0 * ((double)M * N + (want_dx + want_dw) * ((double)M * K + (double)K * N)));
+    const bool codes = s.x8 != nullptr, one = !qx.tile || !qw.tile || qx.tile == qw.tile;
+    b.dx_blocks = (int)qx.blocks;
+    b.dw_blocks = (int)qw.blocks;
+    if (one) {
+      launch_backward(ctx, std::max(std::max(qx.tile, qw.tile), 64), codes, b);
+    } else {  // the bias gradient goes with the first
+      BackwardArgs only = b;
+      only.dw_blocks = 0;
+      launch_backward(ctx, qx.tile, codes, only);
+      only.dx_blocks = 0;
+      only.dw_blocks = b.dw_blocks;
+      only.db = nullptr;
+      launch_backward(ctx, qw.tile, codes, only);
+    }
+    launch_finish(ctx, b.dx, qx, b.dw, qw, op);
   });
 }
 

@@ -19,7 +19,7 @@
 // different banks.
 //
 // Infinities and NaN: inf - inf in the split, and inf times an m or l of zero, make NaN where
-// fp32 has an infinity.  So a block that ends with a NaN anywhere multiplies its tile again
+// fp32 has an infinity.  So a block that ends with a value that is not finite multiplies its tile again
 // on the fp32 instructions, from the same LDS layout (h + m + l is x; an infinity or NaN is
 // kept in h alone).
 #pragma once
@@ -59,91 +59,76 @@ __device__ __forceinline__ uint32_t round_pair(float a, float b) {
 __device__ __forceinline__ float low_half(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float high_half(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
-// The three planes of a pair of values.  SAFE: infinities and NaN stay in h, with m = l = 0.
+// A unit of 8 values on its way to LDS, a piece of work of five or six instructions at a time (what the
+// matrix unit hides behind one of its own): pieces 2 j and 2 j + 1 split pair j, piece 8 stores the
+// three planes (`plane` units apart).  SAFE: infinities and NaN stay in h, with m = l = 0.
 template <bool SAFE>
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t& h, uint32_t& m, uint32_t& l) {
-  if (SAFE) {
-    const bool fa = __builtin_isfinite(a), fb = __builtin_isfinite(b);
-    const uint32_t ua = a != a ? 0x7fc00000u : __float_as_uint(a), ub = b != b ? 0x7fc00000u : __float_as_uint(b);
-    h = upper_halves(ua, ub);
-    const float ra = fa ? a - low_half(h) : 0.0f, rb = fb ? b - high_half(h) : 0.0f;
-    m = round_pair(ra, rb);
-    l = round_pair(ra - low_half(m), rb - high_half(m));
-    return;
-  }
-  h = upper_halves(__float_as_uint(a), __float_as_uint(b));
-  const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-  const float rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-  m = round_pair(ra, rb);
-  l = round_pair(ra - low_half(m), rb - high_half(m));
-}
-
-// 8 values to the unit at `dst` of each plane (`plane` units apart).
-template <bool SAFE>
-__device__ __forceinline__ void store_split(const float (&v)[8], u32x4* dst, int plane) {
+struct SplitUnit {
+  static constexpr int PIECES = 9;
   u32x4 h, m, l;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint32_t a, b, c;
-    split_pair<SAFE>(v[2 * j], v[2 * j + 1], a, b, c);
-    h[j] = a;
-    m[j] = b;
-    l[j] = c;
+  float ra, rb;
+  __device__ __forceinline__ void piece(int k, const float (&v)[8], u32x4* dst, int plane) {
+    if (k == 8) {
+      dst[0] = h;
+      dst[plane] = m;
+      dst[2 * plane] = l;
+      return;
+    }
+    const int j = k / 2;
+    const float a = v[2 * j], b = v[2 * j + 1];
+    if (k % 2 == 0) {
+      if (SAFE) {
+        h[j] = upper_halves(a != a ? 0x7fc00000u : __float_as_uint(a), b != b ? 0x7fc00000u : __float_as_uint(b));
+        ra = __builtin_isfinite(a) ? a - low_half(h[j]) : 0.0f;
+        rb = __builtin_isfinite(b) ? b - high_half(h[j]) : 0.0f;
+      } else {
+        h[j] = upper_halves(__float_as_uint(a), __float_as_uint(b));
+        ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+        rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+      }
+    } else {
+      m[j] = round_pair(ra, rb);
+      l[j] = round_pair(ra - low_half(m[j]), rb - high_half(m[j]));
+    }
   }
-  dst[0] = h;
-  dst[plane] = m;
-  dst[2 * plane] = l;
-}
+};
 
-constexpr int unit_pitch(int rows) { return rows + 2; }
+constexpr int unit_pitch(int rows, int kh) { return rows + 8 / kh; }
 
-// Loaders: a stage is BK k values of ROWS rows, taken as units of 8 k values of one row,
-// UN units per thread.  Rows past the operand's last are the last one again (what they give
-// is never stored); k values past the range are zero (tail).
+// Loaders: a stage is BK k values of ROWS rows, one unit of 8 k values of one row per thread.  Rows past
+// the operand's last are the last one again (what they give is never stored); k values past the range are zero (tail).  piece(k) for k in 0 .. 8 takes the loaded
+// unit to LDS.  The product comes out 1 / SCALE times too large, unless SAFE.
 
 // k is contiguous: a unit is 32 bytes, at any alignment of its floats.
 template <int ROWS, int BK, int THREADS>
 struct LoadKFast {
-  static constexpr int PLANES = 3, KH = BK / 8, UN = ROWS * KH / THREADS, PITCH = unit_pitch(ROWS);
-  static constexpr int UNITS = PLANES * KH * PITCH;
-  static_assert(ROWS * KH % THREADS == 0, "whole units per thread");
-  const float* p[UN];
-  float v[UN][8];
+  static constexpr float SCALE = 1.0f;
+  static constexpr int PLANES = 3, KH = BK / 8, PITCH = unit_pitch(ROWS, KH), UNITS = PLANES * KH * PITCH;
+  static_assert(ROWS * KH == THREADS, "a unit per thread");
+  const float* p;
+  float v[8];
 
   __device__ __forceinline__ void init(const ProductOperand& op, int row0, int64_t k0) {
-#pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const int u = threadIdx.x + i * THREADS;
-      p[i] = static_cast<const float*>(op.p) + (int64_t)min(row0 + u / KH, op.rows - 1) * op.ld + k0 + u % KH * 8;
-    }
+    const int u = threadIdx.x;
+    p = static_cast<const float*>(op.p) + (int64_t)min(row0 + u / KH, op.rows - 1) * op.ld + k0 + u % KH * 8;
   }
   __device__ __forceinline__ void load() {
+    const floatx4 a = *reinterpret_cast<const floatx4_u*>(p), b = *reinterpret_cast<const floatx4_u*>(p + 4);
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const floatx4 a = *reinterpret_cast<const floatx4_u*>(p[i]), b = *reinterpret_cast<const floatx4_u*>(p[i] + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[i][j] = a[j];
-        v[i][4 + j] = b[j];
-      }
-      p[i] += BK;
+    for (int j = 0; j < 4; ++j) {
+      v[j] = a[j];
+      v[4 + j] = b[j];
     }
+    p += BK;
   }
   __device__ __forceinline__ void load_tail(int left) {
+    const int k = threadIdx.x % KH * 8;
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const int k = (threadIdx.x + i * THREADS) % KH * 8;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = k + j < left ? p[i][j] : 0.0f;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = k + j < left ? p[j] : 0.0f;
   }
   template <bool SAFE>
-  __device__ __forceinline__ void store(u32x4* s) const {
-#pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const int u = threadIdx.x + i * THREADS;
-      store_split<SAFE>(v[i], s + u % KH * PITCH + u / KH, KH * PITCH);
-    }
+  __device__ __forceinline__ void piece(int k, SplitUnit<SAFE>& u, u32x4* s) const {
+    u.piece(k, v, s + threadIdx.x % KH * PITCH + threadIdx.x / KH, KH * PITCH);
   }
 };
 
@@ -151,119 +136,96 @@ struct LoadKFast {
 // at a time, and the 8 that a thread collects are a unit, so the transpose costs nothing.
 template <int ROWS, int BK, int THREADS>
 struct LoadKSlow {
-  static constexpr int PLANES = 3, KH = BK / 8, UN = ROWS * KH / THREADS, PITCH = unit_pitch(ROWS);
-  static constexpr int UNITS = PLANES * KH * PITCH;
-  static_assert(ROWS * KH % THREADS == 0 && ROWS % 64 == 0, "whole units per thread, whole waves per k");
-  const float* base;  // uniform
-  int64_t ld;
-  uint32_t col[UN];
-  float v[UN][8];
+  static constexpr float SCALE = 1.0f;
+  static constexpr int PLANES = 3, KH = BK / 8, PITCH = unit_pitch(ROWS, KH), UNITS = PLANES * KH * PITCH;
+  static_assert(ROWS * KH == THREADS && ROWS % 64 == 0, "a unit per thread, whole waves per k");
+  const char* base;  // uniform: the first of this wave's 8 k values
+  int64_t ld;        // bytes
+  uint32_t col;      // bytes
+  float v[8];
 
-  static __device__ __forceinline__ int kh(int i) {
-    return __builtin_amdgcn_readfirstlane((threadIdx.x + i * THREADS) / ROWS);
-  }
+  static __device__ __forceinline__ int kh() { return __builtin_amdgcn_readfirstlane(threadIdx.x / ROWS); }
   __device__ __forceinline__ void init(const ProductOperand& op, int row0, int64_t k0) {
-    ld = op.ld;
-    base = static_cast<const float*>(op.p) + k0 * ld;
-#pragma unroll
-    for (int i = 0; i < UN; ++i) col[i] = (uint32_t)min(row0 + (int)(threadIdx.x + i * THREADS) % ROWS, op.rows - 1);
+    ld = op.ld * 4;
+    base = static_cast<const char*>(op.p) + (k0 + kh() * 8) * ld;
+    col = (uint32_t)min(row0 + (int)threadIdx.x % ROWS, op.rows - 1) * 4u;
   }
   __device__ __forceinline__ void load() {
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const float* q = base + kh(i) * 8 * ld;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = (q + j * ld)[col[i]];
-    }
+    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float*>(base + j * ld + col);
     base += BK * ld;
   }
   __device__ __forceinline__ void load_tail(int left) {
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const float* q = base + kh(i) * 8 * ld;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = kh(i) * 8 + j < left ? (q + j * ld)[col[i]] : 0.0f;
-    }
+    for (int j = 0; j < 8; ++j)
+      v[j] = kh() * 8 + j < left ? *reinterpret_cast<const float*>(base + j * ld + col) : 0.0f;
   }
   template <bool SAFE>
-  __device__ __forceinline__ void store(u32x4* s) const {
-#pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const int u = threadIdx.x + i * THREADS;
-      store_split<SAFE>(v[i], s + u / ROWS * PITCH + u % ROWS, KH * PITCH);
-    }
+  __device__ __forceinline__ void piece(int k, SplitUnit<SAFE>& u, u32x4* s) const {
+    u.piece(k, v, s + threadIdx.x / ROWS * PITCH + threadIdx.x % ROWS, KH * PITCH);
   }
 };
 
 // A checkpoint read the same way: k values are its rows.  One plane, no split.
 template <int ROWS, int BK, int THREADS>
 struct LoadCodes {
-  static constexpr int PLANES = 1, KH = BK / 8, UN = ROWS * KH / THREADS, PITCH = unit_pitch(ROWS);
-  static constexpr int UNITS = PLANES * KH * PITCH;
-  static_assert(ROWS * KH % THREADS == 0 && ROWS % 64 == 0, "whole units per thread, whole waves per k");
-  const int8_t* base;  // uniform
+  static constexpr float SCALE = 1.0f / 64;
+  static constexpr int PLANES = 1, KH = BK / 8, PITCH = unit_pitch(ROWS, KH), UNITS = PLANES * KH * PITCH;
+  static_assert(ROWS * KH == THREADS && ROWS % 64 == 0, "a unit per thread, whole waves per k");
+  const char* base;     // uniform
   int64_t ld;
-  uint32_t col[UN];
-  const uint8_t* step[UN];  // of this thread's 8 k values
-  int v[UN][8];
-  u32x2 b[UN];
+  uint32_t col;
+  const uint8_t* step;  // of this thread's 8 k values
+  int v[8];
+  u32x2 b;
 
-  static __device__ __forceinline__ int kh(int i) {
-    return __builtin_amdgcn_readfirstlane((threadIdx.x + i * THREADS) / ROWS);
-  }
+  static __device__ __forceinline__ int kh() { return __builtin_amdgcn_readfirstlane(threadIdx.x / ROWS); }
   __device__ __forceinline__ void init(const ProductOperand& op, int row0, int64_t k0) {
     ld = op.ld;
-    base = static_cast<const int8_t*>(op.p) + k0 * ld;
-#pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      col[i] = (uint32_t)min(row0 + (int)(threadIdx.x + i * THREADS) % ROWS, op.rows - 1);
-      // k0 and kh(i) * 8 are multiples of 8, a group's bytes fill its row to a multiple of 16
-      step[i] = op.scales + (int64_t)(col[i] / kAct8Group) * op.lds + k0 + kh(i) * 8;
-    }
+    base = static_cast<const char*>(op.p) + (k0 + kh() * 8) * ld;
+    col = (uint32_t)min(row0 + (int)threadIdx.x % ROWS, op.rows - 1);
+    // k0 and kh() * 8 are multiples of 8, a group's bytes fill its row to a multiple of 16
+    step = op.scales + (int64_t)(col / kAct8Group) * op.lds + k0 + kh() * 8;
   }
   __device__ __forceinline__ void load() {
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const int8_t* q = base + kh(i) * 8 * ld;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = (q + j * ld)[col[i]];
-      b[i] = *reinterpret_cast<const u32x2*>(step[i]);
-      step[i] += BK;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const int8_t*>(base + j * ld + col);
+    b = *reinterpret_cast<const u32x2*>(step);
+    step += BK;
     base += BK * ld;
   }
   __device__ __forceinline__ void load_tail(int left) {
+    left -= kh() * 8;
 #pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const int8_t* q = base + kh(i) * 8 * ld;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = kh(i) * 8 + j < left ? (q + j * ld)[col[i]] : 0;
-      // the step bytes of rows past the last are whatever they are: 0 instead
-      b[i] = u32x2{0, 0};
-      if (kh(i) * 8 < left) {
-        b[i] = *reinterpret_cast<const u32x2*>(step[i]);
-        const int have = min(left - kh(i) * 8, 8);
-        if (have < 8) {
-          const uint64_t keep = (1ull << (8 * have)) - 1;
-          b[i][0] &= (uint32_t)keep;
-          b[i][1] &= (uint32_t)(keep >> 32);
-        }
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? *reinterpret_cast<const int8_t*>(base + j * ld + col) : 0;
+    // the step bytes of rows past the last are whatever they are: 0 instead
+    b = u32x2{0, 0};
+    if (left > 0) {
+      b = *reinterpret_cast<const u32x2*>(step);
+      if (left < 8) {
+        const uint64_t keep = (1ull << (8 * left)) - 1;
+        b[0] &= (uint32_t)keep;
+        b[1] &= (uint32_t)(keep >> 32);
       }
     }
   }
   template <bool SAFE>
-  __device__ __forceinline__ void store(u32x4* s) const {
-#pragma unroll
-    for (int i = 0; i < UN; ++i) {
-      const int u = threadIdx.x + i * THREADS;
-      float f[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = (float)v[i][j] * act8_step((b[i][j / 4] >> (8 * (j % 4))) & 255u);
-      u32x4 h;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) h[j] = upper_halves(__float_as_uint(f[2 * j]), __float_as_uint(f[2 * j + 1]));
-      s[u / ROWS * PITCH + u % ROWS] = h;
-    }
+  __device__ __forceinline__ void piece(int k, SplitUnit<SAFE>& u, u32x4* s) const {
+    // The step byte as an exponent is 64 times the step, and an infinity for a group that is not finite:
+    // its codes are zero, so its values NaN.  Where that overflows the product is not finite either, and
+    // the block multiplies again with SAFE.
+    auto value = [&](int j) {
+      const uint32_t w = b[j / 4];
+      if (SAFE) return __float_as_uint((float)v[j] * act8_step((w >> (8 * (j % 4))) & 255u));
+      const uint32_t e = (j % 4 < 3 ? w << (23 - 8 * (j % 4)) : w >> 1) & 0x7f800000u;
+      return __float_as_uint((float)v[j] * __uint_as_float(e));
+    };
+    if (k == 8)
+      s[threadIdx.x / ROWS * PITCH + threadIdx.x % ROWS] = u.h;
+    else if (k % 2 == 0)
+      u.ra = __uint_as_float(value(k));
+    else
+      u.h[k / 2] = upper_halves(__float_as_uint(u.ra), value(k));
   }
 };
 
@@ -274,122 +236,174 @@ struct ProductTile {
   static constexpr int THREADS = WM * WN * 64, FM = BM / WM / 32, FN = BN / WN / 32;
 };
 
-// The stage in `sa`, `sb` onto a wave's blocks.  The first operand of the instruction is B, so
-// a lane holds row lane % 32 of A's and, in element r, column (r / 4) * 8 + (lane / 32) * 4 + r % 4
-// of B's 32: four neighbouring columns of C in four registers.
-template <class T, class LA, class LB, bool FP32>
-__device__ __forceinline__ void product_stage(const u32x4* __restrict__ sa, const u32x4* __restrict__ sb, int ra,
-                                              int rb, acc32 (&acc)[T::FM][T::FN]) {
-  constexpr int KH = T::BK / 8;
-  const int half = (threadIdx.x & 63) >> 5;
+// A unit of work: FN blocks of a wave, 16 k values.  The first operand of the instruction is B, so a lane
+// holds row lane % 32 of A's and, in element r, column (r / 4) * 8 + (lane / 32) * 4 + r % 4 of B's
+// 32: four neighbouring columns of C in four registers.
+// After matrix instruction g (of FN * terms), work(g) adds other work, which runs while the matrix unit is
+// busy: about five vector instructions hide behind one of its 32 cycles.  Nothing moves across:
+// the compiler left to itself puts all other work before the first of them.
+template <class LA>
+constexpr int terms() {
+  return LA::PLANES == 3 ? 6 : 3;
+}
+template <int FN, class LA, class LB, bool FP32, class Work>
+__device__ __forceinline__ void product_unit(const u32x4 (&a)[LA::PLANES], const u32x4 (&b)[FN][LB::PLANES],
+                                             acc32 (&acc)[FN], Work work) {
+  if constexpr (FP32) {
+    auto whole = [](const u32x4* f, int planes, int e) {
+      float x = 0.0f;
+      for (int p = 0; p < planes; ++p) x = x + (e % 2 ? high_half(f[p][e / 2]) : low_half(f[p][e / 2]));
+      return x;
+    };
 #pragma unroll
-  for (int s = 0; s < T::BK / 16; ++s) {
-    const int kh = 2 * s + half;
-    u32x4 b[T::FN][LB::PLANES];
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int j = 0; j < T::FN; ++j)
+      for (int j = 0; j < FN; ++j)
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(whole(b[j], LB::PLANES, e), whole(a, LA::PLANES, e), acc[j], 0, 0, 0);
+  } else {
+    // the smallest terms first
+    constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0}, PB1[3] = {2, 1, 0};
 #pragma unroll
-      for (int p = 0; p < LB::PLANES; ++p) b[j][p] = sb[(p * KH + kh) * LB::PITCH + rb + 32 * j];
+    for (int t = 0; t < terms<LA>(); ++t) {
+      const int pa = LA::PLANES == 3 ? PA[t] : 0, pb = LA::PLANES == 3 ? PB[t] : PB1[t];
 #pragma unroll
-    for (int i = 0; i < T::FM; ++i) {
-      u32x4 a[LA::PLANES];
-#pragma unroll
-      for (int p = 0; p < LA::PLANES; ++p) a[p] = sa[(p * KH + kh) * LA::PITCH + ra + 32 * i];
-      if constexpr (FP32) {
-        auto whole = [](const u32x4* f, int planes, int e) {
-          float x = 0.0f;
-          for (int p = 0; p < planes; ++p) x = x + (e % 2 ? high_half(f[p][e / 2]) : low_half(f[p][e / 2]));
-          return x;
-        };
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int j = 0; j < T::FN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(whole(b[j], LB::PLANES, e), whole(a, LA::PLANES, e),
-                                                             acc[i][j], 0, 0, 0);
-      } else {
-        // the smallest terms first
-        auto term = [&](int pa, int pb) {
-#pragma unroll
-          for (int j = 0; j < T::FN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b[j][pb]),
-                                                                __builtin_bit_cast(bf16x8, a[pa]), acc[i][j], 0, 0, 0);
-        };
-        if constexpr (LA::PLANES == 3) {
-          term(0, 2);
-          term(2, 0);
-          term(1, 1);
-          term(0, 1);
-          term(1, 0);
-          term(0, 0);
-        } else {
-          term(0, 2);
-          term(0, 1);
-          term(0, 0);
-        }
+      for (int j = 0; j < FN; ++j) {
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, b[j][pb]),
+                                                         __builtin_bit_cast(bf16x8, a[pa]), acc[j], 0, 0, 0);
+        work(t * FN + j);
       }
     }
   }
 }
 
-// acc = the tile's product over k in [k0, k1).  Two LDS buffers, one barrier a stage: the next
-// stage's loads are in flight while this one is multiplied.
+// Unit u's parts of a stage: row block u % FM of k step u / FM, and the k step's FN column blocks.
+template <class T, class LA>
+__device__ __forceinline__ void read_a(const u32x4* __restrict__ s, int ra, int u, u32x4 (&a)[LA::PLANES]) {
+  const int kh = 2 * (u / T::FM) + ((threadIdx.x & 63) >> 5);
+#pragma unroll
+  for (int p = 0; p < LA::PLANES; ++p) a[p] = s[(p * (T::BK / 8) + kh) * LA::PITCH + ra + 32 * (u % T::FM)];
+}
+template <class T, class LB>
+__device__ __forceinline__ void read_b(const u32x4* __restrict__ s, int rb, int step, u32x4 (&b)[T::FN][LB::PLANES]) {
+  const int kh = 2 * step + ((threadIdx.x & 63) >> 5);
+#pragma unroll
+  for (int p = LB::PLANES - 1; p >= 0; --p)
+#pragma unroll
+    for (int j = 0; j < T::FN; ++j) b[j][p] = s[(p * (T::BK / 8) + kh) * LB::PITCH + rb + 32 * j];
+}
+
+// A whole stage, its fragments read one unit ahead.
+template <class T, class LA, class LB, bool FP32, class Work>
+__device__ __forceinline__ void product_stage(const u32x4* __restrict__ sa, const u32x4* __restrict__ sb, int ra,
+                                              int rb, acc32 (&acc)[T::FM][T::FN], Work work) {
+  constexpr int UNITS = T::BK / 16 * T::FM;
+  u32x4 a[2][LA::PLANES], b[2][T::FN][LB::PLANES];
+  read_a<T, LA>(sa, ra, 0, a[0]);
+  read_b<T, LB>(sb, rb, 0, b[0]);
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    if (u + 1 < UNITS) {
+      if (u % T::FM == T::FM - 1) read_b<T, LB>(sb, rb, u / T::FM + 1, b[(u / T::FM + 1) & 1]);
+      read_a<T, LA>(sa, ra, u + 1, a[(u + 1) & 1]);
+    }
+    product_unit<T::FN, LA, LB, FP32>(a[u & 1], b[u / T::FM & 1], acc[u % T::FM], [&](int g) { work(u * T::FN * terms<LA>() + g); });
+  }
+}
+
+// acc += the tile's product over k in [k0, k1).  Two LDS buffers, one barrier a stage.  While stage t is
+// multiplied, t + 1 goes from registers to the other buffer, each operand as soon as it may, and its
+// registers take the loads of t + 2, which so have most of a stage to arrive.
 template <class T, class LA, class LB, bool FP32>
 __device__ __forceinline__ void product_loop(const ProductOperand& A, const ProductOperand& B, int m0, int n0,
                                              int64_t k0, int64_t k1, u32x4* __restrict__ smem,
                                              acc32 (&acc)[T::FM][T::FN]) {
-  constexpr int STAGE = LA::UNITS + LB::UNITS;
+  constexpr int STAGE = LA::UNITS + LB::UNITS, PIECES = SplitUnit<FP32>::PIECES;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int ra = wave / T::WN * (T::FM * 32) + (lane & 31), rb = wave % T::WN * (T::FN * 32) + (lane & 31);
-#pragma unroll
-  for (int i = 0; i < T::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < T::FN; ++j) acc[i][j] = acc32{};
   LA la;
   LB lb;
   la.init(A, m0, k0);
   lb.init(B, n0, k0);
+  SplitUnit<FP32> ua, ub;
   const int full = (int)((k1 - k0) / T::BK), left = (int)((k1 - k0) % T::BK), n = full + (left > 0);
   auto load = [&](int t) {
     if (t < full) {
       la.load();
       lb.load();
-    } else {
+    } else if (t < n) {
       la.load_tail(left);
       lb.load_tail(left);
     }
   };
+  auto piece = [&](int k, u32x4* __restrict__ s) {  // A's, then B's
+    if (k < PIECES)
+      la.piece(k, ua, s);
+    else
+      lb.piece(k - PIECES, ub, s + LA::UNITS);
+  };
   auto store = [&](int t) {
-    u32x4* s = smem + (t & 1) * STAGE;
-    la.template store<FP32>(s);
-    lb.template store<FP32>(s + LA::UNITS);
+#pragma unroll
+    for (int k = 0; k < 2 * PIECES; ++k) piece(k, smem + (t & 1) * STAGE);
   };
   if (n == 0) return;
   load(0);
   store(0);
+  load(1);
   __syncthreads();
-  for (int t = 0; t < n; ++t) {
-    if (t + 1 < n) load(t + 1);
-    const u32x4* s = smem + (t & 1) * STAGE;
-    product_stage<T, LA, LB, FP32>(s, s + LA::UNITS, ra, rb, acc);
+  int t = 0;
+  if constexpr (!FP32) {
+    // A stage whose next two are full ones: without a branch, its other work among its matrix
+    // instructions, a piece each from a sixth of them on
+    constexpr int GROUPS = T::BK / 16 * T::FM * T::FN * terms<LA>(), FIRST = GROUPS / 6;
+    constexpr int EVERY = (GROUPS - FIRST) / (2 * PIECES) > 1 ? (GROUPS - FIRST) / (2 * PIECES) : 1;
+    for (; t + 2 < full; ++t) {
+      const u32x4* rd = smem + (t & 1) * STAGE;
+      u32x4* wr = smem + ((t + 1) & 1) * STAGE;
+      product_stage<T, LA, LB, false>(rd, rd + LA::UNITS, ra, rb, acc, [&](int g) {
+#pragma unroll
+        for (int k = 0; k < 2 * PIECES; ++k)
+          if (min(FIRST + k * EVERY, GROUPS - 1) == g) {
+            piece(k, wr);
+            if (k == PIECES - 1) la.load();
+            if (k == 2 * PIECES - 1) lb.load();
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      __syncthreads();
+    }
+  }
+  for (; t < n; ++t) {
     if (t + 1 < n) store(t + 1);
+    load(t + 2);
+    const u32x4* s = smem + (t & 1) * STAGE;
+    product_stage<T, LA, LB, FP32>(s, s + LA::UNITS, ra, rb, acc, [](int) {});
     __syncthreads();
   }
 }
 
-// The product, again on the fp32 instructions if it holds a NaN.
+// The product, again on the fp32 instructions if it holds what is not finite.
 template <class T, class LA, class LB>
 __device__ __forceinline__ void product(const ProductOperand& A, const ProductOperand& B, int m0, int n0, int64_t k0,
                                         int64_t k1, u32x4* __restrict__ smem, acc32 (&acc)[T::FM][T::FN]) {
-  product_loop<T, LA, LB, false>(A, B, m0, n0, k0, k1, smem, acc);
-  bool nan = false;
+  auto run = [&](auto fp32) {
+#pragma unroll
+    for (int i = 0; i < T::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < T::FN; ++j) acc[i][j] = acc32{};
+    product_loop<T, LA, LB, decltype(fp32)::value>(A, B, m0, n0, k0, k1, smem, acc);
+  };
+  run(std::false_type());
+  bool off = false;
 #pragma unroll
   for (int i = 0; i < T::FM; ++i)
 #pragma unroll
     for (int j = 0; j < T::FN; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) nan |= acc[i][j][r] != acc[i][j][r];
-  if (__syncthreads_or(nan)) product_loop<T, LA, LB, true>(A, B, m0, n0, k0, k1, smem, acc);
+      for (int r = 0; r < 16; ++r) {
+        off |= !(fabsf(acc[i][j][r]) < __builtin_inff());
+        if (LA::SCALE != 1.0f) acc[i][j][r] = acc[i][j][r] * LA::SCALE;
+      }
+  if (__syncthreads_or(off)) run(std::true_type());
 }
 
 }  // namespace
