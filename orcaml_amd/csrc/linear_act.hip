@@ -218,6 +218,20 @@ __device__ __forceinline__ void finish_bias(const BackwardArgs& p, int block, fl
   }
 }
 
+#include "row_product.hpp"
+
+// The same with dX on tiles of 64 and dW for a few rows.
+template <class T, int MR>
+__global__ void __launch_bounds__(256, T::OCC) row_backward_kernel(BackwardArgs p) {
+  static_assert(T::THREADS == 256, "row_dw's block");
+  __shared__ u32x4 smem[tile_units<T, LoadKFast, LoadKFast>()];
+  const int block = blockIdx.x;
+  if (block < p.dx_blocks)
+    tile_product<T, LoadKFast, LoadKFast>(p.dx, block, p.dx_blocks, smem);
+  else
+    row_dw<MR>(p.dw, block - p.dx_blocks, reinterpret_cast<float*>(smem));
+}
+
 template <class T, template <int, int, int> class LoadX>
 __global__ void __launch_bounds__(T::THREADS, T::OCC* T::THREADS / 256) linear_act_backward_kernel(BackwardArgs p) {
   __shared__ u32x4 smem[tile_units<T, LoadKFast, LoadKFast>()];  // the larger of the two products'
@@ -343,11 +357,12 @@ constexpr TileCost kTileCosts[2][3] = {
      {128, 32, 1, 5.4, 0.765, 2.93, 0.819, 1.42, 2.2, 3.2e6},
      {256, 16, 1, 9.7, 1.031, 8.29, 1.031, 8.29, 0.0, 4.3e6}}};
 
-// Tiles and splits of `p`'s product.
-Plan plan_product(orca_hip_ctx* ctx, ProductArgs& p, bool codes, const char* op) {
+// Tiles and splits of `p`'s product (of tiles of `only`, if that is given).
+Plan plan_product(orca_hip_ctx* ctx, ProductArgs& p, bool codes, const char* op, int only = 0) {
   Plan best;
   double best_us = 0.0;
   for (const TileCost& c : kTileCosts[codes]) {
+    if (only && c.tile != only) continue;
     const int64_t tm = (p.M + c.tile - 1) / c.tile, tn = (p.N + c.tile - 1) / c.tile;
     if (tm > 0x3fffffff / tn) continue;
     for (int64_t splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
@@ -374,6 +389,23 @@ Plan plan_product(orca_hip_ctx* ctx, ProductArgs& p, bool codes, const char* op)
   }
   if (!best.tile) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
   return best;
+}
+
+// Forward of a few rows: a block for 16 columns, k split so that the blocks cover the CUs.  A checkpoint's group
+// of 32 columns then lies in two blocks, so with one the split products' finish writes it.
+Plan plan_rows(orca_hip_ctx* ctx, ProductArgs& p, const char* op) {
+  Plan q;
+  const int64_t tn = (p.N + kRowCols - 1) / kRowCols;
+  if (tn > 0x7fffffff / 64) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
+  const bool packs = p.out.pre8.codes || p.out.y8.codes;
+  const int64_t splits = std::max<int64_t>(packs ? 2 : 1, std::min<int64_t>({ctx->num_cus / tn, p.K / 512, 32}));
+  p.chunk = std::max<int64_t>(1, (p.K + splits - 1) / splits);
+  p.splits = (int)std::max<int64_t>(packs ? 2 : 1, (p.K + p.chunk - 1) / p.chunk);
+  p.tiles_m = 1;
+  p.tiles_n = (int)tn;
+  q.blocks = tn * p.splits;
+  if (p.splits > 1) q.ws = (size_t)p.splits * p.M * p.N;
+  return q;
 }
 
 int64_t finish_blocks(const ProductArgs& p, const Plan& q) {
@@ -491,7 +523,8 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
     p.N = (int64_t)N;
     p.K = (int64_t)K;
     p.out = o;
-    const Plan q = plan_product(ctx, p, false, op);
+    const bool few = M <= 4;
+    const Plan q = few ? plan_rows(ctx, p, op) : plan_product(ctx, p, false, op);
     std::unique_ptr<Scratch> ws;
     if (q.ws) {
       ws.reset(new Scratch(ctx, sizeof(float) * q.ws));
@@ -502,7 +535,10 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
       pname = std::string(op) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
     ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K, 4.0 * ((double)M * K + (double)K * N + (double)M * N));
     const dim3 grid((unsigned)q.blocks);
-    if (q.tile == 256)
+    if (few)
+      hipLaunchKernelGGL(M == 1 ? row_forward_kernel<1> : row_forward_kernel<4>, grid, dim3(kRowWaves * 64), 0,
+                         ctx->stream, p);
+    else if (q.tile == 256)
       hipLaunchKernelGGL(linear_act_kernel<Tile256>, grid, dim3(Tile256::THREADS), 0, ctx->stream, p);
     else if (q.tile == 128)
       hipLaunchKernelGGL(linear_act_kernel<Tile128>, grid, dim3(Tile128::THREADS), 0, ctx->stream, p);
@@ -568,25 +604,26 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     // 64 rows a block, 16 where that leaves CUs without one
     const bool tall = ((int64_t)M + 63) / 64 * (((int64_t)N + 255) / 256) >= ctx->num_cus;
     const int64_t rows = tall ? 64 : 16, blocks = ((int64_t)M + rows - 1) / rows;
+    const bool few = M && M <= (size_t)kRowsDw && want_dw, direct = blocks == 1;  // direct: a block's column sums are db
     if (N && (want_db || (slope && (want_dx || want_dw)))) {
       if (slope && M) {
         dzs.reset(new Scratch(ctx, sizeof(float) * M * N));
         dz = dzs->as<float>();
         lddz = (int64_t)N;
       }
-      if (want_db && M) partial.reset(new Scratch(ctx, sizeof(float) * (size_t)blocks * N));
+      if (want_db && M && !direct) partial.reset(new Scratch(ctx, sizeof(float) * (size_t)blocks * N));
       if (M) {
         ProfScope prof(ctx, "linear_act_slope", 0.0, (slope ? 12.0 : 4.0) * M * N);
         hipLaunchKernelGGL(tall ? slope_kernel<16> : slope_kernel<4>, quad_grid((int64_t)M, rows, (int64_t)N, op),
                            dim3(256), 0, ctx->stream, dY, (int64_t)lddy, s.act, static_cast<const float*>(z.p),
                            (int64_t)s.ldz, act8_at(const_cast<void*>(z8.p), M, N), dzs ? dzs->as<float>() : nullptr,
-                           partial ? partial->as<float>() : nullptr, (int64_t)M, (int64_t)N);
+                           want_db && direct ? db : partial ? partial->as<float>() : nullptr, (int64_t)M, (int64_t)N);
         ORCA_HIP_CHECK(hipGetLastError());
       }
     }
     BackwardArgs b{};
     b.N = (int64_t)N;
-    if (want_db) {
+    if (want_db && !direct) {
       b.db = db;
       b.partial = partial ? partial->as<float>() : nullptr;
       b.partials = M ? blocks : 0;
@@ -602,7 +639,7 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
       b.dx.out.ldr = (int64_t)s.ldadd;
       b.dx.out.y = dX;
       b.dx.out.ldy = (int64_t)lddx;
-      qx = plan_product(ctx, b.dx, false, op);
+      qx = plan_product(ctx, b.dx, false, op, few ? 64 : 0);
     }
     if (want_dw) {
       b.dw.A = ProductOperand{s.x, (int64_t)s.ldx, (int)K, nullptr, 0};
@@ -616,7 +653,10 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
       b.dw.K = (int64_t)M;
       b.dw.out.y = dW;
       b.dw.out.ldy = (int64_t)lddw;
-      qw = plan_product(ctx, b.dw, s.x8 != nullptr, op);
+      if (few)
+        qw.blocks = ((int64_t)K + kRowDw - 1) / kRowDw * (((int64_t)N + 255) / 256);
+      else
+        qw = plan_product(ctx, b.dw, s.x8 != nullptr, op);
     }
     std::unique_ptr<Scratch> ws;
     if (qx.ws + qw.ws) {
@@ -624,7 +664,9 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
       b.dx.ws = ws->as<float>();
       b.dw.ws = ws->as<float>() + qx.ws;
     }
-    if (!qx.tile && !qw.tile && !b.db) return;
+    const int64_t grid = qx.blocks + qw.blocks + (b.db ? ((int64_t)N + 31) / 32 : 0);
+    if (grid > 0x7fffffff) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
+    if (!grid) return;
     std::string pname;
     if (ctx->prof.enabled)
       pname = std::string(op) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
@@ -633,7 +675,11 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     const bool codes = s.x8 != nullptr, one = !qx.tile || !qw.tile || qx.tile == qw.tile;
     b.dx_blocks = (int)qx.blocks;
     b.dw_blocks = (int)qw.blocks;
-    if (one) {
+    if (few) {
+      hipLaunchKernelGGL((M <= 4 ? row_backward_kernel<Tile64, 4> : row_backward_kernel<Tile64, 16>),
+                         dim3((unsigned)grid), dim3(256), 0, ctx->stream, b);
+      ORCA_HIP_CHECK(hipGetLastError());
+    } else if (one) {
       launch_backward(ctx, std::max(std::max(qx.tile, qw.tile), 64), codes, b);
     } else {  // the bias gradient goes with the first
       BackwardArgs only = b;
