@@ -339,10 +339,10 @@ struct Plan {
   size_t ws = 0;      // floats of partial products
 };
 
-// Microseconds of a product on a tile with its k range split, on an otherwise idle GPU of 256 CUs:
-// fitted to 7700 products of 1 .. 8192 x 16 .. 4096 x 16 .. 4096, each timed with every tile and split
-// (8 % rms near the best ones; the choice by it takes 1.7 % longer than the best, 11 % in one case of
-// twenty).  A launch; then the CU with the most blocks, `together` of them at a time: a stage's chain of
+// Microseconds of products on tiles with their k ranges split, on an otherwise idle GPU of 256 CUs: fitted
+// to 7700 products of 1 .. 8192 x 16 .. 4096 x 16 .. 4096, each timed with every tile and split (8 %
+// rms near the best ones; the choice by it takes 1.7 % longer than the best, 11 % in one case of twenty).
+// A launch; then the CU with the most blocks, `together` of them at a time: a stage's chain of
 // waits, or its throughput; with splits the second launch, which reads and writes them.
 struct TileCost {
   int tile, bk, together;
@@ -357,38 +357,71 @@ constexpr TileCost kTileCosts[2][3] = {
      {128, 32, 1, 5.4, 0.765, 2.93, 0.819, 1.42, 2.2, 3.2e6},
      {256, 16, 1, 9.7, 1.031, 8.29, 1.031, 8.29, 0.0, 4.3e6}}};
 
-// Tiles and splits of `p`'s product (of tiles of `only`, if that is given).
-Plan plan_product(orca_hip_ctx* ctx, ProductArgs& p, bool codes, const char* op, int only = 0) {
-  Plan best;
-  double best_us = 0.0;
-  for (const TileCost& c : kTileCosts[codes]) {
-    if (only && c.tile != only) continue;
-    const int64_t tm = (p.M + c.tile - 1) / c.tile, tn = (p.N + c.tile - 1) / c.tile;
-    if (tm > 0x3fffffff / tn) continue;
-    for (int64_t splits : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      if (splits > 1 && (p.K < 48 * splits || tm * tn * splits > 8 * ctx->num_cus)) break;
-      // even runs of a multiple of every stage's k values
-      const int64_t chunk = std::max<int64_t>(64, ((p.K + splits - 1) / splits + 63) / 64 * 64);
-      const int64_t n = std::max<int64_t>(1, (p.K + chunk - 1) / chunk);
-      if (splits > 1 && n == 1) continue;
-      const int64_t per_cu = (tm * tn * n + ctx->num_cus - 1) / ctx->num_cus;
-      const double stages = (double)((std::min(chunk, p.K) + c.bk - 1) / c.bk);
-      double us = c.launch + std::max((double)((per_cu + c.together - 1) / c.together) * (stages * c.chain + c.block),
-                                      (double)per_cu * (stages * c.stage + c.each));
-      if (n > 1) us += c.finish + 4.0 * (double)(n + 1) * (double)p.M * (double)p.N / c.bytes_per_us;
-      if (best.tile && us >= best_us) continue;
-      best_us = us;
-      best.tile = c.tile;
-      best.blocks = tm * tn * n;
-      best.ws = n > 1 ? (size_t)n * p.M * p.N : 0;
-      p.tiles_m = (int)tm;
-      p.tiles_n = (int)tn;
-      p.splits = (int)n;
-      p.chunk = chunk;
-    }
+// One way to cut a product.
+struct Cut {
+  int64_t tm, tn, splits, chunk, blocks;
+  double chain, work, finish;  // us of a block alone, of a block among others, of the second launch
+  double launch;
+  int together;
+};
+constexpr int kMaxCuts = 10;
+int cuts_of(orca_hip_ctx* ctx, const ProductArgs& p, bool codes, int tile, Cut (&out)[kMaxCuts]) {
+  const TileCost& c = kTileCosts[codes][tile];
+  const int64_t tm = (p.M + c.tile - 1) / c.tile, tn = (p.N + c.tile - 1) / c.tile;
+  int n = 0;
+  if (tm > 0x3fffffff / tn) return 0;
+  for (int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+    if (want > 1 && (p.K < 48 * want || tm * tn * want > 8 * ctx->num_cus)) break;
+    // even runs of a multiple of every stage's k values
+    const int64_t chunk = std::max<int64_t>(64, ((p.K + want - 1) / want + 63) / 64 * 64);
+    const int64_t splits = std::max<int64_t>(1, (p.K + chunk - 1) / chunk);
+    if (want > 1 && splits == 1) continue;
+    const double stages = (double)((std::min(chunk, p.K) + c.bk - 1) / c.bk);
+    const double finish =
+        splits > 1 ? c.finish + 4.0 * (double)(splits + 1) * (double)p.M * (double)p.N / c.bytes_per_us : 0.0;
+    out[n++] = Cut{tm, tn, splits, chunk, tm * tn * splits, stages * c.chain + c.block, stages * c.stage + c.each,
+                   finish, c.launch, c.together};
   }
-  if (!best.tile) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
-  return best;
+  return n;
+}
+Plan take(ProductArgs& p, int tile, const Cut& c) {
+  p.tiles_m = (int)c.tm;
+  p.tiles_n = (int)c.tn;
+  p.splits = (int)c.splits;
+  p.chunk = c.chunk;
+  return Plan{kTileCosts[0][tile].tile, c.blocks, c.splits > 1 ? (size_t)c.splits * p.M * p.N : 0};
+}
+
+// The tile and the cuts of a product, or of two that share a launch (on one tile; `only`: that of this size).
+void plan_products(orca_hip_ctx* ctx, ProductArgs* a, Plan* qa, ProductArgs* b, Plan* qb, bool b_codes, const char* op,
+                   int only = 0) {
+  double best = 0.0;
+  int best_tile = -1;
+  Cut best_a{}, best_b{};
+  for (int tile = 0; tile < 3; ++tile) {
+    if (only && kTileCosts[0][tile].tile != only) continue;
+    Cut ca[kMaxCuts] = {}, cb[kMaxCuts] = {};
+    const int na = a ? cuts_of(ctx, *a, false, tile, ca) : 1, nb = b ? cuts_of(ctx, *b, b_codes, tile, cb) : 1;
+    for (int i = 0; i < na; ++i)
+      for (int j = 0; j < nb; ++j) {
+        const Cut &x = ca[i], &y = cb[j];
+        const int64_t blocks = x.blocks + y.blocks, per_cu = (blocks + ctx->num_cus - 1) / ctx->num_cus;
+        const int together = std::max(x.together, y.together);
+        // each CU's blocks are of both kinds, in proportion
+        const double work = ((double)x.blocks * x.work + (double)y.blocks * y.work) / (double)blocks;
+        const double us = std::max(x.launch, y.launch) + x.finish + y.finish +
+                          std::max((double)((per_cu + together - 1) / together) * std::max(x.chain, y.chain),
+                                   (double)per_cu * work);
+        if (best_tile >= 0 && us >= best) continue;
+        best = us;
+        best_tile = tile;
+        best_a = x;
+        best_b = y;
+      }
+  }
+  if (best_tile < 0) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
+  if (a) *qa = take(*a, best_tile, best_a);
+  if (b) *qb = take(*b, best_tile, best_b);
 }
 
 // Forward of a few rows: a block for 16 columns, k split so that the blocks cover the CUs.  A checkpoint's group
@@ -429,13 +462,12 @@ void launch_backward(orca_hip_ctx* ctx, bool codes, unsigned grid, const Backwar
     hipLaunchKernelGGL((linear_act_backward_kernel<T, LoadKSlow>), dim3(grid), dim3(T::THREADS), 0, ctx->stream, b);
   ORCA_HIP_CHECK(hipGetLastError());
 }
-void launch_backward(orca_hip_ctx* ctx, int tile, bool codes, const BackwardArgs& b) {
-  const unsigned grid = (unsigned)(b.dx_blocks + b.dw_blocks + (b.db ? (b.N + 31) / 32 : 0));
+void launch_backward(orca_hip_ctx* ctx, int tile, bool codes, unsigned grid, const BackwardArgs& b) {
   if (tile == 256)
     launch_backward<Tile256>(ctx, codes, grid, b);
   else if (tile == 128)
     launch_backward<Tile128>(ctx, codes, grid, b);
-  else
+  else  // also where only the bias gradient is left to finish
     launch_backward<Tile64>(ctx, codes, grid, b);
 }
 
@@ -524,7 +556,11 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
     p.K = (int64_t)K;
     p.out = o;
     const bool few = M <= 4;
-    const Plan q = few ? plan_rows(ctx, p, op) : plan_product(ctx, p, false, op);
+    Plan q;
+    if (few)
+      q = plan_rows(ctx, p, op);
+    else
+      plan_products(ctx, &p, &q, nullptr, nullptr, false, op);
     std::unique_ptr<Scratch> ws;
     if (q.ws) {
       ws.reset(new Scratch(ctx, sizeof(float) * q.ws));
@@ -639,7 +675,6 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
       b.dx.out.ldr = (int64_t)s.ldadd;
       b.dx.out.y = dX;
       b.dx.out.ldy = (int64_t)lddx;
-      qx = plan_product(ctx, b.dx, false, op, few ? 64 : 0);
     }
     if (want_dw) {
       b.dw.A = ProductOperand{s.x, (int64_t)s.ldx, (int)K, nullptr, 0};
@@ -653,11 +688,11 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
       b.dw.K = (int64_t)M;
       b.dw.out.y = dW;
       b.dw.out.ldy = (int64_t)lddw;
-      if (few)
-        qw.blocks = ((int64_t)K + kRowDw - 1) / kRowDw * (((int64_t)N + 255) / 256);
-      else
-        qw = plan_product(ctx, b.dw, s.x8 != nullptr, op);
     }
+    if (want_dx || (want_dw && !few))
+      plan_products(ctx, want_dx ? &b.dx : nullptr, &qx, want_dw && !few ? &b.dw : nullptr, &qw, s.x8 != nullptr, op,
+                    few ? Tile64::BM : 0);
+    if (few) qw.blocks = ((int64_t)K + kRowDw - 1) / kRowDw * (((int64_t)N + 255) / 256);
     std::unique_ptr<Scratch> ws;
     if (qx.ws + qw.ws) {
       ws.reset(new Scratch(ctx, sizeof(float) * (qx.ws + qw.ws)));
@@ -672,23 +707,14 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
       pname = std::string(op) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
     ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K * (want_dx + want_dw),
                    4.0 * ((double)M * N + (want_dx + want_dw) * ((double)M * K + (double)K * N)));
-    const bool codes = s.x8 != nullptr, one = !qx.tile || !qw.tile || qx.tile == qw.tile;
     b.dx_blocks = (int)qx.blocks;
     b.dw_blocks = (int)qw.blocks;
     if (few) {
       hipLaunchKernelGGL((M <= 4 ? row_backward_kernel<Tile64, 4> : row_backward_kernel<Tile64, 16>),
                          dim3((unsigned)grid), dim3(256), 0, ctx->stream, b);
       ORCA_HIP_CHECK(hipGetLastError());
-    } else if (one) {
-      launch_backward(ctx, std::max(std::max(qx.tile, qw.tile), 64), codes, b);
-    } else {  // the bias gradient goes with the first
-      BackwardArgs only = b;
-      only.dw_blocks = 0;
-      launch_backward(ctx, qx.tile, codes, only);
-      only.dx_blocks = 0;
-      only.dw_blocks = b.dw_blocks;
-      only.db = nullptr;
-      launch_backward(ctx, qw.tile, codes, only);
+    } else {
+      launch_backward(ctx, std::max(qx.tile, qw.tile), s.x8 != nullptr, (unsigned)grid, b);
     }
     launch_finish(ctx, b.dx, qx, b.dw, qw, op);
   });
