@@ -29,6 +29,7 @@
 #include <cstdint>
 
 #include "act8.hpp"
+#include "activation.hpp"
 #include "slab.hpp"
 
 namespace orca_hip {
@@ -48,6 +49,11 @@ struct ProductOperand {
   int rows;
   const uint8_t* scales;  // 8-bit: step bytes [rows / 32][lds]
   int64_t lds;
+  // LoadSlopeFast, LoadSlopeSlow: the operand is p * act'(z), z of p's shape, in fp32 or as a checkpoint
+  int act;
+  const float* z;
+  int64_t ldz;
+  Act8 z8;
 };
 
 __device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) {
@@ -226,6 +232,128 @@ struct LoadCodes {
       u.ra = __uint_as_float(value(k));
     else
       u.h[k / 2] = upper_halves(__float_as_uint(u.ra), value(k));
+  }
+};
+
+// dz = dy * act'(z) on its way into a product, for backwards too small to make it in a launch of its own.  The
+// slopes of a unit are taken with its first piece.
+struct SlopeUnit {
+  float v[8];
+  uint32_t z[8];  // fp32 bits, or a code in the lowest byte and its step byte above
+};
+__device__ __forceinline__ float slope_code(uint32_t z) { return (float)(int8_t)z * act8_step(z >> 8); }
+
+// k (dy's columns) is contiguous.  8 columns from a multiple of 8 on lie in one group of a checkpoint.
+template <int ROWS, int BK, int THREADS>
+struct LoadSlopeFast {
+  static constexpr float SCALE = 1.0f;
+  static constexpr int PLANES = 3, KH = BK / 8, PITCH = unit_pitch(ROWS, KH), UNITS = PLANES * KH * PITCH;
+  static_assert(ROWS * KH == THREADS, "a unit per thread");
+  const float* p;
+  const float* z;
+  const int8_t* codes;
+  const uint8_t* scales;
+  int64_t lds;
+  int64_t k;
+  int act;
+  SlopeUnit u;
+
+  __device__ __forceinline__ void init(const ProductOperand& op, int row0, int64_t k0) {
+    const int64_t row = min(row0 + (int)threadIdx.x / KH, op.rows - 1);
+    k = k0 + threadIdx.x % KH * 8;
+    act = op.act;
+    p = static_cast<const float*>(op.p) + row * op.ld + k;
+    z = op.z + row * op.ldz + k;
+    codes = op.z8.codes ? op.z8.codes + row * op.z8.cols + k : nullptr;
+    scales = op.z8.scales + row;
+    lds = op.z8.ld;
+  }
+  __device__ __forceinline__ void load() { fetch<false>(BK); }
+  __device__ __forceinline__ void load_tail(int left) { fetch<true>(left); }
+  template <bool TAIL>
+  __device__ __forceinline__ void fetch(int left) {
+    left -= threadIdx.x % KH * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u.v[j] = !TAIL || j < left ? p[j] : 0.0f;
+    if (act != ORCA_HIP_ACT_NONE && codes) {
+      const uint32_t step = !TAIL || left > 0 ? scales[k / (int64_t)kAct8Group * lds] : 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u.z[j] = !TAIL || j < left ? (uint8_t)codes[j] | step << 8 : 0u;
+      codes += BK;
+    } else if (act != ORCA_HIP_ACT_NONE) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u.z[j] = !TAIL || j < left ? __float_as_uint(z[j]) : 0u;
+      z += BK;
+    }
+    p += BK;
+    k += BK;
+  }
+  template <bool SAFE>
+  __device__ __forceinline__ void piece(int i, SplitUnit<SAFE>& unit, u32x4* s) {
+    if (i == 0 && act != ORCA_HIP_ACT_NONE) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = codes ? slope_code(u.z[j]) : __uint_as_float(u.z[j]);
+      activation_slopes<8>(act, f, u.v);
+    }
+    unit.piece(i, u.v, s + threadIdx.x % KH * PITCH + threadIdx.x / KH, KH * PITCH);
+  }
+};
+
+// k values are dy's rows.
+template <int ROWS, int BK, int THREADS>
+struct LoadSlopeSlow {
+  static constexpr float SCALE = 1.0f;
+  static constexpr int PLANES = 3, KH = BK / 8, PITCH = unit_pitch(ROWS, KH), UNITS = PLANES * KH * PITCH;
+  static_assert(ROWS * KH == THREADS && ROWS % 64 == 0, "a unit per thread, whole waves per k");
+  const float* p;
+  const float* z;
+  const int8_t* codes;
+  const uint8_t* scales;
+  int64_t ld, ldz, ldc;
+  int act;
+  SlopeUnit u;
+
+  __device__ __forceinline__ void init(const ProductOperand& op, int row0, int64_t k0) {
+    const int64_t col = min(row0 + (int)threadIdx.x % ROWS, op.rows - 1), k = k0 + threadIdx.x / ROWS * 8;
+    act = op.act;
+    ld = op.ld;
+    ldz = op.ldz;
+    ldc = op.z8.cols;
+    p = static_cast<const float*>(op.p) + k * ld + col;
+    z = op.z + k * ldz + col;
+    codes = op.z8.codes ? op.z8.codes + k * ldc + col : nullptr;
+    scales = op.z8.scales + col / (int64_t)kAct8Group * op.z8.ld + k;
+  }
+  __device__ __forceinline__ void load() { fetch<false>(BK); }
+  __device__ __forceinline__ void load_tail(int left) { fetch<true>(left); }
+  template <bool TAIL>
+  __device__ __forceinline__ void fetch(int left) {
+    left -= threadIdx.x / ROWS * 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u.v[j] = !TAIL || j < left ? p[j * ld] : 0.0f;
+    if (act != ORCA_HIP_ACT_NONE && codes) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        u.z[j] = !TAIL || j < left ? (uint8_t)codes[j * ldc] | (uint32_t)scales[j] << 8 : 0u;
+      codes += BK * ldc;
+      scales += BK;
+    } else if (act != ORCA_HIP_ACT_NONE) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u.z[j] = !TAIL || j < left ? __float_as_uint(z[j * ldz]) : 0u;
+      z += BK * ldz;
+    }
+    p += BK * ld;
+  }
+  template <bool SAFE>
+  __device__ __forceinline__ void piece(int i, SplitUnit<SAFE>& unit, u32x4* s) {
+    if (i == 0 && act != ORCA_HIP_ACT_NONE) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = codes ? slope_code(u.z[j]) : __uint_as_float(u.z[j]);
+      activation_slopes<8>(act, f, u.v);
+    }
+    unit.piece(i, u.v, s + threadIdx.x / ROWS * PITCH + threadIdx.x % ROWS, KH * PITCH);
   }
 };
 
