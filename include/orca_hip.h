@@ -650,12 +650,14 @@ int orca_hip_relu_bw_colsum_noalloc(orca_hip_ctx* ctx, const float* grad, const 
  *
  * Products here read fp32 and give fp32 precision (each operand is taken apart into three bf16
  * terms that add up to it; sums are fp32), on the bf16 matrix instructions.  Their sums run in
- * another order than orca_hip_gemm's.  Infinities and NaN come out as from fp32 products.
- * Sizes are below 2^31 each and may be 0; leading dimensions count elements; fp32 operands
+ * another order than orca_hip_gemm's.  Infinities and NaN come out as from fp32 products; magnitudes
+ * below 2^-100 keep fewer bits, and below 2^-126 none.
+ * Sizes are below 2^30 each and may be 0; leading dimensions count elements; fp32 operands
  * need no alignment beyond a float's.  A call may not write what it reads, or overlap two results,
- * except as said below.  Work is enqueued on the context stream; workspaces come from the
- * context's allocator, so these calls fail while launches go to the side stream, and under
- * stream capture unless a call of the same sizes ran before. */
+ * except as said below (columns of one matrix beside each other, given with its leading dimension,
+ * do not overlap).  Work is enqueued on the context stream; workspaces come from the context's
+ * allocator, so a call that needs one fails while launches go to the side stream and under stream
+ * capture. */
 #define ORCA_HIP_ACT_NONE 0
 #define ORCA_HIP_ACT_RELU 1      /* z > 0 ? z : 0 */
 #define ORCA_HIP_ACT_GELU 2      /* z * (1 + erf(z / sqrt 2)) / 2 */

@@ -390,18 +390,23 @@ struct Cut {
   double launch;
   int together;
 };
-constexpr int kMaxCuts = 10;
+constexpr int kMaxCuts = 13;
 int cuts_of(orca_hip_ctx* ctx, const ProductArgs& p, bool codes, int tile, Cut (&out)[kMaxCuts]) {
   const TileCost& c = kTileCosts[codes][tile];
   const int64_t tm = (p.M + c.tile - 1) / c.tile, tn = (p.N + c.tile - 1) / c.tile;
   int n = 0;
   if (tm > 0x3fffffff / tn) return 0;
-  for (int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-    if (want > 1 && (p.K < 48 * want || tm * tn * want > 8 * ctx->num_cus)) break;
+  for (int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128, 256}) {
+    if (ctx->linear_splits) {  // that many, as far as k goes
+      if (want > 1) break;
+      want = ctx->linear_splits;
+    } else if (want > 1 && (p.K < 48 * want || tm * tn * want > 8 * ctx->num_cus)) {
+      break;
+    }
     // even runs of a multiple of every stage's k values
     const int64_t chunk = std::max<int64_t>(64, ((p.K + want - 1) / want + 63) / 64 * 64);
     const int64_t splits = std::max<int64_t>(1, (p.K + chunk - 1) / chunk);
-    if (want > 1 && splits == 1) continue;
+    if (want > 1 && splits == 1 && n) continue;
     const double stages = (double)((std::min(chunk, p.K) + c.bk - 1) / c.bk);
     const double finish =
         splits > 1 ? c.finish + 4.0 * (double)(splits + 1) * (double)p.M * (double)p.N / c.bytes_per_us : 0.0;
@@ -421,6 +426,7 @@ Plan take(ProductArgs& p, int tile, const Cut& c) {
 // The tile and the cuts of a product, or of two that share a launch (on one tile; `only`: that of this size).
 void plan_products(orca_hip_ctx* ctx, ProductArgs* a, Plan* qa, ProductArgs* b, Plan* qb, bool b_codes, const char* op,
                    int only = 0) {
+  if (ctx->linear_tile) only = ctx->linear_tile;
   double best = 0.0;
   int best_tile = -1;
   Cut best_a{}, best_b{};
@@ -505,22 +511,41 @@ constexpr size_t kInsideRows = 512;
 constexpr double kInsideWork = 2.5e7, kInsideWorkPlain = 3e8;
 
 void check_ld(const char* what, size_t ld, size_t cols) {
+  if (ld > (size_t(1) << 40)) fail_shape(what, "a leading dimension of at most 2^40", std::to_string(ld));
   if (ld < cols) fail_shape(what, "a leading dimension of at least " + std::to_string(cols), std::to_string(ld));
 }
 void check_sizes(const char* op, size_t M, size_t N, size_t K) {
   for (size_t v : {M, N, K})
-    if (v > 0x7fffff00u) fail_shape(op, "sizes below 2^31", std::to_string(v));
+    if (v >= (size_t(1) << 30)) fail_shape(op, "sizes below 2^30", std::to_string(v));
 }
-// A result must not lie in what the call still reads (or in another result).
-void check_apart(const char* op, const void* out, size_t out_bytes, const void* in, size_t in_bytes) {
-  const auto a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in);
-  if (out && in && out_bytes && in_bytes && a < b + in_bytes && b < a + out_bytes)
-    fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": an output overlaps another operand");
-}
+// An operand's rows of `width` bytes, `ld` bytes apart (one row: a contiguous buffer).
 struct Span {
   const void* p;
-  size_t bytes;
+  size_t rows, width, ld;
+  size_t bytes() const { return rows && width ? (rows - 1) * ld + width : 0; }
 };
+Span matrix_span(const void* p, size_t rows, size_t cols, size_t ld) { return Span{p, rows, 4 * cols, 4 * ld}; }
+Span buffer_span(const void* p, size_t bytes) { return Span{p, 1, bytes, bytes}; }
+// A result must not lie in what the call reads, or in another result.  Columns of one matrix beside each
+// other (the same ld) are apart.
+void check_apart(const char* op, const Span& out, const Span& in) {
+  const auto a = reinterpret_cast<uintptr_t>(out.p), b = reinterpret_cast<uintptr_t>(in.p);
+  if (!out.p || !in.p || !out.bytes() || !in.bytes() || a >= b + in.bytes() || b >= a + out.bytes()) return;
+  if (out.ld == in.ld && out.ld) {
+    const size_t d = (a < b ? b - a : out.ld - (a - b) % out.ld) % out.ld;  // from out's columns to in's
+    if (d >= out.width && out.ld - d >= in.width) return;
+  }
+  fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": an output overlaps another operand");
+}
+// A workspace goes back to the context's allocator when the call returns: a captured graph would write
+// it at every replay, whoever has it then.
+std::unique_ptr<Scratch> workspace(orca_hip_ctx* ctx, size_t bytes, const char* op) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  ORCA_HIP_CHECK(hipStreamIsCapturing(ctx->stream, &status));
+  if (status != hipStreamCaptureStatusNone)
+    fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": needs a workspace, which a captured graph cannot keep");
+  return std::make_unique<Scratch>(ctx, bytes);
+}
 void check_act(const char* op, int act) {
   if (act < ORCA_HIP_ACT_NONE || act > ORCA_HIP_ACT_SILU)
     fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": unknown activation " + std::to_string(act));
@@ -548,28 +573,28 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
     if (e.pre) check_ld("linear_act (pre)", e.ldpre, N);
     if (M && N && (!Y || (K && (!X || !W)))) fail(ORCA_HIP_ERR_INTERNAL, "linear_act: null operand");
     const size_t p8 = act8_layout(M, N).bytes;
-    const Span x{X, matrix_bytes(M, K, ldx)}, w{W, matrix_bytes(K, N, ldw)}, b{e.bias, N * sizeof(float)},
-        r{e.residual, matrix_bytes(M, N, e.ldr)}, y{Y, matrix_bytes(M, N, ldy)}, pre{e.pre, matrix_bytes(M, N, e.ldpre)},
-        z8{e.pre8, p8}, y8{e.y8, p8};
+    const Span x = matrix_span(X, M, K, ldx), w = matrix_span(W, K, N, ldw), b = buffer_span(e.bias, 4 * N),
+               r = matrix_span(e.residual, M, N, e.ldr), y = matrix_span(Y, M, N, ldy),
+               pre = matrix_span(e.pre, M, N, e.ldpre), z8 = buffer_span(e.pre8, p8), y8 = buffer_span(e.y8, p8);
     const Span outs[4] = {y, pre, z8, y8};
     for (int i = 0; i < 4; ++i) {
-      for (const Span& s : {x, w, b}) check_apart(op, outs[i].p, outs[i].bytes, s.p, s.bytes);
+      for (const Span& s : {x, w, b}) check_apart(op, outs[i], s);
       // y over its own residual, element by element, is in order
-      if (!(i == 0 && e.residual == Y && e.ldr == ldy)) check_apart(op, outs[i].p, outs[i].bytes, r.p, r.bytes);
-      for (int j = 0; j < i; ++j) check_apart(op, outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes);
+      if (!(i == 0 && e.residual == Y && e.ldr == ldy)) check_apart(op, outs[i], r);
+      for (int j = 0; j < i; ++j) check_apart(op, outs[i], outs[j]);
     }
     act8_aligned(e.pre8, "linear_act (pre8)");
     act8_aligned(e.y8, "linear_act (y8)");
     bind(ctx);
     if (!M || !N) return;
-    check_extent(ctx, x.p, x.bytes, "linear_act (x)");
-    check_extent(ctx, w.p, w.bytes, "linear_act (weight)");
-    check_extent(ctx, b.p, b.bytes, "linear_act (bias)");
-    check_extent(ctx, r.p, r.bytes, "linear_act (residual)");
-    check_extent(ctx, y.p, y.bytes, "linear_act (y)");
-    check_extent(ctx, pre.p, pre.bytes, "linear_act (pre)");
-    check_extent(ctx, z8.p, z8.bytes, "linear_act (pre8)");
-    check_extent(ctx, y8.p, y8.bytes, "linear_act (y8)");
+    check_extent(ctx, x.p, x.bytes(), "linear_act (x)");
+    check_extent(ctx, w.p, w.bytes(), "linear_act (weight)");
+    check_extent(ctx, b.p, b.bytes(), "linear_act (bias)");
+    check_extent(ctx, r.p, r.bytes(), "linear_act (residual)");
+    check_extent(ctx, y.p, y.bytes(), "linear_act (y)");
+    check_extent(ctx, pre.p, pre.bytes(), "linear_act (pre)");
+    check_extent(ctx, z8.p, z8.bytes(), "linear_act (pre8)");
+    check_extent(ctx, y8.p, y8.bytes(), "linear_act (y8)");
     LinearOut o;
     o.act = e.act;
     o.bias = e.bias;
@@ -588,7 +613,7 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
     p.N = (int64_t)N;
     p.K = (int64_t)K;
     p.out = o;
-    const bool few = M <= 4;
+    const bool few = M <= 4 && !ctx->linear_tile;
     Plan q;
     if (few)
       q = plan_rows(ctx, p, op);
@@ -596,12 +621,13 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
       plan_products(ctx, &p, &q, nullptr, nullptr, false, op);
     std::unique_ptr<Scratch> ws;
     if (q.ws) {
-      ws.reset(new Scratch(ctx, sizeof(float) * q.ws));
+      ws = workspace(ctx, sizeof(float) * q.ws, op);
       p.ws = ws->as<float>();
     }
     std::string pname;
     if (ctx->prof.enabled)
-      pname = std::string(op) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
+      pname = std::string(op) + (few ? "_rows" : "_t" + std::to_string(q.tile)) + " " + std::to_string(M) + "x" +
+              std::to_string(N) + "x" + std::to_string(K);
     ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K, 4.0 * ((double)M * K + (double)K * N + (double)M * N));
     const dim3 grid((unsigned)q.blocks);
     if (few)
@@ -641,31 +667,33 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
       fail(ORCA_HIP_ERR_INTERNAL, "linear_act_backward: one of x and x8 is needed for dw");
     if (M && N && !dY) fail(ORCA_HIP_ERR_INTERNAL, "linear_act_backward: null dy");
     if (dX && M && N && K && !W) fail(ORCA_HIP_ERR_INTERNAL, "linear_act_backward: null weight");
-    const Span dy{dY, matrix_bytes(M, N, lddy)}, w{dX ? W : nullptr, matrix_bytes(K, N, ldw)},
-        z{slope ? s.z : nullptr, matrix_bytes(M, N, s.ldz)}, z8{slope ? s.z8 : nullptr, act8_layout(M, N).bytes},
-        x{dW ? s.x : nullptr, matrix_bytes(M, K, s.ldx)}, x8{dW ? s.x8 : nullptr, act8_layout(M, K).bytes},
-        add{dX ? s.dx_add : nullptr, matrix_bytes(M, K, s.ldadd)}, dx{dX, matrix_bytes(M, K, lddx)},
-        dw{dW, matrix_bytes(K, N, lddw)}, dbs{db, N * sizeof(float)};
+    const Span dy = matrix_span(dY, M, N, lddy), w = matrix_span(dX ? W : nullptr, K, N, ldw),
+               z = matrix_span(slope ? s.z : nullptr, M, N, s.ldz),
+               z8 = buffer_span(slope ? s.z8 : nullptr, act8_layout(M, N).bytes),
+               x = matrix_span(dW ? s.x : nullptr, M, K, s.ldx),
+               x8 = buffer_span(dW ? s.x8 : nullptr, act8_layout(M, K).bytes),
+               add = matrix_span(dX ? s.dx_add : nullptr, M, K, s.ldadd), dx = matrix_span(dX, M, K, lddx),
+               dw = matrix_span(dW, K, N, lddw), dbs = buffer_span(db, 4 * N);
     const Span outs[3] = {dx, dw, dbs};
     for (int i = 0; i < 3; ++i) {
-      for (const Span& in : {dy, w, z, z8, x, x8}) check_apart(op, outs[i].p, outs[i].bytes, in.p, in.bytes);
+      for (const Span& in : {dy, w, z, z8, x, x8}) check_apart(op, outs[i], in);
       // dx over dx_add, element by element, is in order (a gradient added up in place)
-      if (!(i == 0 && s.dx_add == dX && s.ldadd == lddx)) check_apart(op, outs[i].p, outs[i].bytes, add.p, add.bytes);
-      for (int j = 0; j < i; ++j) check_apart(op, outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes);
+      if (!(i == 0 && s.dx_add == dX && s.ldadd == lddx)) check_apart(op, outs[i], add);
+      for (int j = 0; j < i; ++j) check_apart(op, outs[i], outs[j]);
     }
     act8_aligned(z8.p, "linear_act_backward (z8)");
     act8_aligned(x8.p, "linear_act_backward (x8)");
     bind(ctx);
-    check_extent(ctx, dy.p, dy.bytes, "linear_act_backward (dy)");
-    check_extent(ctx, w.p, w.bytes, "linear_act_backward (weight)");
-    check_extent(ctx, z.p, z.bytes, "linear_act_backward (z)");
-    check_extent(ctx, z8.p, z8.bytes, "linear_act_backward (z8)");
-    check_extent(ctx, x.p, x.bytes, "linear_act_backward (x)");
-    check_extent(ctx, x8.p, x8.bytes, "linear_act_backward (x8)");
-    check_extent(ctx, add.p, add.bytes, "linear_act_backward (dx_add)");
-    check_extent(ctx, dx.p, dx.bytes, "linear_act_backward (dx)");
-    check_extent(ctx, dw.p, dw.bytes, "linear_act_backward (dw)");
-    check_extent(ctx, db, dbs.bytes, "linear_act_backward (db)");
+    check_extent(ctx, dy.p, dy.bytes(), "linear_act_backward (dy)");
+    check_extent(ctx, w.p, w.bytes(), "linear_act_backward (weight)");
+    check_extent(ctx, z.p, z.bytes(), "linear_act_backward (z)");
+    check_extent(ctx, z8.p, z8.bytes(), "linear_act_backward (z8)");
+    check_extent(ctx, x.p, x.bytes(), "linear_act_backward (x)");
+    check_extent(ctx, x8.p, x8.bytes(), "linear_act_backward (x8)");
+    check_extent(ctx, add.p, add.bytes(), "linear_act_backward (dx_add)");
+    check_extent(ctx, dx.p, dx.bytes(), "linear_act_backward (dx)");
+    check_extent(ctx, dw.p, dw.bytes(), "linear_act_backward (dw)");
+    check_extent(ctx, db, dbs.bytes(), "linear_act_backward (db)");
     const bool want_dx = dX && M && K, want_dw = dW && K && N, want_db = db && N;
     const float* dz = dY;
     int64_t lddz = (int64_t)lddy;
@@ -676,20 +704,20 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     dyz.ldz = (int64_t)s.ldz;
     dyz.z8 = act8_at(const_cast<void*>(z8.p), M, N);
     // slopes inside the products: a launch less, but every tile takes its panel's slopes again
-    const bool inside = M && N && M <= kInsideRows && (double)M * N * K <= (slope ? kInsideWork : kInsideWorkPlain);
+    const bool inside = M && N && !ctx->linear_tile && M <= kInsideRows && (double)M * N * K <= (slope ? kInsideWork : kInsideWorkPlain);
     // dW as outer products; the slopes of 16 rows there cost a thread more (4 us with GELU) than the tiles' padding
-    const bool few = M && M <= (size_t)kRowsDw && want_dw && !(inside && slope && M > 4);
+    const bool few = M && !ctx->linear_tile && M <= (size_t)kRowsDw && want_dw && !(inside && slope && M > 4);
     // 64 rows a block, 16 where that leaves CUs without one
     const bool tall = ((int64_t)M + 63) / 64 * (((int64_t)N + 255) / 256) >= ctx->num_cus;
     const int64_t rows = tall ? 64 : 16, blocks = ((int64_t)M + rows - 1) / rows;
     const bool direct = blocks == 1 && !inside;  // a block's column sums are db
     if (N && !inside && (want_db || (slope && (want_dx || want_dw)))) {
       if (slope && M) {
-        dzs.reset(new Scratch(ctx, sizeof(float) * M * N));
+        dzs = workspace(ctx, sizeof(float) * M * N, op);
         dz = dzs->as<float>();
         lddz = (int64_t)N;
       }
-      if (want_db && M && !direct) partial.reset(new Scratch(ctx, sizeof(float) * (size_t)blocks * N));
+      if (want_db && M && !direct) partial = workspace(ctx, sizeof(float) * (size_t)blocks * N, op);
       if (M) {
         ProfScope prof(ctx, "linear_act_slope", 0.0, (slope ? 12.0 : 4.0) * M * N);
         hipLaunchKernelGGL(tall ? slope_kernel<16> : slope_kernel<4>, quad_grid((int64_t)M, rows, (int64_t)N, op),
@@ -739,7 +767,7 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     if (few) qw.blocks = ((int64_t)K + kRowDw - 1) / kRowDw * (((int64_t)N + 255) / 256);
     std::unique_ptr<Scratch> ws;
     if (qx.ws + qw.ws) {
-      ws.reset(new Scratch(ctx, sizeof(float) * (qx.ws + qw.ws)));
+      ws = workspace(ctx, sizeof(float) * (qx.ws + qw.ws), op);
       b.dx.ws = ws->as<float>();
       b.dw.ws = ws->as<float>() + qx.ws;
     }
@@ -749,7 +777,8 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     if (!grid) return;
     std::string pname;
     if (ctx->prof.enabled)
-      pname = std::string(op) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
+      pname = std::string(op) + (inside ? "_inside" : "") +
+              (few ? "_rows" : "_t" + std::to_string(std::max(qx.tile, qw.tile))) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
     ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K * (want_dx + want_dw),
                    4.0 * ((double)M * N + (want_dx + want_dw) * ((double)M * K + (double)K * N)));
     b.dx_blocks = (int)qx.blocks;

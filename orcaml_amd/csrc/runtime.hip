@@ -133,6 +133,11 @@ int orca_hip_ctx_create(int device, orca_hip_ctx** out) {
       if (std::strcmp(v, "128x64") == 0) ctx->gemm_generic_bn = 64;
     }
     if (const char* v = std::getenv("ORCA_HIP_GEMM_SPLITS")) ctx->gemm_splits = std::max(0, std::min(64, std::atoi(v)));
+    if (const char* v = std::getenv("ORCA_HIP_LINEAR_TILE"))
+      for (int t : {64, 128, 256})
+        if (std::to_string(t) == v) ctx->linear_tile = t;
+    if (const char* v = std::getenv("ORCA_HIP_LINEAR_SPLITS"))
+      ctx->linear_splits = std::max(0, std::min(256, std::atoi(v)));
     hipError_t e = hipStreamCreateWithFlags(&ctx->stream, hipStreamNonBlocking);
     if (e == hipSuccess) e = hipEventCreate(&ctx->timer_start);
     if (e == hipSuccess) e = hipEventCreate(&ctx->timer_stop);

@@ -229,6 +229,11 @@ struct orca_hip_ctx {
   // 128 x 128 tiles; 1 prefers the eight-band grid (every CU), 2 the 112-row tiles
   // (the CUs the 128 x 128 grid leaves free stay free) where both apply.
   int gemm_band = 2;
+  // ORCA_HIP_LINEAR_TILE=64|128|256 fixes the tile of the fused Linear's products (0 = by the
+  // product's size, and kernels of their own for a few rows and small backwards) and
+  // ORCA_HIP_LINEAR_SPLITS=n their K split.
+  int linear_tile = 0;
+  int linear_splits = 0;
   // Host waits on this context's work so far (stream or event synchronisations).
   std::atomic<uint64_t> host_syncs{0};
   orca_hip::StagingRing staging;

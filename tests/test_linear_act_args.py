@@ -34,7 +34,9 @@ def _backward(m=4, n=8, k=16, dy=P, lddy=None, w=2 * P, ldw=None, dx=3 * P, lddx
 def test_good_arguments_reach_the_context():
     for rc, msg in (_forward(), _forward(act=4, bias=7 * P, residual=8 * P, ldr=8, pre=9 * P, ldpre=9, pre8=10 * P,
                                          y8=11 * P),
-                    _forward(residual=3 * P, ldr=8), _forward(m=0, x=None, w=None, y=None), _backward(),
+                    _forward(residual=3 * P, ldr=8), _forward(ldy=24, residual=3 * P + 32, ldr=24),
+                    _forward(ldy=24, residual=3 * P + 64, ldr=24), _forward(ldy=24, residual=3 * P - 32, ldr=24),
+                    _forward(ldy=24, x=3 * P + 32, ldx=24), _forward(m=0, x=None, w=None, y=None), _backward(),
                     _backward(act=2, z=7 * P, ldz=8), _backward(act=2, z8=7 * P, x=None, x8=8 * P),
                     _backward(dx_add=3 * P, ldadd=16), _backward(dx_add=P, ldadd=16, k=8, ldx=8, lddx=8),
                     _backward(dx=None, w=None), _backward(dw=None, x=None), _backward(m=0, dy=None, x=None)):
@@ -54,8 +56,12 @@ def test_good_arguments_reach_the_context():
     (dict(residual=3 * P, ldr=9), _lib.ERR_INTERNAL, "overlaps"),
     (dict(residual=3 * P + 4, ldr=8), _lib.ERR_INTERNAL, "overlaps"),
     (dict(pre=7 * P, ldpre=8, residual=7 * P, ldr=8), _lib.ERR_INTERNAL, "overlaps"),
-    (dict(m=1 << 31), _lib.ERR_SHAPE, "2^31"), (dict(n=1 << 31), _lib.ERR_SHAPE, "2^31"),
-    (dict(k=1 << 32), _lib.ERR_SHAPE, "2^31")])
+    (dict(m=1 << 30), _lib.ERR_SHAPE, "2^30"), (dict(n=1 << 30), _lib.ERR_SHAPE, "2^30"),
+    (dict(k=1 << 32), _lib.ERR_SHAPE, "2^30"), (dict(ldx=1 << 41), _lib.ERR_SHAPE, "2^40"),
+    (dict(ldy=24, residual=3 * P + 28, ldr=24), _lib.ERR_INTERNAL, "overlaps"),
+    (dict(ldy=24, residual=3 * P + 68, ldr=24), _lib.ERR_INTERNAL, "overlaps"),
+    (dict(ldy=24, residual=3 * P - 28, ldr=24), _lib.ERR_INTERNAL, "overlaps"),
+    (dict(ldy=24, residual=3 * P + 32, ldr=23), _lib.ERR_INTERNAL, "overlaps")])
 def test_forward_refuses(bad, code, word):
     rc, msg = _forward(**bad)
     assert rc == code and word in msg, (rc, msg)
@@ -73,7 +79,7 @@ def test_forward_refuses(bad, code, word):
     (dict(act=1, z8=7 * P + 1), _lib.ERR_INTERNAL, "aligned"), (dict(dx=P), _lib.ERR_INTERNAL, "overlaps"),
     (dict(dw=2 * P), _lib.ERR_INTERNAL, "overlaps"), (dict(db=4 * P), _lib.ERR_INTERNAL, "overlaps"),
     (dict(dx=6 * P), _lib.ERR_INTERNAL, "overlaps"), (dict(dx_add=3 * P, ldadd=17), _lib.ERR_INTERNAL, "overlaps"),
-    (dict(dx_add=4 * P, ldadd=16), _lib.ERR_INTERNAL, "overlaps"), (dict(m=1 << 31), _lib.ERR_SHAPE, "2^31")])
+    (dict(dx_add=4 * P, ldadd=16), _lib.ERR_INTERNAL, "overlaps"), (dict(m=1 << 30), _lib.ERR_SHAPE, "2^30")])
 def test_backward_refuses(bad, code, word):
     rc, msg = _backward(**bad)
     assert rc == code and word in msg, (rc, msg)
