@@ -652,7 +652,7 @@ int orca_hip_relu_bw_colsum_noalloc(orca_hip_ctx* ctx, const float* grad, const 
  * terms that add up to it; sums are fp32), on the bf16 matrix instructions.  Their sums run in
  * another order than orca_hip_gemm's.  Infinities and NaN come out as from fp32 products; magnitudes
  * below 2^-100 keep fewer bits, and below 2^-126 none.
- * Sizes are below 2^30 each and may be 0; leading dimensions count elements; fp32 operands
+ * Sizes are below 2^27 each and may be 0; leading dimensions count elements, up to 2^34; fp32 operands
  * need no alignment beyond a float's.  A call may not write what it reads, or overlap two results,
  * except as said below (columns of one matrix beside each other, given with its leading dimension,
  * do not overlap).  Work is enqueued on the context stream; workspaces come from the context's

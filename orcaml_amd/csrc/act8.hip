@@ -1,5 +1,6 @@
 // Packing activations into 8-bit checkpoints and back (format and arithmetic: act8.hpp).
 // Both are one pass over memory.
+#include <algorithm>
 #include <string>
 
 #include "act8.hpp"
@@ -15,7 +16,7 @@ __global__ void __launch_bounds__(256) act8_pack_kernel(const float* __restrict_
                                                         int64_t cols, Act8 out) {
   typedef uint32_t word_u __attribute__((aligned(1)));
   const int64_t r0 = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 6);
-  const int64_t c = (int64_t)blockIdx.y * 256 + (threadIdx.x & 63) * 4;
+  const int64_t c = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 256 + (threadIdx.x & 63) * 4;
   const int have = (int)max((int64_t)0, min((int64_t)4, cols - c));
   floatx4 v[4];
 #pragma unroll
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(Act8 in, int64_t rows,
                                                           int64_t ldo) {
   typedef uint32_t word_u __attribute__((aligned(1)));
   const int64_t r0 = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 6);
-  const int64_t c = (int64_t)blockIdx.y * 256 + (threadIdx.x & 63) * 4;
+  const int64_t c = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 256 + (threadIdx.x & 63) * 4;
   if (c >= cols) return;
   const int have = (int)min((int64_t)4, cols - c);
   uint32_t w[4], b[4];
@@ -103,10 +104,17 @@ __global__ void __launch_bounds__(256) act8_unpack_kernel(Act8 in, int64_t rows,
   }
 }
 
-dim3 act8_grid(size_t rows, size_t per, size_t cols, const char* op) {
-  const size_t gx = (rows + per - 1) / per, gy = (cols + 255) / 256;
-  if (gx > 0x7fffffffu || gy > 65535) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
-  return dim3((unsigned)gx, (unsigned)gy);
+dim3 act8_grid(size_t rows, size_t cols) {
+  const size_t gx = (rows + 15) / 16, gy = (cols + 255) / 256, y = std::min<size_t>(gy, 32768);
+  return dim3((unsigned)gx, (unsigned)y, (unsigned)((gy + y - 1) / y));
+}
+
+void act8_check(const char* op, size_t rows, size_t cols, size_t ld) {
+  for (size_t v : {rows, cols})
+    if (v >> kMaxSizeBits) fail_shape(op, "sizes below 2^" + std::to_string(kMaxSizeBits), std::to_string(v));
+  if (ld > size_t(1) << kMaxLdBits)
+    fail_shape(op, "a leading dimension of at most 2^" + std::to_string(kMaxLdBits), std::to_string(ld));
+  if (ld < cols) fail_shape(op, "a leading dimension of at least " + std::to_string(cols), std::to_string(ld));
 }
 
 void act8_apart(const char* op, const void* out, size_t out_bytes, const void* in, size_t in_bytes) {
@@ -131,7 +139,7 @@ extern "C" {
 int orca_hip_act8_size(size_t rows, size_t cols, size_t* bytes, size_t* scales_offset) {
   return guard([&] {
     if (!bytes) fail(ORCA_HIP_ERR_INTERNAL, "act8_size: null output pointer");
-    if (cols && rows > (SIZE_MAX >> 8) / cols) fail(ORCA_HIP_ERR_SHAPE, "Shape mismatch during act8_size: size overflow");
+    act8_check("act8_size", rows, cols, cols);
     const Act8Layout l = act8_layout(rows, cols);
     *bytes = l.bytes;
     if (scales_offset) *scales_offset = l.scales;
@@ -140,7 +148,7 @@ int orca_hip_act8_size(size_t rows, size_t cols, size_t* bytes, size_t* scales_o
 
 int orca_hip_act8_pack(orca_hip_ctx* ctx, const float* x, size_t rows, size_t cols, size_t ldx, void* packed) {
   return guard([&] {
-    if (ldx < cols) fail_shape("act8_pack", "a leading dimension of at least " + std::to_string(cols), std::to_string(ldx));
+    act8_check("act8_pack", rows, cols, ldx);
     if (rows && cols && (!x || !packed)) fail(ORCA_HIP_ERR_INTERNAL, "act8_pack: null operand");
     act8_aligned(packed, "act8_pack");
     act8_apart("act8_pack", packed, act8_layout(rows, cols).bytes, x, matrix_bytes(rows, cols, ldx));
@@ -148,7 +156,7 @@ int orca_hip_act8_pack(orca_hip_ctx* ctx, const float* x, size_t rows, size_t co
     if (!rows || !cols) return;
     check_extent(ctx, x, matrix_bytes(rows, cols, ldx), "act8_pack (x)");
     check_extent(ctx, packed, act8_layout(rows, cols).bytes, "act8_pack (checkpoint)");
-    const dim3 grid = act8_grid(rows, 16, cols, "act8_pack");
+    const dim3 grid = act8_grid(rows, cols);
     ProfScope prof(ctx, "act8_pack", 0.0, 4.0 * rows * cols + (double)act8_layout(rows, cols).bytes);
     hipLaunchKernelGGL(act8_pack_kernel, grid, dim3(256), 0, ctx->stream, x, (int64_t)ldx, (int64_t)rows, (int64_t)cols,
                        act8_at(packed, rows, cols));
@@ -160,7 +168,7 @@ int orca_hip_act8_unpack(orca_hip_ctx* ctx, const void* packed, size_t rows, siz
                          size_t ldo) {
   return guard([&] {
     if (dtype != ORCA_HIP_F32 && dtype != ORCA_HIP_BF16) fail_dtype("act8_unpack", dtype);
-    if (ldo < cols) fail_shape("act8_unpack", "a leading dimension of at least " + std::to_string(cols), std::to_string(ldo));
+    act8_check("act8_unpack", rows, cols, ldo);
     if (rows && cols && (!out || !packed)) fail(ORCA_HIP_ERR_INTERNAL, "act8_unpack: null operand");
     act8_aligned(packed, "act8_unpack");
     const size_t width = dtype == ORCA_HIP_F32 ? 4 : 2, out_bytes = matrix_bytes(rows, cols, ldo) / 4 * width;
@@ -169,7 +177,7 @@ int orca_hip_act8_unpack(orca_hip_ctx* ctx, const void* packed, size_t rows, siz
     if (!rows || !cols) return;
     check_extent(ctx, out, out_bytes, "act8_unpack (out)");
     check_extent(ctx, packed, act8_layout(rows, cols).bytes, "act8_unpack (checkpoint)");
-    const dim3 grid = act8_grid(rows, 16, cols, "act8_unpack");
+    const dim3 grid = act8_grid(rows, cols);
     const Act8 in = act8_at(const_cast<void*>(packed), rows, cols);
     ProfScope prof(ctx, "act8_unpack", 0.0, (double)width * rows * cols + (double)act8_layout(rows, cols).bytes);
     if (dtype == ORCA_HIP_F32)

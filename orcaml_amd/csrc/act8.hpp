@@ -17,6 +17,11 @@ namespace orca_hip {
 
 constexpr size_t kAct8Group = 32;
 
+// Bounds on the sizes and leading dimensions of the calls that take checkpoints: byte offsets stay below
+// 2^63, column indexes in bytes below 2^32, and a launch of a block of 256 threads for 16 rows or columns below
+// the runtime's 2^32 threads.
+constexpr int kMaxSizeBits = 27, kMaxLdBits = 34;
+
 struct Act8Layout {
   size_t groups;   // groups of 32 columns
   size_t ld;       // rows of a group's row of step bytes: a multiple of 16, so that 8 rows' bytes are one load

@@ -211,8 +211,8 @@ __global__ void __launch_bounds__(256, T::OCC) row_backward_kernel(BackwardArgs 
 // Column sums of dz = dy * act'(z), 16 columns a block: 16 threads for each, every sixteenth row, eight rows'
 // loads at a time, and the threads' sums in order.
 constexpr int kSumCols = 16;
-__device__ __forceinline__ void slope_sums(const ProductOperand& o, int64_t M, int64_t N, int block, float* __restrict__ db,
-                                           float* __restrict__ sums) {
+__device__ __forceinline__ void slope_sums(const ProductOperand& o, int64_t M, int64_t N, int block,
+                                           float* __restrict__ db, float* __restrict__ sums) {
   const int col = threadIdx.x % kSumCols, run = threadIdx.x / kSumCols;
   const int64_t n = min((int64_t)block * kSumCols + col, N - 1);
   const float* dy = static_cast<const float*>(o.p) + n;
@@ -311,14 +311,15 @@ __global__ void __launch_bounds__(256) split_finish_kernel(FinishArgs a) {
 }
 
 // dz = dy * act'(z) (z in fp32, or its checkpoint) and, per block of 4 R rows, the column sums of dz.
-// A thread takes four columns of R rows, four rows' loads at a time.
-template <int R>
-__global__ void __launch_bounds__(256) slope_kernel(ProductOperand o, float* __restrict__ dz, float* __restrict__ partial,
-                                                    int64_t M, int64_t N) {
+// A thread takes four columns of R rows (a multiple of 4), four rows' loads at a time.
+__global__ void __launch_bounds__(256) slope_kernel(ProductOperand o, float* __restrict__ dz,
+                                                    float* __restrict__ partial, int64_t M, int64_t N, int R) {
   __shared__ floatx4 sums[4][64];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int64_t r0 = (int64_t)blockIdx.x * (4 * R) + wave * R;
-  const Quad q = quad_of((int64_t)blockIdx.y * 256 + lane * 4, N);
+  const int64_t r0 = ((int64_t)blockIdx.x * 4 + wave) * R;
+  const int64_t c0 = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * 256;
+  if (c0 >= N) return;  // the whole block
+  const Quad q = quad_of(c0 + lane * 4, N);
   const float* dy = static_cast<const float*>(o.p);
   floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int r = 0; r < R && r0 + r < M; r += 4) {
@@ -347,17 +348,13 @@ __global__ void __launch_bounds__(256) slope_kernel(ProductOperand o, float* __r
     store_quad(partial + (int64_t)blockIdx.x * N, q, sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]);
 }
 
-dim3 quad_grid(int64_t rows, int64_t per, int64_t cols, const char* op) {
-  const int64_t gx = (rows + per - 1) / per, gy = (cols + 255) / 256;
-  if (gx > 0x7fffffff || gy > 65535) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
-  return dim3((unsigned)gx, (unsigned)gy);
-}
-
 // 256: eight waves of 128 x 64, the least LDS traffic for a matrix instruction; at 8192 x 4096 x 4096 228 TFLOP/s
 // (of fp32 work; 128: 201, 64: 154).  128 and 64 for products with too few tiles of 256.
 using Tile256 = ProductTile<256, 256, 2, 4, 16, 1>;
 using Tile128 = ProductTile<128, 128, 2, 4, 32, 1>;
 using Tile64 = ProductTile<64, 64, 2, 2, 32, 3>;
+
+constexpr int64_t kMaxThreads = 0x7fffffff;  // of a launch
 
 struct Plan {
   int tile = 0;       // 0: nothing to do
@@ -395,7 +392,8 @@ int cuts_of(orca_hip_ctx* ctx, const ProductArgs& p, bool codes, int tile, Cut (
   const TileCost& c = kTileCosts[codes][tile];
   const int64_t tm = (p.M + c.tile - 1) / c.tile, tn = (p.N + c.tile - 1) / c.tile;
   int n = 0;
-  if (tm > 0x3fffffff / tn) return 0;
+  const int64_t most = kMaxThreads / 512;  // threads of the largest tiles' blocks
+  if (tm > most / tn) return 0;
   for (int64_t want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 64, 128, 256}) {
     if (ctx->linear_splits) {  // that many, as far as k goes
       if (want > 1) break;
@@ -406,7 +404,7 @@ int cuts_of(orca_hip_ctx* ctx, const ProductArgs& p, bool codes, int tile, Cut (
     // even runs of a multiple of every stage's k values
     const int64_t chunk = std::max<int64_t>(64, ((p.K + want - 1) / want + 63) / 64 * 64);
     const int64_t splits = std::max<int64_t>(1, (p.K + chunk - 1) / chunk);
-    if (want > 1 && splits == 1 && n) continue;
+    if ((want > 1 && splits == 1 && n) || tm * tn > most / splits) continue;
     const double stages = (double)((std::min(chunk, p.K) + c.bk - 1) / c.bk);
     const double finish =
         splits > 1 ? c.finish + 4.0 * (double)(splits + 1) * (double)p.M * (double)p.N / c.bytes_per_us : 0.0;
@@ -458,10 +456,9 @@ void plan_products(orca_hip_ctx* ctx, ProductArgs* a, Plan* qa, ProductArgs* b, 
 
 // Forward of a few rows: a block for 16 columns, k split so that the blocks cover the CUs.  A checkpoint's group
 // of 32 columns then lies in two blocks, so with one the split products' finish writes it.
-Plan plan_rows(orca_hip_ctx* ctx, ProductArgs& p, const char* op) {
+Plan plan_rows(orca_hip_ctx* ctx, ProductArgs& p) {
   Plan q;
   const int64_t tn = (p.N + kRowCols - 1) / kRowCols;
-  if (tn > 0x7fffffff / 64) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
   const bool packs = p.out.pre8.codes || p.out.y8.codes;
   const int64_t splits = std::max<int64_t>(packs ? 2 : 1, std::min<int64_t>({ctx->num_cus / tn, p.K / 512, 32}));
   p.chunk = std::max<int64_t>(1, (p.K + splits - 1) / splits);
@@ -481,7 +478,7 @@ void launch_finish(orca_hip_ctx* ctx, const ProductArgs& a, const Plan& qa, cons
   FinishArgs f{{a, b}, {finish_blocks(a, qa), finish_blocks(b, qb)}};
   const int64_t grid = f.blocks[0] + f.blocks[1];
   if (!grid) return;
-  if (grid > 0x7fffffff) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
+  if (grid > kMaxThreads / 256) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
   hipLaunchKernelGGL(split_finish_kernel, dim3((unsigned)grid), dim3(256), 0, ctx->stream, f);
   ORCA_HIP_CHECK(hipGetLastError());
 }
@@ -511,12 +508,13 @@ constexpr size_t kInsideRows = 512;
 constexpr double kInsideWork = 2.5e7, kInsideWorkPlain = 3e8;
 
 void check_ld(const char* what, size_t ld, size_t cols) {
-  if (ld > (size_t(1) << 40)) fail_shape(what, "a leading dimension of at most 2^40", std::to_string(ld));
+  if (ld > size_t(1) << kMaxLdBits)
+    fail_shape(what, "a leading dimension of at most 2^" + std::to_string(kMaxLdBits), std::to_string(ld));
   if (ld < cols) fail_shape(what, "a leading dimension of at least " + std::to_string(cols), std::to_string(ld));
 }
 void check_sizes(const char* op, size_t M, size_t N, size_t K) {
   for (size_t v : {M, N, K})
-    if (v >= (size_t(1) << 30)) fail_shape(op, "sizes below 2^30", std::to_string(v));
+    if (v >> kMaxSizeBits) fail_shape(op, "sizes below 2^" + std::to_string(kMaxSizeBits), std::to_string(v));
 }
 // An operand's rows of `width` bytes, `ld` bytes apart (one row: a contiguous buffer).
 struct Span {
@@ -613,10 +611,10 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
     p.N = (int64_t)N;
     p.K = (int64_t)K;
     p.out = o;
-    const bool few = M <= 4 && !ctx->linear_tile;
+    const bool few = M <= 4 && N <= kRowMaxCols && !ctx->linear_tile;
     Plan q;
     if (few)
-      q = plan_rows(ctx, p, op);
+      q = plan_rows(ctx, p);
     else
       plan_products(ctx, &p, &q, nullptr, nullptr, false, op);
     std::unique_ptr<Scratch> ws;
@@ -704,12 +702,15 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     dyz.ldz = (int64_t)s.ldz;
     dyz.z8 = act8_at(const_cast<void*>(z8.p), M, N);
     // slopes inside the products: a launch less, but every tile takes its panel's slopes again
-    const bool inside = M && N && !ctx->linear_tile && M <= kInsideRows && (double)M * N * K <= (slope ? kInsideWork : kInsideWorkPlain);
+    const bool inside = M && N && !ctx->linear_tile && M <= kInsideRows &&
+                        (double)M * N * K <= (slope ? kInsideWork : kInsideWorkPlain);
     // dW as outer products; the slopes of 16 rows there cost a thread more (4 us with GELU) than the tiles' padding
     const bool few = M && !ctx->linear_tile && M <= (size_t)kRowsDw && want_dw && !(inside && slope && M > 4);
-    // 64 rows a block, 16 where that leaves CUs without one
-    const bool tall = ((int64_t)M + 63) / 64 * (((int64_t)N + 255) / 256) >= ctx->num_cus;
-    const int64_t rows = tall ? 64 : 16, blocks = ((int64_t)M + rows - 1) / rows;
+    // 64 rows a block, 16 where that leaves CUs without one; more where the column sums would get long to add up
+    const int64_t panels = ((int64_t)N + 255) / 256;
+    int64_t rows = ((int64_t)M + 63) / 64 * panels >= ctx->num_cus ? 64 : 16;
+    rows = std::max(rows, ((int64_t)M / 2048 + 15) / 16 * 16);
+    const int64_t blocks = ((int64_t)M + rows - 1) / rows;
     const bool direct = blocks == 1 && !inside;  // a block's column sums are db
     if (N && !inside && (want_db || (slope && (want_dx || want_dw)))) {
       if (slope && M) {
@@ -720,8 +721,11 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
       if (want_db && M && !direct) partial = workspace(ctx, sizeof(float) * (size_t)blocks * N, op);
       if (M) {
         ProfScope prof(ctx, "linear_act_slope", 0.0, (slope ? 12.0 : 4.0) * M * N);
-        hipLaunchKernelGGL(tall ? slope_kernel<16> : slope_kernel<4>, quad_grid((int64_t)M, rows, (int64_t)N, op),
-                           dim3(256), 0, ctx->stream, dyz, dzs ? dzs->as<float>() : nullptr, want_db && direct ? db : partial ? partial->as<float>() : nullptr, (int64_t)M, (int64_t)N);
+        const int64_t gy = std::min<int64_t>(panels, 32768);
+        hipLaunchKernelGGL(slope_kernel, dim3((unsigned)blocks, (unsigned)gy, (unsigned)((panels + gy - 1) / gy)),
+                           dim3(256), 0, ctx->stream, dyz, dzs ? dzs->as<float>() : nullptr,
+                           want_db && direct ? db : partial ? partial->as<float>() : nullptr, (int64_t)M, (int64_t)N,
+                           (int)(rows / 4));
         ORCA_HIP_CHECK(hipGetLastError());
       }
     }
@@ -773,12 +777,13 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     }
     const int64_t sums = inside ? kSumCols : 32;
     const int64_t grid = qx.blocks + qw.blocks + (b.db ? ((int64_t)N + sums - 1) / sums : 0);
-    if (grid > 0x7fffffff) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
+    if (grid > kMaxThreads / 512) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
     if (!grid) return;
     std::string pname;
     if (ctx->prof.enabled)
       pname = std::string(op) + (inside ? "_inside" : "") +
-              (few ? "_rows" : "_t" + std::to_string(std::max(qx.tile, qw.tile))) + " " + std::to_string(M) + "x" + std::to_string(N) + "x" + std::to_string(K);
+              (few ? "_rows" : "_t" + std::to_string(std::max(qx.tile, qw.tile))) + " " + std::to_string(M) + "x" +
+              std::to_string(N) + "x" + std::to_string(K);
     ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K * (want_dx + want_dw),
                    4.0 * ((double)M * N + (want_dx + want_dw) * ((double)M * K + (double)K * N)));
     b.dx_blocks = (int)qx.blocks;

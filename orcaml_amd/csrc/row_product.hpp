@@ -7,6 +7,7 @@
 // each finishes its outputs itself; a wave reads 16 k values of those columns with one load, and
 // the block's 16 waves walk down k together, eight such loads each in flight.
 constexpr int kRowCols = 16, kRowWaves = 16, kRowLoads = 8;
+constexpr size_t kRowMaxCols = size_t(1) << 24;  // 2^30 threads
 template <int MR>
 __global__ void __launch_bounds__(kRowWaves * 64) row_forward_kernel(ProductArgs p) {
   __shared__ floatx4 sums[kRowWaves][MR][4];
@@ -62,8 +63,9 @@ __global__ void __launch_bounds__(kRowWaves * 64) row_forward_kernel(ProductArgs
 }
 
 // Block (64 rows of dW, 256 columns) of dW = x^T dz for batches of at most 16 rows, x in fp32 or as a
-// checkpoint, dz in memory or (SLOPE) made here from dy and z: a lane holds its four columns of dz and writes one row of dW after the other.  67 MB of dW in
-// 13 us (1 to 4 rows) and 18 us (16; the tiles 23), 5 us where the launch is all.
+// checkpoint, dz in memory or (SLOPE) made here from dy and z: a lane holds its four columns of dz and
+// writes one row of dW after the other.  67 MB of dW in 13 us (1 to 4 rows) and 18 us (16; the tiles 23),
+// 5 us where the launch is all.
 constexpr int kRowsDw = 16, kRowDw = 64;
 template <int MR, bool SLOPE>
 __device__ __forceinline__ void row_dw(const ProductArgs& p, int block, float* __restrict__ smem) {

@@ -14,9 +14,9 @@
 // Operands are read in fp32 (or 8 bits) and taken apart on their way into LDS: no extra
 // pass over memory and no copy of them.  LDS holds, for each of the three planes, 16-byte
 // units of 8 consecutive k of one row, [k / 8][row], which is what a lane of the 32x32x16
-// instruction takes.  The rows of one k / 8 are followed by two units of padding, so that
-// the stores of a k-fast operand (neighbouring lanes hold neighbouring k / 8) fall into
-// different banks.
+// instruction takes.  The rows of one k / 8 are followed by padding, 8 units for all k / 8
+// together, so that the stores of a k-fast operand (neighbouring lanes hold neighbouring
+// k / 8) fall into different banks.
 //
 // Infinities and NaN: inf - inf in the split, and inf times an m or l of zero, make NaN where
 // fp32 has an infinity.  So a block that ends with a value that is not finite multiplies its tile again
@@ -102,8 +102,9 @@ struct SplitUnit {
 constexpr int unit_pitch(int rows, int kh) { return rows + 8 / kh; }
 
 // Loaders: a stage is BK k values of ROWS rows, one unit of 8 k values of one row per thread.  Rows past
-// the operand's last are the last one again (what they give is never stored); k values past the range are zero (tail).  piece(k) for k in 0 .. 8 takes the loaded
-// unit to LDS.  The product comes out 1 / SCALE times too large, unless SAFE.
+// the operand's last are the last one again (what they give is never stored); k values past the range are
+// zero (tail).  piece(k) for k in 0 .. 8 takes the loaded unit to LDS.  The product comes out 1 / SCALE
+// times too large, unless SAFE.
 
 // k is contiguous: a unit is 32 bytes, at any alignment of its floats.
 template <int ROWS, int BK, int THREADS>
@@ -387,7 +388,8 @@ __device__ __forceinline__ void product_unit(const u32x4 (&a)[LA::PLANES], const
     for (int e = 0; e < 8; ++e)
 #pragma unroll
       for (int j = 0; j < FN; ++j)
-        acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(whole(b[j], LB::PLANES, e), whole(a, LA::PLANES, e), acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(whole(b[j], LB::PLANES, e), whole(a, LA::PLANES, e), acc[j], 0,
+                                                      0, 0);
   } else {
     // the smallest terms first
     constexpr int PA[6] = {0, 2, 1, 0, 1, 0}, PB[6] = {2, 0, 1, 1, 0, 0}, PB1[3] = {2, 1, 0};
@@ -434,7 +436,8 @@ __device__ __forceinline__ void product_stage(const u32x4* __restrict__ sa, cons
       if (u % T::FM == T::FM - 1) read_b<T, LB>(sb, rb, u / T::FM + 1, b[(u / T::FM + 1) & 1]);
       read_a<T, LA>(sa, ra, u + 1, a[(u + 1) & 1]);
     }
-    product_unit<T::FN, LA, LB, FP32>(a[u & 1], b[u / T::FM & 1], acc[u % T::FM], [&](int g) { work(u * T::FN * terms<LA>() + g); });
+    product_unit<T::FN, LA, LB, FP32>(a[u & 1], b[u / T::FM & 1], acc[u % T::FM],
+                                      [&](int g) { work(u * T::FN * terms<LA>() + g); });
   }
 }
 

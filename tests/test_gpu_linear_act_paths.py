@@ -260,3 +260,39 @@ def test_tiny_magnitudes(ctx):
     assert (np.abs(y.astype(np.float64) - x) <= 2.0 ** -125).all()
     fine = np.abs(x) >= 2.0 ** -100
     np.testing.assert_array_equal(y[fine], x[fine])
+
+
+@pytest.mark.parametrize("m,n,k", [(1, (1 << 25) + 5, 1), (3, 17000003, 2), ((1 << 25) + 5, 1, 1), (40000000, 2, 3),
+                                   (20, 17000001, 1), (1, 2, 17000001)])
+def test_the_longest_sizes(ctx, m, n, k):
+    """Past 65535 blocks of 256 columns, past the few rows' longest rows, and millions of rows: small whole numbers, so
+    exact (the checkpoint too: codes of up to 7 bits with steps of powers of two)."""
+    x = (np.arange(m * k, dtype=np.int64) % 7 - 3).astype(np.float32).reshape(m, k)
+    w = (np.arange(k * n, dtype=np.int64) % 5 - 2).astype(np.float32).reshape(k, n)
+    want = sum(x[:, i:i + 1] * w[i:i + 1] for i in range(k)) if k < 10 else x @ w
+    if k >= 10:  # by sums that stay whole numbers below 2^24
+        want = np.add.reduce((x[0][:, None] * w).astype(np.float64), axis=0)[None].astype(np.float32)
+    X, W, y8 = L.Mat(ctx, x), L.Mat(ctx, w), L.Packed(ctx, m, n)
+    np.testing.assert_array_equal(L.forward(ctx, X, W, y8=y8).get(), want)
+    small = np.abs(want).max() < 64
+    back = L.Mat(ctx, shape=(m, n))
+    _lib.call("orca_hip_act8_unpack", ctx.handle, y8.ptr, m, n, _lib.F32, back.ptr, n)
+    if small:
+        np.testing.assert_array_equal(back.get(), want)
+    z = (np.arange(m * n, dtype=np.int64) % 3 - 1).astype(np.float32).reshape(m, n)
+    dy = (np.arange(m * n, dtype=np.int64) % 11 - 5).astype(np.float32).reshape(m, n)
+    g = dy * (z > 0)
+    dx, dw, db = L.Mat(ctx, shape=(m, k)), L.Mat(ctx, shape=(k, n)), L.Mat(ctx, shape=(1, n))
+    L.backward(ctx, L.Mat(ctx, dy), W, "relu", z=L.Mat(ctx, z), x=X, dx=dx, dw=dw, db=db)
+    g64 = g.astype(np.float64)
+    for what, got, exact, size in (("db", db, g64.sum(0, keepdims=True), np.abs(g64).sum(0).max()),
+                                   ("dx", dx, g64 @ w.T.astype(np.float64), 10 * n),
+                                   ("dw", dw, x.T.astype(np.float64) @ g64, 15 * m)):
+        got = got.get()
+        if size < 1 << 24:
+            np.testing.assert_array_equal(got, exact, err_msg=what)
+        else:
+            # fp32 sums of whole numbers: runs of at most 2^15 terms and fewer than 2^12 runs a sum, each addition off by half a
+            # step of a partial sum, which stays below `size`; steps of runs are exact below 2^24
+            tol = 2.0 ** -24 * (1 << 12) * np.abs(exact) + 2.0 ** -24 * size * 600
+            assert (np.abs(got - exact) <= tol).all(), what

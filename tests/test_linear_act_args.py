@@ -56,8 +56,8 @@ def test_good_arguments_reach_the_context():
     (dict(residual=3 * P, ldr=9), _lib.ERR_INTERNAL, "overlaps"),
     (dict(residual=3 * P + 4, ldr=8), _lib.ERR_INTERNAL, "overlaps"),
     (dict(pre=7 * P, ldpre=8, residual=7 * P, ldr=8), _lib.ERR_INTERNAL, "overlaps"),
-    (dict(m=1 << 30), _lib.ERR_SHAPE, "2^30"), (dict(n=1 << 30), _lib.ERR_SHAPE, "2^30"),
-    (dict(k=1 << 32), _lib.ERR_SHAPE, "2^30"), (dict(ldx=1 << 41), _lib.ERR_SHAPE, "2^40"),
+    (dict(m=1 << 27), _lib.ERR_SHAPE, "2^27"), (dict(n=1 << 27), _lib.ERR_SHAPE, "2^27"),
+    (dict(k=1 << 32), _lib.ERR_SHAPE, "2^27"), (dict(ldx=(1 << 34) + 1), _lib.ERR_SHAPE, "2^34"),
     (dict(ldy=24, residual=3 * P + 28, ldr=24), _lib.ERR_INTERNAL, "overlaps"),
     (dict(ldy=24, residual=3 * P + 68, ldr=24), _lib.ERR_INTERNAL, "overlaps"),
     (dict(ldy=24, residual=3 * P - 28, ldr=24), _lib.ERR_INTERNAL, "overlaps"),
@@ -79,7 +79,7 @@ def test_forward_refuses(bad, code, word):
     (dict(act=1, z8=7 * P + 1), _lib.ERR_INTERNAL, "aligned"), (dict(dx=P), _lib.ERR_INTERNAL, "overlaps"),
     (dict(dw=2 * P), _lib.ERR_INTERNAL, "overlaps"), (dict(db=4 * P), _lib.ERR_INTERNAL, "overlaps"),
     (dict(dx=6 * P), _lib.ERR_INTERNAL, "overlaps"), (dict(dx_add=3 * P, ldadd=17), _lib.ERR_INTERNAL, "overlaps"),
-    (dict(dx_add=4 * P, ldadd=16), _lib.ERR_INTERNAL, "overlaps"), (dict(m=1 << 30), _lib.ERR_SHAPE, "2^30")])
+    (dict(dx_add=4 * P, ldadd=16), _lib.ERR_INTERNAL, "overlaps"), (dict(m=1 << 27), _lib.ERR_SHAPE, "2^27")])
 def test_backward_refuses(bad, code, word):
     rc, msg = _backward(**bad)
     assert rc == code and word in msg, (rc, msg)
@@ -118,6 +118,11 @@ def test_checkpoints_refuse():
                              ((P, 4, 8, _lib.BF16, 2 * P, 8), _lib.ERR_INTERNAL, "null orca_hip_ctx")):
         rc, msg = _call("orca_hip_act8_unpack", None, *args)
         assert rc == code and word in msg, (args, rc, msg)
+    for rows, cols, ld, word in ((1 << 27, 1, 1, "2^27"), (1, 1 << 27, 1 << 27, "2^27"), (1 << 40, 1 << 40, 1 << 62, "2^27"),
+                                 (5, 8, 1 << 62, "2^34"), ((1 << 24) + 1, 8, 1 << 38, "2^34")):
+        for fn, args in (("pack", (P, rows, cols, ld, 1 << 50)), ("unpack", (1 << 50, rows, cols, _lib.F32, P, ld))):
+            rc, msg = _call("orca_hip_act8_" + fn, None, *args)
+            assert rc == _lib.ERR_SHAPE and word in msg, (fn, rows, cols, ld, msg)
     rc, msg = _call("orca_hip_act8_size", 1 << 60, 1 << 60, None, None)
     assert rc == _lib.ERR_INTERNAL and "null output" in msg
     rc, msg = _call("orca_hip_act8_size", 1 << 40, 1 << 40, ctypes.byref(ctypes.c_size_t()), None)
