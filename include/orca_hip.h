@@ -422,6 +422,23 @@ int orca_hip_trait_max_to_shape_backward(orca_hip_backend* be, orca_hip_storage*
  * dL/dlogits for a loss seed of 1 (orca_hip_softmax_ce; python/orca/nn/loss.py:59-100). */
 int orca_hip_be_softmax_ce(orca_hip_backend* be, orca_hip_storage* logits, orca_hip_storage* onehot, size_t B, size_t C,
                            int want_grad, orca_hip_storage** loss, orca_hip_storage** dlogits);
+/* Linear with activation and residual on storages (orca_hip_linear_act: its comment says what each means; no
+ * counterpart in the reference): y = act(x w + bias) + residual, bias and residual NULL for none; z, z8 and y8
+ * (NULL: not kept) receive the pre-activation, its 8-bit checkpoint and y's. */
+int orca_hip_be_linear_act(orca_hip_backend* be, orca_hip_storage* x, orca_hip_storage* w, orca_hip_storage* bias,
+                           orca_hip_storage* residual, size_t M, size_t N, size_t K, int act, orca_hip_storage** y,
+                           orca_hip_storage** z, orca_hip_storage** z8, orca_hip_storage** y8);
+/* Its gradients (orca_hip_linear_act_backward): z or z8 and x or x8 as the forward kept them, NULL what is not
+ * needed; dx, dw and db NULL where not wanted. */
+int orca_hip_be_linear_act_backward(orca_hip_backend* be, orca_hip_storage* dy, orca_hip_storage* w, size_t M,
+                                    size_t N, size_t K, int act, orca_hip_storage* z, orca_hip_storage* z8,
+                                    orca_hip_storage* x, orca_hip_storage* x8, orca_hip_storage* dx_add,
+                                    orca_hip_storage** dx, orca_hip_storage** dw, orca_hip_storage** db);
+/* A matrix to its 8-bit checkpoint, in a storage of ceil(bytes / 4) elements (orca_hip_act8_size), and back. */
+int orca_hip_be_act8_pack(orca_hip_backend* be, orca_hip_storage* x, size_t rows, size_t cols,
+                          orca_hip_storage** out);
+int orca_hip_be_act8_unpack(orca_hip_backend* be, orca_hip_storage* packed, size_t rows, size_t cols,
+                            orca_hip_storage** out);
 /* A new storage holding the same values (device to device). */
 int orca_hip_be_clone(orca_hip_backend* be, orca_hip_storage* s, orca_hip_storage** out);
 /* A flat arena of n floats (set to `value` when fill != 0); view: n floats at `offset` floats of

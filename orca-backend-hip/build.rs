@@ -10,9 +10,10 @@ use std::fs;
 use std::path::{Path, PathBuf};
 use std::process::Command;
 
-const SOURCES: [&str; 11] = [
+const SOURCES: [&str; 12] = [
     "runtime_host.cpp",
     "storage.cpp",
+    "linear_be.cpp",
     "runtime.hip",
     "ops.hip",
     "gemm.hip",

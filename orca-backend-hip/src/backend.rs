@@ -48,6 +48,44 @@ fn dims(shape: &Shape) -> (*const usize, usize) {
     (shape.0.as_ptr(), shape.0.len())
 }
 
+/// The activation of `HipBackend::linear_act` (ORCA_HIP_ACT_*).
+#[repr(i32)]
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum Activation {
+    None = 0,
+    Relu = 1,
+    Gelu = 2,
+    GeluTanh = 3,
+    Silu = 4,
+}
+
+/// What `HipBackend::linear_act` keeps beside y: the pre-activation, its 8-bit checkpoint, y's checkpoint.
+#[derive(Clone, Copy, Debug, Default)]
+pub struct Keep {
+    pub z: bool,
+    pub z8: bool,
+    pub y8: bool,
+}
+
+pub struct LinearActOut {
+    pub y: HipStorage,
+    pub z: Option<HipStorage>,
+    pub z8: Option<HipStorage>,
+    pub y8: Option<HipStorage>,
+}
+
+fn raw_or_null(s: Option<&HipStorage>) -> *mut ffi::OrcaHipStorage {
+    s.map_or(ptr::null_mut(), |s| s.raw())
+}
+
+fn out_if(want: bool, out: &mut *mut ffi::OrcaHipStorage) -> *mut *mut ffi::OrcaHipStorage {
+    if want { out } else { ptr::null_mut() }
+}
+
+fn adopted(raw: *mut ffi::OrcaHipStorage) -> Option<HipStorage> {
+    if raw.is_null() { None } else { Some(HipStorage::adopt(raw)) }
+}
+
 impl HipBackend {
     /// A backend on HIP device 0 (GpuBackend::new's counterpart, orca-backend-gpu/src/backend.rs:53).
     pub fn new() -> Result<Self> {
@@ -92,6 +130,68 @@ impl HipBackend {
             ffi::orca_hip_be_softmax_ce(self.be(), logits.raw(), onehot.raw(), b, c, want_grad as c_int, &mut loss, &mut grad)
         })?;
         Ok((HipStorage::adopt(loss), if want_grad { Some(HipStorage::adopt(grad)) } else { None }))
+    }
+
+    /// y = act(x w + bias) + residual of [m, k] x [k, n] in one product, and what `keep` asks for besides.
+    #[allow(clippy::too_many_arguments)]
+    pub fn linear_act(
+        &self,
+        x: &HipStorage,
+        w: &HipStorage,
+        bias: Option<&HipStorage>,
+        residual: Option<&HipStorage>,
+        m: usize,
+        n: usize,
+        k: usize,
+        act: Activation,
+        keep: Keep,
+    ) -> Result<LinearActOut> {
+        let (mut y, mut z, mut z8, mut y8) = (ptr::null_mut(), ptr::null_mut(), ptr::null_mut(), ptr::null_mut());
+        check(unsafe {
+            ffi::orca_hip_be_linear_act(
+                self.be(), x.raw(), w.raw(), raw_or_null(bias), raw_or_null(residual), m, n, k, act as c_int, &mut y,
+                out_if(keep.z, &mut z), out_if(keep.z8, &mut z8), out_if(keep.y8, &mut y8),
+            )
+        })?;
+        Ok(LinearActOut { y: HipStorage::adopt(y), z: adopted(z), z8: adopted(z8), y8: adopted(y8) })
+    }
+
+    /// Its gradients [dx, dw, db] where `want` asks for them; z or z8 and x or x8 as the forward kept them.
+    #[allow(clippy::too_many_arguments)]
+    pub fn linear_act_backward(
+        &self,
+        dy: &HipStorage,
+        w: &HipStorage,
+        m: usize,
+        n: usize,
+        k: usize,
+        act: Activation,
+        z: Option<&HipStorage>,
+        z8: Option<&HipStorage>,
+        x: Option<&HipStorage>,
+        x8: Option<&HipStorage>,
+        dx_add: Option<&HipStorage>,
+        want: [bool; 3],
+    ) -> Result<[Option<HipStorage>; 3]> {
+        let (mut dx, mut dw, mut db) = (ptr::null_mut(), ptr::null_mut(), ptr::null_mut());
+        check(unsafe {
+            ffi::orca_hip_be_linear_act_backward(
+                self.be(), dy.raw(), w.raw(), m, n, k, act as c_int, raw_or_null(z), raw_or_null(z8), raw_or_null(x),
+                raw_or_null(x8), raw_or_null(dx_add), out_if(want[0], &mut dx), out_if(want[1], &mut dw),
+                out_if(want[2], &mut db),
+            )
+        })?;
+        Ok([adopted(dx), adopted(dw), adopted(db)])
+    }
+
+    /// The 8-bit checkpoint of a [rows, cols] matrix.
+    pub fn act8_pack(&self, x: &HipStorage, rows: usize, cols: usize) -> Result<HipStorage> {
+        self.out(|o| unsafe { ffi::orca_hip_be_act8_pack(self.be(), x.raw(), rows, cols, o) })
+    }
+
+    /// The values a checkpoint stands for.
+    pub fn act8_unpack(&self, packed: &HipStorage, rows: usize, cols: usize) -> Result<HipStorage> {
+        self.out(|o| unsafe { ffi::orca_hip_be_act8_unpack(self.be(), packed.raw(), rows, cols, o) })
     }
 
     /// A new storage with the same values.

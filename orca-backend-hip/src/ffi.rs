@@ -487,6 +487,52 @@ extern "C" {
         loss: *mut *mut OrcaHipStorage,
         dlogits: *mut *mut OrcaHipStorage,
     ) -> c_int;
+    pub fn orca_hip_be_linear_act(
+        be: *mut OrcaHipBackend,
+        x: *mut OrcaHipStorage,
+        w: *mut OrcaHipStorage,
+        bias: *mut OrcaHipStorage,
+        residual: *mut OrcaHipStorage,
+        m: usize,
+        n: usize,
+        k: usize,
+        act: c_int,
+        y: *mut *mut OrcaHipStorage,
+        z: *mut *mut OrcaHipStorage,
+        z8: *mut *mut OrcaHipStorage,
+        y8: *mut *mut OrcaHipStorage,
+    ) -> c_int;
+    pub fn orca_hip_be_linear_act_backward(
+        be: *mut OrcaHipBackend,
+        dy: *mut OrcaHipStorage,
+        w: *mut OrcaHipStorage,
+        m: usize,
+        n: usize,
+        k: usize,
+        act: c_int,
+        z: *mut OrcaHipStorage,
+        z8: *mut OrcaHipStorage,
+        x: *mut OrcaHipStorage,
+        x8: *mut OrcaHipStorage,
+        dx_add: *mut OrcaHipStorage,
+        dx: *mut *mut OrcaHipStorage,
+        dw: *mut *mut OrcaHipStorage,
+        db: *mut *mut OrcaHipStorage,
+    ) -> c_int;
+    pub fn orca_hip_be_act8_pack(
+        be: *mut OrcaHipBackend,
+        x: *mut OrcaHipStorage,
+        rows: usize,
+        cols: usize,
+        out: *mut *mut OrcaHipStorage,
+    ) -> c_int;
+    pub fn orca_hip_be_act8_unpack(
+        be: *mut OrcaHipBackend,
+        packed: *mut OrcaHipStorage,
+        rows: usize,
+        cols: usize,
+        out: *mut *mut OrcaHipStorage,
+    ) -> c_int;
     pub fn orca_hip_be_clone(be: *mut OrcaHipBackend, s: *mut OrcaHipStorage, out: *mut *mut OrcaHipStorage) -> c_int;
     pub fn orca_hip_be_arena(
         be: *mut OrcaHipBackend,

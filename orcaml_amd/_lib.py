@@ -185,6 +185,10 @@ SIGNATURES = {
     "orca_hip_trait_has_nan_or_inf": [_P, _P, _I, ctypes.POINTER(_I)],
     "orca_hip_trait_max_to_shape": _TR,
     "orca_hip_trait_max_to_shape_backward": [_P, _P, _P, _P, _SZP, _SZ, _SZP, _SZ, _I, _PP],
+    "orca_hip_be_linear_act": [_P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _PP, _PP, _PP, _PP],
+    "orca_hip_be_linear_act_backward": [_P, _P, _P, _SZ, _SZ, _SZ, _I, _P, _P, _P, _P, _P, _PP, _PP, _PP],
+    "orca_hip_be_act8_pack": [_P, _P, _SZ, _SZ, _PP],
+    "orca_hip_be_act8_unpack": [_P, _P, _SZ, _SZ, _PP],
     "orca_hip_be_softmax_ce": [_P, _P, _P, _SZ, _SZ, _I, _PP, _PP],
     "orca_hip_be_clone": [_P, _P, _PP],
     "orca_hip_be_arena": [_P, _SZ, _I, _F, _PP],

@@ -581,8 +581,8 @@ class Module:
                     t.require_grad()
                 p.tensor = t
 
-    def __call__(self, *args):
-        return self.forward(*args)
+    def __call__(self, *args, **kwargs):
+        return self.forward(*args, **kwargs)
 
 
 class Linear(Module):

@@ -387,95 +387,62 @@ class HipBackend:
             raise ValueError(f"unknown activation {name!r}: one of {', '.join(self.ACTIVATIONS)}")
         return self.ACTIVATIONS[name]
 
-    def _operand(self, s: HipStorage | None, n: int, what: str):
-        """(address, storage to hold until the call) of a contiguous storage of n values."""
+    def _handle(self, s: HipStorage | None, what: str):
         if s is None:
-            return None, None
+            return None
         if s.be.ctx is not self.ctx:
             raise ValueError(f"Device mismatch: {what} is on another context")
-        if s.n != n:
-            raise ValueError(f"Shape mismatch during {what}: expected {n} elements, got {s.n}")
-        if s.transposed:
-            s = self.clone(s)
-        return s.ptr, s
+        return s.h
 
-    def _checkpoint(self, rows: int, cols: int) -> Act8:
-        c = Act8(None, rows, cols)
-        c.storage = self.arena(-(-c.nbytes // 4))
-        return c
-
-    def _checkpoint_ptr(self, c: Act8 | None, rows: int, cols: int, what: str):
-        if c is None:
-            return None
-        if c.storage.be.ctx is not self.ctx:
-            raise ValueError(f"Device mismatch: {what} is on another context")
-        if (c.rows, c.cols) != (rows, cols):
-            raise ValueError(f"Shape mismatch during {what}: expected {[rows, cols]}, got {[c.rows, c.cols]}")
-        return c.storage.ptr
+    def _kept_handle(self, t, rows: int, cols: int, what: str):
+        """(handle, None) of a storage, (None, handle) of a checkpoint."""
+        if not isinstance(t, Act8):
+            return self._handle(t, what), None
+        if (t.rows, t.cols) != (rows, cols):
+            raise ValueError(f"Shape mismatch during {what}: expected {[rows, cols]}, got {[t.rows, t.cols]}")
+        return None, self._handle(t.storage, what)
 
     def act8_pack(self, s: HipStorage, rows: int, cols: int) -> Act8:
-        """The 8-bit checkpoint of a matrix (orca_hip_act8_pack)."""
-        p, hold = self._operand(s, rows * cols, "act8_pack")  # noqa: F841
-        c = self._checkpoint(rows, cols)
-        _lib.call("orca_hip_act8_pack", self.ctx.handle, p, rows, cols, cols, c.storage.ptr)
-        return c
+        """The 8-bit checkpoint of a matrix (orca_hip_be_act8_pack)."""
+        return Act8(self._out("orca_hip_be_act8_pack", self._handle(s, "act8_pack"), rows, cols), rows, cols)
 
     def act8_unpack(self, c: Act8) -> HipStorage:
-        """The values a checkpoint stands for, in f32 (orca_hip_act8_unpack)."""
-        p = self._checkpoint_ptr(c, c.rows, c.cols, "act8_unpack")
-        out = self.arena(c.rows * c.cols)
-        _lib.call("orca_hip_act8_unpack", self.ctx.handle, p, c.rows, c.cols, _lib.F32, out.ptr, c.cols)
-        return out
+        """The values a checkpoint stands for, in f32 (orca_hip_be_act8_unpack)."""
+        return self._out("orca_hip_be_act8_unpack", self._handle(c.storage, "act8_unpack"), c.rows, c.cols)
 
     def linear_act(self, x: HipStorage, w: HipStorage, bias: HipStorage | None, residual: HipStorage | None, M: int,
                    N: int, K: int, act: str = "none", keep: tuple = ()):
-        """y = act(x w + bias) + residual of [M, K] x [K, N] in one product (orca_hip_linear_act).
+        """y = act(x w + bias) + residual of [M, K] x [K, N] in one product (orca_hip_be_linear_act).
         Returns y and what `keep` names besides: "z" the pre-activation, "z8" and "y8" checkpoints
         of the pre-activation and of y, as a dict."""
         act = self._act(act)
         if not set(keep) <= {"z", "z8", "y8"}:
             raise ValueError(f"linear_act cannot keep {sorted(set(keep) - {'z', 'z8', 'y8'})}")
-        xp, hx = self._operand(x, M * K, "linear_act (x)")
-        wp, hw = self._operand(w, K * N, "linear_act (weight)")
-        bp, hb = self._operand(bias, N, "linear_act (bias)")
-        rp, hr = self._operand(residual, M * N, "linear_act (residual)")
-        y = self.arena(M * N)
-        kept = {k: self.arena(M * N) if k == "z" else self._checkpoint(M, N) for k in keep}
-        e = _lib.LinearEpilogue(act=act, bias=bp, residual=rp, ldr=N, pre=kept["z"].ptr if "z" in kept else None,
-                                ldpre=N, pre8=kept["z8"].storage.ptr if "z8" in kept else None,
-                                y8=kept["y8"].storage.ptr if "y8" in kept else None)
-        _lib.call("orca_hip_linear_act", self.ctx.handle, M, N, K, xp, K, wp, N, y.ptr, N, ctypes.byref(e))
-        del hx, hw, hb, hr
-        return y, kept
+        out = {k: _VP() for k in ("y", *keep)}
+        p = {k: ctypes.byref(v) for k, v in out.items()}
+        _lib.call("orca_hip_be_linear_act", self.handle, self._handle(x, "linear_act (x)"),
+                  self._handle(w, "linear_act (weight)"), self._handle(bias, "linear_act (bias)"),
+                  self._handle(residual, "linear_act (residual)"), M, N, K, act, p["y"], p.get("z"), p.get("z8"),
+                  p.get("y8"))
+        out = {k: self._wrap(v.value) for k, v in out.items()}
+        return out.pop("y"), {k: s if k == "z" else Act8(s, M, N) for k, s in out.items()}
 
     def linear_act_backward(self, dy: HipStorage, w: HipStorage, M: int, N: int, K: int, act: str = "none",
                             z: HipStorage | Act8 | None = None, x: HipStorage | Act8 | None = None,
                             dx_add: HipStorage | None = None, want: tuple = ("dx", "dw", "db")) -> dict:
-        """The gradients that `want` names (orca_hip_linear_act_backward); z and x are what the
+        """The gradients that `want` names (orca_hip_be_linear_act_backward); z and x are what the
         forward kept, in f32 or as checkpoints."""
         act = self._act(act)
         if not set(want) <= {"dx", "dw", "db"}:
             raise ValueError(f"linear_act_backward cannot give {sorted(set(want) - {'dx', 'dw', 'db'})}")
-        dyp, hdy = self._operand(dy, M * N, "linear_act_backward (dy)")
-        wp, hw = self._operand(w, K * N, "linear_act_backward (weight)")
-        ap, ha = self._operand(dx_add, M * K, "linear_act_backward (dx_add)")
-        held = {}
-
-        def kept(t, cols, what):
-            if isinstance(t, Act8):
-                return None, self._checkpoint_ptr(t, M, cols, what)
-            p, held[what] = self._operand(t, M * cols, what)
-            return p, None
-
-        zp, z8 = kept(z if act != _lib.ACT_NONE else None, N, "linear_act_backward (z)")
-        xp, x8 = kept(x if "dw" in want else None, K, "linear_act_backward (x)")
-        out = {k: self.arena({"dx": M * K, "dw": K * N, "db": N}[k]) for k in want}
-        s = _lib.LinearSaved(act=act, z=zp, ldz=N, z8=z8, x=xp, ldx=K, x8=x8, dx_add=ap, ldadd=K)
-        p = {k: t.ptr for k, t in out.items()}
-        _lib.call("orca_hip_linear_act_backward", self.ctx.handle, M, N, K, dyp, N, wp, N, ctypes.byref(s),
-                  p.get("dx"), K, p.get("dw"), N, p.get("db"))
-        del hdy, hw, ha
-        return out
+        zs = self._kept_handle(z if act != _lib.ACT_NONE else None, M, N, "linear_act_backward (z)")
+        xs = self._kept_handle(x if "dw" in want else None, M, K, "linear_act_backward (x)")
+        out = {k: _VP() for k in want}
+        p = {k: ctypes.byref(v) for k, v in out.items()}
+        _lib.call("orca_hip_be_linear_act_backward", self.handle, self._handle(dy, "linear_act_backward (dy)"),
+                  self._handle(w, "linear_act_backward (weight)"), M, N, K, act, *zs, *xs,
+                  self._handle(dx_add, "linear_act_backward (dx_add)"), p.get("dx"), p.get("dw"), p.get("db"))
+        return {k: self._wrap(v.value) for k, v in out.items()}
 
     # ---- flat arenas and one-launch optimizer passes ----
     def arena(self, n: int, fill: float | None = None) -> HipStorage:

@@ -9,6 +9,7 @@
 #include <atomic>
 #include <cstdint>
 #include <deque>
+#include <functional>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -324,6 +325,23 @@ void check_extent(orca_hip_ctx* ctx, const void* p, size_t bytes, const char* wh
 inline size_t matrix_bytes(size_t rows, size_t cols, size_t ld) {
   return rows == 0 || cols == 0 ? 0 : ((rows - 1) * ld + cols) * sizeof(float);
 }
+
+// A call of the buffer-level ABI on storages, under the backend's lock (storage.cpp): its operands'
+// values are computed first and transposed views made contiguous; `run` gets their addresses (null for
+// an optional null storage) and those of new storages (null where `out` is), which the caller receives.
+struct BeOperand {
+  orca_hip_storage* storage;
+  size_t n;  // the elements it must have
+  const char* what;
+  bool optional = false;
+};
+struct BeResult {
+  size_t n;
+  orca_hip_storage** out;
+  bool optional = false;
+};
+int be_run(orca_hip_backend* be, const std::vector<BeOperand>& in, const std::vector<BeResult>& out,
+           const std::function<int(orca_hip_ctx*, float* const* in, float* const* out)>& run);
 
 inline void check_ctx(const orca_hip_ctx* ctx) {
   if (!ctx) fail(ORCA_HIP_ERR_INTERNAL, "null orca_hip_ctx");

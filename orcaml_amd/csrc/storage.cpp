@@ -1554,6 +1554,35 @@ Node* take_colsum_waiter(Node* s, size_t cols) {
 [[noreturn]] void unsupported(const char* op, int dtype) { fail_dtype(op, dtype); }
 
 }  // namespace
+
+int be_run(orca_hip_backend* be, const std::vector<BeOperand>& in, const std::vector<BeResult>& out,
+           const std::function<int(orca_hip_ctx*, float* const* in, float* const* out)>& run) {
+  return entry(be, [&](Backend* b) {
+    std::vector<Ref> operands, results;
+    std::vector<float*> ip, op;
+    for (const BeOperand& o : in) {
+      ip.push_back(nullptr);
+      if (!o.storage && o.optional) continue;
+      Node* x = arg(b, o.storage, o.what);
+      if (x->n != o.n)
+        fail_shape(o.what, std::to_string(o.n) + " elements", std::to_string(x->n) + " elements");
+      operands.push_back(plain(b, x));
+      ip.back() = dptr(b, operands.back().get());
+    }
+    for (const BeResult& r : out) {
+      op.push_back(nullptr);
+      if (!r.out && r.optional) continue;
+      check_out(r.out);
+      results.push_back(Ref(value_node(b, r.n, alloc_buf(b, r.n))));
+      op.back() = results.back()->buf->ptr;
+    }
+    ck(run(b->ctx, ip.data(), op.data()));
+    size_t i = 0;
+    for (const BeResult& r : out)
+      if (r.out) put(r.out, results[i++].release());
+  });
+}
+
 }  // namespace orca_hip
 
 using namespace orca_hip;

@@ -251,3 +251,38 @@ def test_fails_while_launches_go_to_the_side_stream(hb):
             hb.linear_act(s, w, None, None, 64, 64, 64)
     finally:
         hb.ctx.use_side_stream(0)
+
+
+def test_calls_from_several_threads(hb):
+    """Layers and fused optimizer passes (whose updates run on the second stream) on one backend from four threads: each
+    thread's results are those of one thread."""
+    import threading
+
+    def work(seed, steps, out):
+        rng = np.random.default_rng(seed)
+        ad = A.Autodiff(hb)
+        layers = [A.LinearAct(ad, rng.standard_normal((96, 96)).astype(np.float32) / 10, np.zeros(96, np.float32), "silu",
+                              checkpoint=c) for c in (True, False)]
+        opt = A.AdamW([p for layer in layers for p in layer.parameters()], lr=1e-3, fused=True)
+        x = A.Tensor.from_numpy(ad, rng.standard_normal((130, 96)).astype(np.float32))
+        t = A.Tensor.from_numpy(ad, rng.standard_normal((130, 96)).astype(np.float32))
+        for _ in range(steps):
+            opt.zero_grad()
+            h = layers[0](x, residual=x)
+            diff = layers[1](h, residual=h) - t
+            (diff * diff).mean().backward()
+            opt.step()
+        out[seed] = [p.tensor.numpy() for layer in layers for p in layer.parameters()]
+
+    alone, together = {}, {}
+    for seed in range(4):
+        work(seed, 6, alone)
+    threads = [threading.Thread(target=work, args=(seed, 6, together)) for seed in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert sorted(together) == sorted(alone)
+    for seed in alone:
+        for a, b in zip(alone[seed], together[seed]):
+            np.testing.assert_array_equal(a, b)
