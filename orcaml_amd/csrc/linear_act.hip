@@ -457,20 +457,34 @@ void plan_products(orca_hip_ctx* ctx, ProductArgs* a, Plan* qa, ProductArgs* b, 
   if (b) *qb = take(*b, best_tile, best_b);
 }
 
-// Forward of a few rows: a block for 16 columns, k split so that the blocks cover the CUs.  A checkpoint's group
-// of 32 columns then lies in two blocks, so with one the split products' finish writes it.
-Plan plan_rows(orca_hip_ctx* ctx, ProductArgs& p) {
+// Forward of a few rows: blocks of 16 columns, of more where that gives more blocks than CUs.  k is split, so that
+// the blocks cover the CUs, from three steps of a block's loads on (4096 x 512 weights, two steps: 7.1 us
+// in one launch and 8.3 in two; 10000 x 1000: 13.2 split).  A checkpoint's group of 32 columns lies in two
+// blocks of 16, so there the split products' finish writes it.
+Plan plan_rows(orca_hip_ctx* ctx, ProductArgs& p, int& groups) {
   Plan q;
-  const int64_t tn = (p.N + kRowCols - 1) / kRowCols;
-  const bool packs = p.out.pre8.codes || p.out.y8.codes;
-  const int64_t splits = std::max<int64_t>(packs ? 2 : 1, std::min<int64_t>({ctx->num_cus / tn, p.K / 512, 32}));
+  groups = 1;
+  while (groups < kRowWaves && p.N > (int64_t)groups * kRowCols * ctx->num_cus) groups *= 2;
+  const int64_t tn = (p.N + groups * kRowCols - 1) / (groups * kRowCols);
+  const int64_t least = groups == 1 && (p.out.pre8.codes || p.out.y8.codes) ? 2 : 1;
+  const int64_t step = kRowWaves * 16 * row_loads(p.M), steps = (p.K + step - 1) / step;
+  const int64_t splits =
+      std::max<int64_t>(least, steps < 3 ? 1 : std::min<int64_t>({ctx->num_cus / tn, p.K / step, 32}));
   p.chunk = std::max<int64_t>(1, (p.K + splits - 1) / splits);
-  p.splits = (int)std::max<int64_t>(packs ? 2 : 1, (p.K + p.chunk - 1) / p.chunk);
+  p.splits = (int)std::max<int64_t>(least, (p.K + p.chunk - 1) / p.chunk);
   p.tiles_m = 1;
   p.tiles_n = (int)tn;
   q.blocks = tn * p.splits;
   if (p.splits > 1) q.ws = (size_t)p.splits * p.M * p.N;
   return q;
+}
+
+void launch_rows(orca_hip_ctx* ctx, const ProductArgs& p, unsigned blocks, int groups) {
+  const auto kernel = p.M == 1   ? row_forward_kernel<1>
+                      : p.M == 2 ? row_forward_kernel<2>
+                      : p.M <= 4 ? row_forward_kernel<4>
+                                 : row_forward_kernel<8>;
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kRowWaves * 64), 0, ctx->stream, p, groups);
 }
 
 int64_t finish_blocks(const ProductArgs& p, const Plan& q) {
@@ -614,10 +628,11 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
     p.N = (int64_t)N;
     p.K = (int64_t)K;
     p.out = o;
-    const bool few = M <= 4 && N <= kRowMaxCols && !ctx->linear_tile;
+    const bool few = M <= kRowsForward && !ctx->linear_tile;
     Plan q;
+    int groups = 1;
     if (few)
-      q = plan_rows(ctx, p);
+      q = plan_rows(ctx, p, groups);
     else
       plan_products(ctx, &p, &q, nullptr, nullptr, false, op);
     std::unique_ptr<Scratch> ws;
@@ -632,8 +647,7 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
     ProfScope prof(ctx, pname.c_str(), 2.0 * M * N * K, 4.0 * ((double)M * K + (double)K * N + (double)M * N));
     const dim3 grid((unsigned)q.blocks);
     if (few)
-      hipLaunchKernelGGL(M == 1 ? row_forward_kernel<1> : row_forward_kernel<4>, grid, dim3(kRowWaves * 64), 0,
-                         ctx->stream, p);
+      launch_rows(ctx, p, (unsigned)q.blocks, groups);
     else if (q.tile == 256)
       hipLaunchKernelGGL(linear_act_kernel<Tile256>, grid, dim3(Tile256::THREADS), 0, ctx->stream, p);
     else if (q.tile == 128)

@@ -72,10 +72,13 @@ def test_the_switch_fixes_the_tile(tiled):
 
 
 # shapes that the kernels for few rows and for small backwards take: 1 .. 16 rows, widths around 16, 64 and 256
-# columns and below 4, k of one wave's step, of several, and split
+# columns and below 4, and past 16 columns for each CU (blocks of 2 to 16 groups), k of one wave's step, of several,
+# and split
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 16, 256), (2, 17, 100), (3, 3, 2000), (4, 258, 4100), (4, 4096, 700),
                                    (1, 70, 9000), (5, 64, 65), (9, 255, 63), (16, 256, 128), (16, 1030, 70),
-                                   (17, 130, 40), (12, 2, 300)])
+                                   (17, 130, 40), (12, 2, 300),
+                                   (2, 5001, 300), (3, 9000, 70), (1, 17003, 257), (4, 40000, 33), (5, 5001, 130),
+                                   (6, 33, 3100), (7, 8200, 40), (8, 66000, 17), (8, 30, 5000), (8, 4100, 1100)])
 def test_few_rows(ctx, m, n, k):
     L.test_forward(ctx, m, n, k)
     L.test_backward(ctx, m, n, k)
@@ -91,7 +94,7 @@ def test_which_kernels_take_what(ctx):
         return names(ctx, lambda: L.backward(ctx, one(m, n), one(k, n), act, z=one(m, n) if act != "none" else None,
                                              x=one(m, k), dx=one(m, k), dw=one(k, n), db=one(1, n)))
 
-    assert fwd(4, 300, 300) == ["linear_act_rows"] and fwd(5, 300, 300) == ["linear_act_t64"]
+    assert fwd(8, 300, 300) == ["linear_act_rows"] and fwd(9, 300, 300) == ["linear_act_t64"]
     assert bwd(64, 128, 128, "gelu") == ["linear_act_backward_inside_t64"]
     assert bwd(4, 128, 128, "gelu") == ["linear_act_backward_inside_rows"]
     assert bwd(16, 128, 128, "none") == ["linear_act_backward_inside_rows"]
