@@ -391,7 +391,7 @@ struct Cut {
   int together;
 };
 constexpr int kMaxCuts = 13;
-int cuts_of(orca_hip_ctx* ctx, const ProductArgs& p, bool codes, int tile, Cut (&out)[kMaxCuts]) {
+int cuts_of(orca_hip_ctx* ctx, const ProductArgs& p, bool codes, int tile, double slopes, Cut (&out)[kMaxCuts]) {
   const TileCost& c = kTileCosts[codes][tile];
   const int64_t tm = (p.M + c.tile - 1) / c.tile, tn = (p.N + c.tile - 1) / c.tile;
   int n = 0;
@@ -411,8 +411,8 @@ int cuts_of(orca_hip_ctx* ctx, const ProductArgs& p, bool codes, int tile, Cut (
     const double stages = (double)((std::min(chunk, p.K) + c.bk - 1) / c.bk);
     const double finish =
         splits > 1 ? c.finish + 4.0 * (double)(splits + 1) * (double)p.M * (double)p.N / c.bytes_per_us : 0.0;
-    out[n++] = Cut{tm, tn, splits, chunk, tm * tn * splits, stages * c.chain + c.block, stages * c.stage + c.each,
-                   finish, c.launch, c.together};
+    out[n++] = Cut{tm, tn, splits, chunk, tm * tn * splits, stages * (c.chain + slopes) + c.block,
+                   stages * (c.stage + slopes / 2) + c.each, finish, c.launch, c.together};
   }
   return n;
 }
@@ -425,8 +425,9 @@ Plan take(ProductArgs& p, int tile, const Cut& c) {
 }
 
 // The tile and the cuts of a product, or of two that share a launch (on one tile; `only`: that of this size).
-void plan_products(orca_hip_ctx* ctx, ProductArgs* a, Plan* qa, ProductArgs* b, Plan* qb, bool b_codes, const char* op,
-                   int only = 0) {
+// `slopes`: what a stage takes longer because dz is made in it.  Returns the microseconds expected.
+double plan_products(orca_hip_ctx* ctx, ProductArgs* a, Plan* qa, ProductArgs* b, Plan* qb, bool b_codes,
+                     const char* op, int only = 0, double slopes = 0.0) {
   if (ctx->linear_tile) only = ctx->linear_tile;
   double best = 0.0;
   int best_tile = -1;
@@ -434,7 +435,8 @@ void plan_products(orca_hip_ctx* ctx, ProductArgs* a, Plan* qa, ProductArgs* b, 
   for (int tile = 0; tile < 3; ++tile) {
     if (only && kTileCosts[0][tile].tile != only) continue;
     Cut ca[kMaxCuts] = {}, cb[kMaxCuts] = {};
-    const int na = a ? cuts_of(ctx, *a, false, tile, ca) : 1, nb = b ? cuts_of(ctx, *b, b_codes, tile, cb) : 1;
+    const int na = a ? cuts_of(ctx, *a, false, tile, slopes, ca) : 1;
+    const int nb = b ? cuts_of(ctx, *b, b_codes, tile, slopes, cb) : 1;
     for (int i = 0; i < na; ++i)
       for (int j = 0; j < nb; ++j) {
         const Cut &x = ca[i], &y = cb[j];
@@ -455,23 +457,22 @@ void plan_products(orca_hip_ctx* ctx, ProductArgs* a, Plan* qa, ProductArgs* b, 
   if (best_tile < 0) fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": matrix too large");
   if (a) *qa = take(*a, best_tile, best_a);
   if (b) *qb = take(*b, best_tile, best_b);
+  return best;
 }
 
-// Forward of a few rows: blocks of 16 columns, of more where that gives more blocks than CUs.  k is split, so that
-// the blocks cover the CUs, from three steps of a block's loads on (4096 x 512 weights, two steps: 7.1 us
-// in one launch and 8.3 in two; 10000 x 1000: 13.2 split).  A checkpoint's group of 32 columns lies in two
-// blocks of 16, so there the split products' finish writes it.
+// Forward of a few rows: blocks of 16 columns, or of a checkpoint's groups of 32, and of more where that gives more
+// blocks than CUs.  k is split, so that the blocks cover the CUs, from three steps of a block's loads on
+// (4096 x 512 weights, two steps: 7.1 us in one launch and 8.3 in two; 10000 x 1000: 13.2 split).
 Plan plan_rows(orca_hip_ctx* ctx, ProductArgs& p, int& groups) {
   Plan q;
-  groups = 1;
+  groups = p.out.pre8.codes || p.out.y8.codes ? 2 : 1;
   while (groups < kRowWaves && p.N > (int64_t)groups * kRowCols * ctx->num_cus) groups *= 2;
   const int64_t tn = (p.N + groups * kRowCols - 1) / (groups * kRowCols);
-  const int64_t least = groups == 1 && (p.out.pre8.codes || p.out.y8.codes) ? 2 : 1;
-  const int64_t step = kRowWaves * 16 * row_loads(p.M), steps = (p.K + step - 1) / step;
+  const int64_t step = kRowWaves / groups * 16 * row_loads(p.M), steps = (p.K + step - 1) / step;
   const int64_t splits =
-      std::max<int64_t>(least, steps < 3 ? 1 : std::min<int64_t>({ctx->num_cus / tn, p.K / step, 32}));
+      steps < 3 ? 1 : std::max<int64_t>(1, std::min<int64_t>({ctx->num_cus / tn, p.K / step, 32}));
   p.chunk = std::max<int64_t>(1, (p.K + splits - 1) / splits);
-  p.splits = (int)std::max<int64_t>(least, (p.K + p.chunk - 1) / p.chunk);
+  p.splits = (int)std::max<int64_t>(1, (p.K + p.chunk - 1) / p.chunk);
   p.tiles_m = 1;
   p.tiles_n = (int)tn;
   q.blocks = tn * p.splits;
@@ -523,6 +524,10 @@ void launch_backward(orca_hip_ctx* ctx, int tile, bool codes, unsigned grid, con
 // 3e7 (96 x 1605 x 341: 19.7 and 17.7 us, 64 x 784 x 128: 9.9 and 12.6).
 constexpr size_t kInsideRows = 512;
 constexpr double kInsideWork = 2.5e7, kInsideWorkPlain = 3e8;
+// Below that the model decides: a stage of 32 k values takes 0.42 us longer with ReLU's slopes in it (40 x 30 x 1800
+// unsplit: 60 us, 40 with a launch for the slopes), 0.69 with another activation's, 0.26 more from a
+// checkpoint; the launch that makes them apart takes this long.
+constexpr double kSlopeLaunch = 4.0;
 
 void check_ld(const char* what, size_t ld, size_t cols) {
   if (ld > size_t(1) << kMaxLdBits)
@@ -709,7 +714,6 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     check_extent(ctx, dx.p, dx.bytes(), "linear_act_backward (dx)");
     check_extent(ctx, dw.p, dw.bytes(), "linear_act_backward (dw)");
     check_extent(ctx, db, dbs.bytes(), "linear_act_backward (db)");
-    const bool want_dx = dX && M && K, want_dw = dW && K && N, want_db = db && N;
     const float* dz = dY;
     int64_t lddz = (int64_t)lddy;
     std::unique_ptr<Scratch> dzs, partial;
@@ -718,11 +722,31 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     dyz.z = static_cast<const float*>(z.p);
     dyz.ldz = (int64_t)s.ldz;
     dyz.z8 = act8_at(const_cast<void*>(z8.p), M, N);
-    // slopes inside the products: a launch less, but every tile takes its panel's slopes again
-    const bool inside = M && N && !ctx->linear_tile && M <= kInsideRows &&
-                        (double)M * N * K <= (slope ? kInsideWork : kInsideWorkPlain);
+    const bool want_dx = dX && M && K, want_dw = dW && K && N, want_db = db && N;
     // dW as outer products; the slopes of 16 rows there cost a thread more (4 us with GELU) than the tiles' padding
-    const bool few = M && !ctx->linear_tile && M <= (size_t)kRowsDw && want_dw && !(inside && slope && M > 4);
+    auto few_rows = [&](bool in) {
+      return M && !ctx->linear_tile && M <= (size_t)kRowsDw && want_dw && !(in && slope && M > 4);
+    };
+    // slopes inside the products: a launch less, but every tile takes its panel's slopes again
+    bool inside = M && N && !ctx->linear_tile && M <= kInsideRows &&
+                  (double)M * N * K <= (slope ? kInsideWork : kInsideWorkPlain);
+    double slopes = 0.0;
+    if (inside && slope) {
+      slopes = (s.act == ORCA_HIP_ACT_RELU ? 0.42 : 0.69) + (s.z8 ? 0.26 : 0.0);
+      auto expected = [&](bool in) {
+        ProductArgs x{}, w{};
+        x.M = w.K = (int64_t)M;
+        x.N = w.M = (int64_t)K;
+        x.K = w.N = (int64_t)N;
+        Plan qx, qw;
+        const bool on_tiles = want_dw && !few_rows(in);
+        return !want_dx && !on_tiles ? kTileCosts[0][0].launch
+                                     : plan_products(ctx, want_dx ? &x : nullptr, &qx, on_tiles ? &w : nullptr, &qw,
+                                                     s.x8 != nullptr, op, Tile64::BM, in ? slopes : 0.0);
+      };
+      inside = expected(true) <= expected(false) + kSlopeLaunch;
+    }
+    const bool few = few_rows(inside);
     // 64 rows a block, 16 where that leaves CUs without one; more where the column sums would get long to add up
     const int64_t panels = ((int64_t)N + 255) / 256;
     int64_t rows = ((int64_t)M + 63) / 64 * panels >= ctx->num_cus ? 64 : 16;
@@ -785,7 +809,7 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
     }
     if (want_dx || (want_dw && !few))
       plan_products(ctx, want_dx ? &b.dx : nullptr, &qx, want_dw && !few ? &b.dw : nullptr, &qw, s.x8 != nullptr, op,
-                    few || inside ? Tile64::BM : 0);
+                    few || inside ? Tile64::BM : 0, inside ? slopes : 0.0);
     if (few) qw.blocks = ((int64_t)K + kRowDw - 1) / kRowDw * (((int64_t)N + 255) / 256);
     std::unique_ptr<Scratch> ws;
     if (qx.ws + qw.ws) {
