@@ -177,15 +177,23 @@ struct BackwardArgs {
   int64_t M;
 };
 
-// db[n] = the sum of the slope kernel's column sums: RUNS runs of blocks, each in order, then the runs in order.
+// db[n] = the sum of the slope kernel's column sums: RUNS runs of blocks, each in order, eight loads at a time, then
+// the runs in order.
 template <int RUNS>
 __device__ __forceinline__ void finish_bias(const BackwardArgs& p, int block, float* __restrict__ sums) {
   const int64_t n = (int64_t)block * 32 + (threadIdx.x & 31);
   const int run = threadIdx.x >> 5;
   const int64_t per = (p.partials + RUNS - 1) / RUNS, end = min(p.partials, (run + 1) * per);
+  const float* column = p.partial + min(n, p.N - 1);
   float s = 0.0f;
-  if (n < p.N)
-    for (int64_t b = run * per; b < end; ++b) s = s + p.partial[b * p.N + n];
+  for (int64_t b = run * per; b < end; b += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = column[min(b + i, end - 1) * p.N];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (b + i < end) s = s + v[i];
+  }
   sums[threadIdx.x] = s;
   __syncthreads();
   if (run == 0 && n < p.N) {
