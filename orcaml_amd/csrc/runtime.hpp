@@ -9,7 +9,7 @@
 #include <atomic>
 #include <cstdint>
 #include <deque>
-#include <functional>
+#include <initializer_list>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -340,8 +340,18 @@ struct BeResult {
   orca_hip_storage** out;
   bool optional = false;
 };
-int be_run(orca_hip_backend* be, const std::vector<BeOperand>& in, const std::vector<BeResult>& out,
-           const std::function<int(orca_hip_ctx*, float* const* in, float* const* out)>& run);
+typedef int (*BeCall)(void* self, orca_hip_ctx* ctx, float* const* in, float* const* out);
+int be_run(orca_hip_backend* be, std::initializer_list<BeOperand> in, std::initializer_list<BeResult> out, BeCall call,
+           void* self);
+template <class F>
+int be_run(orca_hip_backend* be, std::initializer_list<BeOperand> in, std::initializer_list<BeResult> out, F run) {
+  return be_run(
+      be, in, out,
+      [](void* self, orca_hip_ctx* ctx, float* const* i, float* const* o) {
+        return (*static_cast<F*>(self))(ctx, i, o);
+      },
+      &run);
+}
 
 inline void check_ctx(const orca_hip_ctx* ctx) {
   if (!ctx) fail(ORCA_HIP_ERR_INTERNAL, "null orca_hip_ctx");

@@ -1555,8 +1555,8 @@ Node* take_colsum_waiter(Node* s, size_t cols) {
 
 }  // namespace
 
-int be_run(orca_hip_backend* be, const std::vector<BeOperand>& in, const std::vector<BeResult>& out,
-           const std::function<int(orca_hip_ctx*, float* const* in, float* const* out)>& run) {
+int be_run(orca_hip_backend* be, std::initializer_list<BeOperand> in, std::initializer_list<BeResult> out, BeCall call,
+           void* self) {
   return entry(be, [&](Backend* b) {
     std::vector<Ref> operands, results;
     std::vector<float*> ip, op;
@@ -1576,7 +1576,7 @@ int be_run(orca_hip_backend* be, const std::vector<BeOperand>& in, const std::ve
       results.push_back(Ref(value_node(b, r.n, alloc_buf(b, r.n))));
       op.back() = results.back()->buf->ptr;
     }
-    ck(run(b->ctx, ip.data(), op.data()));
+    ck(call(self, b->ctx, ip.data(), op.data()));
     size_t i = 0;
     for (const BeResult& r : out)
       if (r.out) put(r.out, results[i++].release());

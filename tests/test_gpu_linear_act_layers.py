@@ -7,6 +7,7 @@ import gc
 import numpy as np
 import pytest
 
+from orcaml_amd import _lib
 from orcaml_amd import autodiff as A
 from orcaml_amd.backend import Act8, HipBackend
 from tests.test_gpu_linear_act import U, act64, pack64, product_tol, value64
@@ -286,3 +287,33 @@ def test_calls_from_several_threads(hb):
     for seed in alone:
         for a, b in zip(alone[seed], together[seed]):
             np.testing.assert_array_equal(a, b)
+
+
+def test_refusals_of_the_calls_on_storages(hb):
+    import ctypes
+
+    s = hb.from_f32_slice((3, 8), np.ones(24, np.float32))
+    w = hb.from_f32_slice((8, 4), np.ones(32, np.float32))
+    out = ctypes.c_void_p()
+    p = ctypes.byref(out)
+
+    def refused(word, name, *args):
+        with pytest.raises(ValueError, match=word):
+            _lib.call(name, hb.handle, *args)
+        assert out.value is None
+
+    fwd, bwd = "orca_hip_be_linear_act", "orca_hip_be_linear_act_backward"
+    refused("null storage", fwd, None, w.h, None, None, 3, 4, 8, 0, p, None, None, None)
+    refused("null output", fwd, s.h, w.h, None, None, 3, 4, 8, 0, None, None, None, None)
+    refused("Shape mismatch", fwd, s.h, w.h, None, None, 3, 4, 7, 0, p, None, None, None)
+    refused("Shape mismatch", fwd, s.h, w.h, s.h, None, 3, 4, 8, 0, p, None, None, None)
+    refused("Shape mismatch", fwd, s.h, w.h, None, None, 1 << 61, 4, 8, 0, p, None, None, None)
+    refused("unknown activation", fwd, s.h, w.h, None, None, 3, 4, 8, 9, p, None, None, None)
+    refused("one of z and z8", bwd, s.h, w.h, 3, 8, 4, 2, None, None, None, None, None, p, None, None)
+    refused("one of x and x8", bwd, s.h, w.h, 3, 8, 4, 0, None, None, None, None, None, None, p, None)
+    refused("Shape mismatch", bwd, s.h, w.h, 3, 8, 5, 0, None, None, None, None, None, p, None, None)
+    refused("Shape mismatch", "orca_hip_be_act8_pack", s.h, 3, 9, p)
+    refused("Shape mismatch", "orca_hip_be_act8_unpack", s.h, 1 << 27, 1 << 37, p)
+    refused("null storage", "orca_hip_be_act8_unpack", None, 3, 8, p)
+    with pytest.raises(ValueError, match="null orca_hip_backend"):
+        _lib.call(fwd, None, s.h, w.h, None, None, 3, 4, 8, 0, p, None, None, None)
