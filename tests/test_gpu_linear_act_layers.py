@@ -317,3 +317,28 @@ def test_refusals_of_the_calls_on_storages(hb):
     refused("null storage", "orca_hip_be_act8_unpack", None, 3, 8, p)
     with pytest.raises(ValueError, match="null orca_hip_backend"):
         _lib.call(fwd, None, s.h, w.h, None, None, 3, 4, 8, 0, p, None, None, None)
+
+
+@pytest.mark.parametrize("m", [9, 64, 300])
+def test_checkpoints_change_no_output(hb, m):
+    rng = np.random.default_rng(m)
+    x, w = (hb.from_f32_slice(v.shape, v) for v in (rng.standard_normal((m, 70)).astype(np.float32),
+                                                    rng.standard_normal((70, 90)).astype(np.float32)))
+    plain, _ = hb.linear_act(x, w, None, None, m, 90, 70, "gelu")
+    y, kept = hb.linear_act(x, w, None, None, m, 90, 70, "gelu", ("z", "z8", "y8"))
+    np.testing.assert_array_equal(hb.to_f32_vec(plain), hb.to_f32_vec(y))
+    for k, v in (("z8", kept["z"]), ("y8", y)):  # the epilogue's checkpoints are those of its results
+        np.testing.assert_array_equal(hb.to_f32_vec(hb.act8_unpack(kept[k])),
+                                      hb.to_f32_vec(hb.act8_unpack(hb.act8_pack(v, m, 90))))
+
+
+def test_no_rows(hb):
+    x = hb.from_f32_slice((0, 8), np.zeros((0, 8), np.float32))
+    w = hb.from_f32_slice((8, 4), np.ones((8, 4), np.float32))
+    b = hb.from_f32_slice((1, 4), np.ones((1, 4), np.float32))
+    y, kept = hb.linear_act(x, w, b, None, 0, 4, 8, "silu", ("z", "y8"))
+    assert hb.to_f32_vec(y).size == 0 and hb.to_f32_vec(hb.act8_unpack(kept["y8"])).size == 0
+    g = hb.linear_act_backward(y, w, 0, 4, 8, "silu", z=kept["z"], x=x)
+    assert hb.to_f32_vec(g["dx"]).size == 0
+    assert hb.to_f32_vec(g["dw"]).size == 32 and not np.any(hb.to_f32_vec(g["dw"]))
+    assert hb.to_f32_vec(g["db"]).size == 4 and not np.any(hb.to_f32_vec(g["db"]))
