@@ -98,10 +98,13 @@ class HipStorage:
         h = self.h
         if be is None or not h:
             return
+        # the release lets other threads run, and one may be given the same handle for a new storage: this
+        # wrapper, which its weak reference still reaches until the end of __del__, must be out of sight by then
+        self.h = None
         try:
             live = be._live
             r = live.get(h)
-            if r is not None and r() is None:
+            if r is not None and r() in (None, self):
                 del live[h]
             if be.ctx.handle:
                 rc = be._release_fn(h)
@@ -109,7 +112,6 @@ class HipStorage:
                     _lib.check(rc)
         except Exception:
             pass
-        self.h = None
 
 
 class Act8:
