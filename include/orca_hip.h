@@ -689,8 +689,8 @@ int orca_hip_relu_bw_colsum_noalloc(orca_hip_ctx* ctx, const float* grad, const 
  * least of 7 .. 254 with which no code passes 127, so a value is off by at most half a step and by
  * 2^-7 of the group's largest magnitude (values above 127.5 * 2^121 become 127 * 2^121, groups below
  * 2^-127 become zeros).  A group that holds an infinity or a NaN is stored as NaN as a whole
- * (byte 255).  Bytes between the codes and the step bytes, and behind a group's last row, are not
- * written and mean nothing. */
+ * (byte 255).  Step bytes below 7, which are never written, read as 7.  Bytes between the codes and
+ * the step bytes, and behind a group's last row, are not written and mean nothing. */
 int orca_hip_act8_size(size_t rows, size_t cols, size_t* bytes, size_t* scales_offset);
 int orca_hip_act8_pack(orca_hip_ctx* ctx, const float* x, size_t rows, size_t cols, size_t ldx, void* packed);
 /* dtype: ORCA_HIP_F32 or ORCA_HIP_BF16, of out [rows][ldo]. */

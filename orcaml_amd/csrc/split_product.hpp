@@ -225,7 +225,7 @@ struct LoadCodes {
       const uint32_t w = b[j / 4];
       if (SAFE) return __float_as_uint((float)v[j] * act8_step((w >> (8 * (j % 4))) & 255u));
       const uint32_t e = (j % 4 < 3 ? w << (23 - 8 * (j % 4)) : w >> 1) & 0x7f800000u;
-      return __float_as_uint((float)v[j] * __uint_as_float(e));
+      return __float_as_uint((float)v[j] * __uint_as_float(max(e, 7u << 23)));  // act8_step's least
     };
     if (k == 8)
       s[threadIdx.x / ROWS * PITCH + threadIdx.x % ROWS] = u.h;
