@@ -303,6 +303,7 @@ int orca_hip_storage_len(const orca_hip_storage* s, size_t* n);
 #define ORCA_HIP_STORAGE_TRANSPOSED 2u  /* a lazy transpose view */
 #define ORCA_HIP_STORAGE_MARKED 4u      /* written on the second stream; its first use waits there */
 #define ORCA_HIP_STORAGE_CONSTANT 8u    /* a one-element value known on the host */
+#define ORCA_HIP_STORAGE_WRITTEN 16u    /* an update wrote its memory in place (itself, or a view that shares it) */
 int orca_hip_storage_flags(const orca_hip_storage* s, uint32_t* flags);
 /* The device address of a storage's values, computing them first (a transpose view gives
  * its untransposed buffer).  No counterpart in the reference: for interop and tests. */

@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import contextlib
 import math
+import weakref
 from typing import Iterable
 
 import numpy as np
@@ -620,7 +621,7 @@ class LinearAct(Linear):
     checkpoints instead of in 32 bits: 33/32 bytes a value in place of 4, and a weight gradient at half the
     matrix work, with gradients that see x and the pre-activation to about 2^-8 of the largest
     magnitude among 32 neighbours.  The output then carries its own checkpoint, which a
-    LinearAct(checkpoint=True) above takes as its input's."""
+    LinearAct(checkpoint=True) above takes as its input's while the output has the values it came with."""
 
     def __init__(self, ad: Autodiff, weight: np.ndarray, bias: np.ndarray | None, activation: str = "none",
                  checkpoint: bool = False):
@@ -660,7 +661,7 @@ class LinearAct(Linear):
         if record and ids[1] is not None:
             saved_x = x.storage.primal
             if self.checkpoint:
-                saved_x = x.checkpoint if getattr(x, "checkpoint", None) is not None else be.act8_pack(saved_x, M, K)
+                saved_x = self._checkpoint_of(x) or be.act8_pack(saved_x, M, K)
         z, wp = kept.get("z8", kept.get("z")), w.primal
         want = tuple(k for k, i in zip(("dx", "dw", "db"), ids[:3]) if i is not None)
         same = ids[3] is not None and ids[3] == ids[0]  # y = act(x W) + x: both gradients in one product
@@ -677,8 +678,15 @@ class LinearAct(Linear):
             return grads
         t = Tensor(ad, ad.custom(y, [s for s in (x.storage, w, b, r) if s is not None], backward), out_shape)
         if "y8" in kept:
-            t.checkpoint = kept["y8"]
+            t.checkpoint, t.checkpoint_of = kept["y8"], weakref.ref(y)
         return t
+
+    @staticmethod
+    def _checkpoint_of(x: Tensor):
+        """The checkpoint that a layer's output carries, if it is still that of the tensor's values: not after the
+        tensor was given another storage, or an update wrote this one in place."""
+        s, of = x.storage.primal, getattr(x, "checkpoint_of", None)
+        return x.checkpoint if of is not None and of() is s and not s.written else None
 
 
 class ReLU(Module):

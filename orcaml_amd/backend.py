@@ -33,7 +33,7 @@ from .device import Context
 
 _VP = ctypes.c_void_p
 _byref = ctypes.byref
-_FLAG_PENDING, _FLAG_TRANSPOSED, _FLAG_MARKED, _FLAG_CONSTANT = 1, 2, 4, 8
+_FLAG_PENDING, _FLAG_TRANSPOSED, _FLAG_MARKED, _FLAG_CONSTANT, _FLAG_WRITTEN = 1, 2, 4, 8, 16
 
 
 def _dims(shape):
@@ -85,6 +85,11 @@ class HipStorage:
     def marked(self) -> bool:
         """Written on the second stream; its first use makes the context stream wait."""
         return bool(self.flags() & _FLAG_MARKED)
+
+    @property
+    def written(self) -> bool:
+        """An update wrote its memory in place: what was kept of its values before may be old."""
+        return bool(self.flags() & _FLAG_WRITTEN)
 
     @property
     def ptr(self) -> int:

@@ -89,6 +89,7 @@ struct Buf {
   float* ptr = nullptr;
   size_t bytes = 0;
   std::shared_ptr<Buf> owner;
+  bool written = false;  // an update changed these values, or a view of them, in place
   ~Buf() {
     if (!owner && ptr) (void)orca_hip_free(ctx, ptr);
   }
@@ -1221,6 +1222,11 @@ Node* fold_const(Backend* be, uint8_t op, Node* a, Node* b) {
   return ew(be, op == ORCA_HIP_EW_ADD ? ORCA_HIP_EW_ADD_SCALAR : ORCA_HIP_EW_MUL_SCALAR, std::move(o), n, c);
 }
 
+// An update changes the values in place: of this storage, and so of what it is a view of.
+void mark_written(Node* s) {
+  for (Buf* b = s->buf.get(); b; b = b->owner.get()) b->written = true;
+}
+
 // Before an in-place update: values derived lazily from these storages are computed
 // from their current contents, and their memoised identity reductions are dropped.
 template <class Targets>
@@ -1244,6 +1250,7 @@ void mutating(Backend* be, const Targets& targets) {
       materialize(be, s);  // a constant not yet on the device is uploaded before it changes there
       s->has_const = false;
     }
+    mark_written(s);
   }
 }
 
@@ -1678,6 +1685,8 @@ int orca_hip_storage_flags(const orca_hip_storage* s, uint32_t* flags) {
   if (!x->tshape.empty()) f |= ORCA_HIP_STORAGE_TRANSPOSED;
   if (x->ready) f |= ORCA_HIP_STORAGE_MARKED;
   if (x->has_const) f |= ORCA_HIP_STORAGE_CONSTANT;
+  for (const Buf* b = x->buf.get(); b; b = b->owner.get())
+    if (b->written) f |= ORCA_HIP_STORAGE_WRITTEN;
   *flags = f;
   return ORCA_HIP_OK;
 }
@@ -2206,7 +2215,10 @@ int orca_hip_be_copy_into(orca_hip_backend* be, orca_hip_storage* dst, orca_hip_
     Ref s = plain(b, arg(b, src, "copy_into"));
     if (s->n != d->n) fail_shape("copy_into", std::to_string(d->n) + " elements", std::to_string(s->n) + " elements");
     d->in_place = true;
-    if (s->n) ck(orca_hip_d2d(b->ctx, dptr(b, d), dptr(b, s.get()), 4 * s->n));
+    if (!s->n) return;
+    float* dp = dptr(b, d);
+    mark_written(d);
+    ck(orca_hip_d2d(b->ctx, dp, dptr(b, s.get()), 4 * s->n));
   });
 }
 

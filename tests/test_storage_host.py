@@ -531,3 +531,41 @@ def test_fused_update_on_the_second_stream_changes_no_bit(lib, ctx, kind):
     ref = O.mlp_train(dims, params, x, onehot, O.make_opt(kind, **opt), steps=3)
     for p, r in zip(out[True][3], ref["params"]):
         np.testing.assert_array_equal(p.reshape(r.shape), r)
+
+
+def test_storages_say_when_they_were_written_in_place(hb):
+    """Themselves or through a view, by any update; not by being read."""
+    n = 64
+    v = np.arange(n, dtype=np.float32)
+
+    def fresh():
+        return up(hb, v)
+
+    s, g = fresh(), fresh()
+    hb.add(s, g, (n,))
+    hb.sgd_step_(fresh(), s, n, 0.5)
+    assert not s.written and not g.written
+    hb.sgd_step_(s, g, n, 0.5)
+    assert s.written and not g.written
+    a, m, w = fresh(), fresh(), fresh()
+    hb.adamw_step_(a, g, m, w, n, 0.1, 0.9, 0.999, 1e-8, 0.0, 1)
+    assert a.written and m.written and w.written
+    src, dst = fresh(), fresh()
+    hb.sgd_multi_([(src, dst, g, n)], 0.5)
+    assert dst.written and not src.written and not g.written
+    c = fresh()
+    hb.copy_into(c, g)
+    assert c.written and not g.written
+    base = fresh()
+    one, two = hb.view(base, 0, 32), hb.view(base, 32, 32)
+    assert not base.written and not one.written
+    hb.sgd_step_(two, hb.view(g, 0, 32), 32, 0.5)
+    assert base.written and two.written and not g.written
+    t = fresh()
+    flat = hb.transpose(t, (8, 8), 0, 1)
+    hb.sgd_step_(t, g, n, 0.5)
+    assert t.written and flat.written
+    lazy = hb.add(g, g, (n,))  # computed first, then written
+    hb.sgd_step_(lazy, g, n, 0.5)
+    assert lazy.written
+    np.testing.assert_array_equal(down(hb, lazy), 2 * v - np.float32(0.5) * v)
