@@ -621,16 +621,17 @@ class LinearAct(Linear):
     checkpoints instead of in 32 bits: 33/32 bytes a value in place of 4, and a weight gradient at half the
     matrix work, with gradients that see x and the pre-activation to about 2^-8 of the largest
     magnitude among 32 neighbours.  The output then carries its own checkpoint, which a
-    LinearAct(checkpoint=True) above takes as its input's while the output has the values it came with."""
+    LinearAct(checkpoint=True) above takes as its input's while the output has the values it came with.
+    output_checkpoint=False leaves that out, for an output that no such layer reads (a model's last)."""
 
     def __init__(self, ad: Autodiff, weight: np.ndarray, bias: np.ndarray | None, activation: str = "none",
-                 checkpoint: bool = False):
+                 checkpoint: bool = False, output_checkpoint: bool = True):
         super().__init__(ad, weight, bias)
         if not hasattr(ad.inner, "linear_act"):
             raise OrcaError("LinearAct needs a backend with linear_act")
         if activation not in ad.inner.ACTIVATIONS:
             raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ad.inner.ACTIVATIONS)}")
-        self.activation, self.checkpoint = activation, checkpoint
+        self.activation, self.checkpoint, self.output_checkpoint = activation, checkpoint, output_checkpoint
 
     def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
         K, N = self.in_features, self.out_features
@@ -653,7 +654,7 @@ class LinearAct(Linear):
         keep = ()
         if want_z:
             keep += ("z8",) if self.checkpoint else ("z",)
-        if record and self.checkpoint:
+        if record and self.checkpoint and self.output_checkpoint:
             keep += ("y8",)
         y, kept = be.linear_act(x.storage.primal, w.primal, b.primal if b else None, r.primal if r else None, M, N, K,
                                 act, keep)

@@ -1,6 +1,8 @@
 """The checkpoint that a LinearAct's output carries: taken only while it is that of the tensor's values."""
 from __future__ import annotations
 
+import gc
+
 import numpy as np
 import pytest
 
@@ -84,3 +86,28 @@ def test_the_checkpoint_is_taken_otherwise(hb):
         assert len(packs) == 1
     finally:
         del hb.act8_pack
+
+
+def test_an_output_nobody_reads_takes_no_checkpoint(hb):
+    """A last layer without its output's checkpoint: the same gradients, and its bytes less alive."""
+    rng = np.random.default_rng(8)
+    m, d, f = 256, 64, 128
+    w1, w2 = (rng.standard_normal(s).astype(np.float32) / 8 for s in ((d, f), (f, d)))
+    x = rng.standard_normal((m, d)).astype(np.float32)
+    live, grads = {}, {}
+    for keep in (True, False):
+        ad = A.Autodiff(hb)
+        l1, l2 = A.LinearAct(ad, w1, None, "gelu", True), A.LinearAct(ad, w2, None, "none", True, output_checkpoint=keep)
+        tx = A.Tensor.from_numpy(ad, x)
+        gc.collect()
+        before = hb.ctx.mem_stats()["live"]
+        y = l2(l1(tx))
+        gc.collect()
+        live[keep] = hb.ctx.mem_stats()["live"] - before
+        assert hasattr(y, "checkpoint") == keep
+        y.sum().backward()
+        grads[keep] = [q.weight.tensor.grad().numpy() for q in (l1, l2)]
+        del y, ad, l1, l2, tx
+    assert live[True] - live[False] == m * d * 33 // 32  # a multiple of the allocator's 256 bytes
+    for a, b in zip(grads[True], grads[False]):
+        np.testing.assert_array_equal(a, b)
