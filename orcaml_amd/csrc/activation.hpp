@@ -28,7 +28,9 @@ __device__ __forceinline__ float gauss(float z) { return __builtin_amdgcn_exp2f(
 // Phi(z) = erfc(-z / sqrt 2) / 2, given gauss(z): the upper tail Q(|z|) is gauss(z) times a function that
 // falls smoothly from 1/2, here t times a polynomial in t = 1 / (1 + 0.21 |z|).  Coefficients: a
 // weighted least-squares fit of the scaled erfc, iterated towards equal relative errors on [0, 14]
-// (1.6e-8; in fp32 4e-7).  The tail keeps its relative precision, where 1 + erf would cancel.
+// (2.4e-8; with constants and arithmetic in fp32 4.4e-7).  The tail is a product, so its error stays relative, where
+// 1 + erf would cancel; it grows with gauss's, whose exponent is rounded: 2.5 * 2^-24 of z^2 / 2 (in all 2.0e-6 at
+// z = -6, 7.8e-6 at -12.5), about what z's own rounding to fp32 does to Phi there (z^2 * 2^-24).
 __device__ __forceinline__ float normal_cdf(float z, float g) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.21f, fabsf(z), 1.0f));
   float r = -0.07167498f;
