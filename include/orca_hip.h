@@ -687,9 +687,10 @@ int orca_hip_relu_bw_colsum_noalloc(orca_hip_ctx* ctx, const float* grad, const 
  * of *bytes: int8 codes [rows][cols], then at *scales_offset (optional) the step bytes
  * [ceil(cols / 32)][rows in multiples of 16].  A value is code * 2^(byte - 133), exact in bf16 and
  * f32.  Codes lie in -127 .. 127 and are rounded to nearest, ties to even; a group's byte is the
- * least of 7 .. 254 with which no code passes 127, so a value is off by at most half a step and by
- * 2^-7 of the group's largest magnitude (values above 127.5 * 2^121 become 127 * 2^121, groups below
- * 2^-127 become zeros).  A group that holds an infinity or a NaN is stored as NaN as a whole
+ * least of 7 .. 254 with which no code passes 127, so a value is off by at most half a step, which is at
+ * most 1 / 127.5 of the group's largest magnitude where that is at least 2^-120.  (Below, the least step,
+ * 2^-126, is larger than that takes, and groups up to 2^-127 become zeros; values above 127.5 * 2^121
+ * become 127 * 2^121.)  A group that holds an infinity or a NaN is stored as NaN as a whole
  * (byte 255).  Step bytes below 7, which are never written, read as 7.  Bytes between the codes and
  * the step bytes, and behind a group's last row, are not written and mean nothing. */
 int orca_hip_act8_size(size_t rows, size_t cols, size_t* bytes, size_t* scales_offset);

@@ -619,7 +619,7 @@ class LinearAct(Linear):
 
     checkpoint=True keeps what the backward reads (x and the pre-activation) as 8-bit
     checkpoints instead of in 32 bits: 33/32 bytes a value in place of 4, and a weight gradient at half the
-    matrix work, with gradients that see x and the pre-activation to about 2^-8 of the largest
+    matrix work, with gradients that see x and the pre-activation to at most 1 / 127.5 of the largest
     magnitude among 32 neighbours.  The output then carries its own checkpoint, which a
     LinearAct(checkpoint=True) above takes as its input's while the output has the values it came with.
     output_checkpoint=False leaves that out, for an output that no such layer reads (a model's last)."""

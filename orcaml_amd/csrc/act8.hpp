@@ -3,7 +3,8 @@
 // 32 values along a row share the step 2^(b - 133), b the step byte.  With t the bits of the
 // group's largest magnitude, (t + 0x10000) >> 23 is the biased exponent of t, one more where
 // the mantissa is at least 127.5 / 64: the least b for which every value rounds to a code
-// within 127.  So no value is clipped, and each is off by at most half a step.  The bits of
+// within 127.  So each is off by at most half a step, and none is clipped but where the step would pass
+// the largest, 2^121 (magnitudes above 127.5 * 2^121).  The bits of
 // magnitudes order as the magnitudes do, infinities and NaN above every number: one integer
 // maximum finds all three.
 #pragma once

@@ -1,4 +1,4 @@
-"""The checkpoint format at its ends: step bytes that nothing here writes."""
+"""The checkpoint format at its ends: step bytes that nothing here writes, and the largest error."""
 from __future__ import annotations
 
 import numpy as np
@@ -36,3 +36,16 @@ def test_step_bytes_below_7_read_as_7(ctx, rows, infinite):
     out = L.Mat(ctx, shape=(rows, cols))
     _lib.call("orca_hip_act8_unpack", ctx.handle, x8.ptr, rows, cols, _lib.F32, out.ptr, cols)
     np.testing.assert_array_equal(out.get(), value.astype(np.float32))
+
+
+def test_the_largest_error_of_a_checkpoint(ctx):
+    """Half a step is the most where the group's largest value is 127.5 of the step below: 1 / 127.5 of that value,
+    a little more than 2^-7."""
+    step = 2.0 ** -6
+    x = np.zeros((1, 32), np.float32)
+    x[0, 0], x[0, 1] = 127.5 * step, 0.9999 * step  # too large for that step by half a code: the step doubles
+    X, p, out = L.Mat(ctx, x), L.Packed(ctx, 1, 32), L.Mat(ctx, shape=(1, 32))
+    _lib.call("orca_hip_act8_pack", ctx.handle, X.ptr, 1, 32, 32, p.ptr)
+    _lib.call("orca_hip_act8_unpack", ctx.handle, p.ptr, 1, 32, _lib.F32, out.ptr, 32)
+    err = np.abs(out.get() - x.astype(np.float64)).max() / x.max()
+    assert 2.0 ** -7 < err <= 1 / 127.5
