@@ -640,6 +640,13 @@ class LinearAct(Linear):
         out_shape = x.shape[:-1] + (N,)
         if residual is not None and residual.shape != out_shape:
             raise OrcaError(f"Shape mismatch during linear_act: expected {list(out_shape)}, got {list(residual.shape)}")
+        # load_weights and optimizers replace the parameters; the product sees numbers of elements only
+        if self.weight.tensor.shape != (K, N):
+            raise OrcaError(f"Shape mismatch during linear_act: expected a weight of {[K, N]}, "
+                            f"got {list(self.weight.tensor.shape)}")
+        if self.bias is not None and (_numel(self.bias.tensor.shape) != N or self.bias.tensor.shape[-1] != N):
+            raise OrcaError(f"Shape mismatch during linear_act: expected a bias of {[1, N]}, "
+                            f"got {list(self.bias.tensor.shape)}")
         ad, be, act = x.ad, x.ad.inner, self.activation
         tensors = [x, self.weight.tensor] + ([self.bias.tensor] if self.bias is not None else []) \
             + ([residual] if residual is not None else [])
