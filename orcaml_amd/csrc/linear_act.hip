@@ -375,7 +375,8 @@ struct Plan {
 
 // Microseconds of products on tiles with their k ranges split, on an otherwise idle GPU of 256 CUs: fitted
 // to 7700 products of 1 .. 8192 x 16 .. 4096 x 16 .. 4096, each timed with every tile and split (8 %
-// rms near the best ones; the choice by it takes 1.7 % longer than the best, 11 % in one case of twenty).
+// rms near the best ones; the choice by it takes 1.7 % longer than the best of these tiles and splits, 11 % in one case of
+// twenty).  The fp32 tiles of orca_hip_gemm are no part of it; below 1e9 multiply-adds they are quicker, up to twice.
 // A launch; then the CU with the most blocks, `together` of them at a time: a stage's chain of
 // waits, or its throughput; with splits the second launch, which reads and writes them.
 struct TileCost {
