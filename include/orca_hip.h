@@ -440,6 +440,43 @@ int orca_hip_be_act8_pack(orca_hip_backend* be, orca_hip_storage* x, size_t rows
                           orca_hip_storage** out);
 int orca_hip_be_act8_unpack(orca_hip_backend* be, orca_hip_storage* packed, size_t rows, size_t cols,
                             orca_hip_storage** out);
+/* Norms of rows, dropout and the joint of two residual blocks on storages (orca_hip_norm and its neighbours: their
+ * comments say what each means; no counterpart in the reference).  weight and bias NULL for ones and zeros;
+ * results NULL where not wanted. */
+int orca_hip_be_norm(orca_hip_backend* be, orca_hip_storage* x, size_t rows, size_t cols, int kind, float eps,
+                     orca_hip_storage* weight, orca_hip_storage* bias, orca_hip_storage** y, orca_hip_storage** y8);
+int orca_hip_be_norm_backward(orca_hip_backend* be, orca_hip_storage* dy, orca_hip_storage* x, size_t rows, size_t cols,
+                              int kind, float eps, orca_hip_storage* weight, orca_hip_storage* dx_add,
+                              orca_hip_storage** dx, orca_hip_storage** dweight, orca_hip_storage** dbias);
+int orca_hip_be_dropout(orca_hip_backend* be, orca_hip_storage* x, size_t rows, size_t cols, double p, uint64_t seed,
+                        uint64_t offset, orca_hip_storage** y);
+/* orca_hip_residual_block with storages (gate [groups][cols]). */
+typedef struct {
+  int post;
+  float post_eps;
+  orca_hip_storage* post_weight;
+  orca_hip_storage* post_bias;
+  int next;
+  float next_eps;
+  orca_hip_storage* next_weight;
+  orca_hip_storage* next_bias;
+  orca_hip_storage* gate;
+  size_t groups;
+  float residual_scale;
+  float block_scale;
+  double p;
+  uint64_t seed;
+  uint64_t offset;
+} orca_hip_be_residual_block;
+int orca_hip_be_residual_norm(orca_hip_backend* be, orca_hip_storage* x, orca_hip_storage* f, size_t rows, size_t cols,
+                              const orca_hip_be_residual_block* block, orca_hip_storage** y, orca_hip_storage** u,
+                              orca_hip_storage** u8);
+int orca_hip_be_residual_norm_backward(orca_hip_backend* be, orca_hip_storage* dy, orca_hip_storage* du,
+                                       orca_hip_storage* f, orca_hip_storage* y, size_t rows, size_t cols,
+                                       const orca_hip_be_residual_block* block, orca_hip_storage** dx,
+                                       orca_hip_storage** df, orca_hip_storage** dgate, orca_hip_storage** dpost_weight,
+                                       orca_hip_storage** dpost_bias, orca_hip_storage** dnext_weight,
+                                       orca_hip_storage** dnext_bias);
 /* A new storage holding the same values (device to device). */
 int orca_hip_be_clone(orca_hip_backend* be, orca_hip_storage* s, orca_hip_storage** out);
 /* A flat arena of n floats (set to `value` when fill != 0); view: n floats at `offset` floats of
@@ -732,6 +769,86 @@ typedef struct {
 int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const float* dY, size_t lddy,
                                  const float* W, size_t ldw, const orca_hip_linear_saved* saved, float* dX,
                                  size_t lddx, float* dW, size_t lddw, float* db);
+
+/* ---------------- norms of rows, dropout, and the joint of two residual blocks ----------------
+ * No counterpart in the reference's Backend trait.  Operands are fp32 matrices [rows][cols] with a leading dimension,
+ * and vectors [cols]; sizes, leading dimensions, alignment, overlaps and workspaces are as for
+ * orca_hip_linear_act above: sizes below 2^27 that may be 0, no alignment beyond a float's, no result in
+ * what the call reads but where said.  Forwards and orca_hip_dropout need no workspace.
+ *
+ * unit(v) of a row v of n values:
+ *   ORCA_HIP_NORM_LAYER  (v - mean) / sqrt(mean((v - mean)^2) + eps)
+ *   ORCA_HIP_NORM_RMS    v / sqrt(mean(v^2) + eps)
+ * and norm(v) = unit(v) * weight + bias.  A NaN or an infinity makes its row's outputs NaN or 0, as the
+ * formula in fp32 does, and no other's; so do values whose squares overflow fp32 (beyond 2^63). */
+#define ORCA_HIP_NORM_NONE 0
+#define ORCA_HIP_NORM_LAYER 1
+#define ORCA_HIP_NORM_RMS 2
+typedef struct {
+  int kind;            /* ORCA_HIP_NORM_* */
+  float eps;           /* from 0 on */
+  const float* weight; /* [cols], NULL: ones */
+  const float* bias;   /* [cols], NULL: zeros */
+} orca_hip_norm_params;
+
+/* y = norm(x), and with y8 the 8-bit checkpoint of y (orca_hip_act8_pack's, which the next Linear's weight
+ * gradient can read).  y may be x itself (ldx = ldy). */
+int orca_hip_norm(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* x, size_t ldx,
+                  const orca_hip_norm_params* norm, float* y, size_t ldy, void* y8);
+/* dx = its gradient + dx_add (NULL: none; may be dx itself, ldadd = lddx), dweight[c] = the sum over the rows of
+ * dy * unit(x), dbias[c] = that of dy, each optional.  The statistics are taken again from x: the forward
+ * leaves nothing else.  Sums over rows have a fixed order, so results repeat bit for bit. */
+int orca_hip_norm_backward(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* dy, size_t lddy, const float* x,
+                           size_t ldx, const orca_hip_norm_params* norm, const float* dx_add, size_t ldadd, float* dx,
+                           size_t lddx, float* dweight, float* dbias);
+
+/* y = x / (1 - p) where a value is kept, else 0 (also where x is NaN or infinite).  The value in row r and column c
+ * is kept where word c % 4 of Philox4x32-10 (Salmon et al., SC 2011) at the counter (c / 4, r, offset's low and
+ * high word) under the key (seed's low and high word) is at least rint(p 2^32); 1 - p above is the share of
+ * words that keep.  The mask depends on the seed, the offset and the place alone (not on leading dimensions), so the
+ * gradient of x is the same call on the gradient of y, and no mask is stored.  Calls that are to be independent
+ * take different offsets.  0 <= p <= 1; y may be x itself (ldx = ldy). */
+int orca_hip_dropout(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* x, size_t ldx, double p, uint64_t seed,
+                     uint64_t offset, float* y, size_t ldy);
+
+/* The joint of one residual block with the next:
+ *   y = residual_scale * x + block_scale * gate * dropout(post(f)),   u = next(y)
+ * for the residual stream x and a block's output f; u is the next block's input. */
+typedef struct {
+  orca_hip_norm_params post; /* of f; ORCA_HIP_NORM_NONE: f itself */
+  orca_hip_norm_params next; /* of y; ORCA_HIP_NORM_NONE: no u */
+  const float* gate;         /* [groups][ldgate], or NULL: ones.  Row g is for rows g * rows / groups and on: 1 row for
+                                all (a scale a channel), one a sample, or one a row */
+  size_t groups;             /* divides rows; not read without a gate */
+  size_t ldgate;
+  float residual_scale, block_scale;
+  double p; /* dropout's (orca_hip_dropout); 0: none */
+  uint64_t seed, offset;
+} orca_hip_residual_block;
+/* u is NULL without a next norm; u8 (NULL: not kept) receives u's 8-bit checkpoint.  y may be x itself (ldx = ldy). */
+int orca_hip_residual_norm(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* x, size_t ldx, const float* f,
+                           size_t ldf, const orca_hip_residual_block* block, float* y, size_t ldy, float* u,
+                           size_t ldu, void* u8);
+/* Results of the backward, each optional (NULL).  dgate is [groups][lddgate], with the sum over each of the gate's rows. */
+typedef struct {
+  float* dx;
+  size_t lddx;
+  float* df;
+  size_t lddf;
+  float* dgate;
+  size_t lddgate;
+  float* dpost_weight;
+  float* dpost_bias;
+  float* dnext_weight;
+  float* dnext_bias;
+} orca_hip_residual_grads;
+/* From dy (the gradient that reached y past u; NULL: none) and du (NULL: none, and then no dnext_*): with g the whole
+ * gradient of y, dx = residual_scale * g, and g through gate, dropout and post norm.  f is read for a post norm's
+ * or the gate's gradients and y for du, else they may be NULL.  dx may be dy itself (lddx = lddy). */
+int orca_hip_residual_norm_backward(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* dy, size_t lddy,
+                                    const float* du, size_t lddu, const float* f, size_t ldf, const float* y,
+                                    size_t ldy, const orca_hip_residual_block* block,
+                                    const orca_hip_residual_grads* grads);
 
 /* One AdamW step over flat buffers, same f32 op order as
  * python/orca/optim/adamw.py:71-94 with the f64 scalars rounded to f32 as

@@ -10,10 +10,11 @@ use std::fs;
 use std::path::{Path, PathBuf};
 use std::process::Command;
 
-const SOURCES: [&str; 12] = [
+const SOURCES: [&str; 15] = [
     "runtime_host.cpp",
     "storage.cpp",
     "linear_be.cpp",
+    "norm_be.cpp",
     "runtime.hip",
     "ops.hip",
     "gemm.hip",
@@ -23,6 +24,8 @@ const SOURCES: [&str; 12] = [
     "ewprog.hip",
     "act8.hip",
     "linear_act.hip",
+    "norm.hip",
+    "dropout.hip",
 ];
 
 fn run(cmd: &mut Command) {

@@ -74,6 +74,61 @@ pub struct LinearActOut {
     pub y8: Option<HipStorage>,
 }
 
+/// A norm of rows (ORCA_HIP_NORM_*).
+#[repr(i32)]
+#[derive(Clone, Copy, Debug, PartialEq, Eq)]
+pub enum NormKind {
+    None = 0,
+    Layer = 1,
+    Rms = 2,
+}
+
+/// A norm with its parameters; weight None for ones, bias None for zeros.
+#[derive(Clone, Copy)]
+pub struct Norm<'a> {
+    pub kind: NormKind,
+    pub eps: f32,
+    pub weight: Option<&'a HipStorage>,
+    pub bias: Option<&'a HipStorage>,
+}
+
+/// The joint of two residual blocks: y = residual_scale x + block_scale gate dropout(post(f)), u = next(y).
+#[derive(Clone, Copy)]
+pub struct ResidualBlock<'a> {
+    pub post: Norm<'a>,
+    pub next: Norm<'a>,
+    /// [groups, cols]: each row for rows / groups successive rows.
+    pub gate: Option<&'a HipStorage>,
+    pub groups: usize,
+    pub residual_scale: f32,
+    pub block_scale: f32,
+    pub p: f64,
+    pub seed: u64,
+    pub offset: u64,
+}
+
+impl ResidualBlock<'_> {
+    fn raw(&self) -> ffi::OrcaHipBeResidualBlock {
+        ffi::OrcaHipBeResidualBlock {
+            post: self.post.kind as c_int,
+            post_eps: self.post.eps,
+            post_weight: raw_or_null(self.post.weight),
+            post_bias: raw_or_null(self.post.bias),
+            next: self.next.kind as c_int,
+            next_eps: self.next.eps,
+            next_weight: raw_or_null(self.next.weight),
+            next_bias: raw_or_null(self.next.bias),
+            gate: raw_or_null(self.gate),
+            groups: self.groups,
+            residual_scale: self.residual_scale,
+            block_scale: self.block_scale,
+            p: self.p,
+            seed: self.seed,
+            offset: self.offset,
+        }
+    }
+}
+
 fn raw_or_null(s: Option<&HipStorage>) -> *mut ffi::OrcaHipStorage {
     s.map_or(ptr::null_mut(), |s| s.raw())
 }
@@ -182,6 +237,97 @@ impl HipBackend {
             )
         })?;
         Ok([adopted(dx), adopted(dw), adopted(db)])
+    }
+
+    /// The norm of each row of a [rows, cols] matrix and, if `checkpoint`, its 8-bit checkpoint.
+    pub fn norm(
+        &self,
+        x: &HipStorage,
+        rows: usize,
+        cols: usize,
+        norm: Norm,
+        checkpoint: bool,
+    ) -> Result<(HipStorage, Option<HipStorage>)> {
+        let (mut y, mut y8) = (ptr::null_mut(), ptr::null_mut());
+        check(unsafe {
+            ffi::orca_hip_be_norm(
+                self.be(), x.raw(), rows, cols, norm.kind as c_int, norm.eps, raw_or_null(norm.weight),
+                raw_or_null(norm.bias), &mut y, out_if(checkpoint, &mut y8),
+            )
+        })?;
+        Ok((HipStorage::adopt(y), adopted(y8)))
+    }
+
+    /// Its gradients [dx + dx_add, dweight, dbias] where `want` asks for them.
+    #[allow(clippy::too_many_arguments)]
+    pub fn norm_backward(
+        &self,
+        dy: &HipStorage,
+        x: &HipStorage,
+        rows: usize,
+        cols: usize,
+        norm: Norm,
+        dx_add: Option<&HipStorage>,
+        want: [bool; 3],
+    ) -> Result<[Option<HipStorage>; 3]> {
+        let (mut dx, mut dw, mut db) = (ptr::null_mut(), ptr::null_mut(), ptr::null_mut());
+        check(unsafe {
+            ffi::orca_hip_be_norm_backward(
+                self.be(), dy.raw(), x.raw(), rows, cols, norm.kind as c_int, norm.eps, raw_or_null(norm.weight),
+                raw_or_null(dx_add), out_if(want[0], &mut dx), out_if(want[1], &mut dw), out_if(want[2], &mut db),
+            )
+        })?;
+        Ok([adopted(dx), adopted(dw), adopted(db)])
+    }
+
+    /// x / (1 - p) where the numbers of (seed, offset) keep a value, else 0; its own gradient.
+    pub fn dropout(&self, x: &HipStorage, rows: usize, cols: usize, p: f64, seed: u64, offset: u64) -> Result<HipStorage> {
+        self.out(|o| unsafe { ffi::orca_hip_be_dropout(self.be(), x.raw(), rows, cols, p, seed, offset, o) })
+    }
+
+    /// (y, u, u's 8-bit checkpoint) of the joint of two blocks; u is None without a next norm.
+    pub fn residual_norm(
+        &self,
+        x: &HipStorage,
+        f: &HipStorage,
+        rows: usize,
+        cols: usize,
+        block: &ResidualBlock,
+        checkpoint: bool,
+    ) -> Result<(HipStorage, Option<HipStorage>, Option<HipStorage>)> {
+        let (mut y, mut u, mut packed) = (ptr::null_mut(), ptr::null_mut(), ptr::null_mut());
+        check(unsafe {
+            ffi::orca_hip_be_residual_norm(
+                self.be(), x.raw(), f.raw(), rows, cols, &block.raw(), &mut y,
+                out_if(block.next.kind != NormKind::None, &mut u), out_if(checkpoint, &mut packed),
+            )
+        })?;
+        Ok((HipStorage::adopt(y), adopted(u), adopted(packed)))
+    }
+
+    /// Its gradients [dx, df, dgate, dpost_weight, dpost_bias, dnext_weight, dnext_bias] where `want` asks for them.
+    #[allow(clippy::too_many_arguments)]
+    pub fn residual_norm_backward(
+        &self,
+        dy: Option<&HipStorage>,
+        du: Option<&HipStorage>,
+        f: Option<&HipStorage>,
+        y: Option<&HipStorage>,
+        rows: usize,
+        cols: usize,
+        block: &ResidualBlock,
+        want: [bool; 7],
+    ) -> Result<[Option<HipStorage>; 7]> {
+        let mut o = [ptr::null_mut(); 7];
+        let p = o.as_mut_ptr();
+        let at = |i: usize| if want[i] { unsafe { p.add(i) } } else { ptr::null_mut() };
+        check(unsafe {
+            ffi::orca_hip_be_residual_norm_backward(
+                self.be(), raw_or_null(dy), raw_or_null(du), raw_or_null(f), raw_or_null(y), rows, cols, &block.raw(),
+                at(0), at(1), at(2), at(3), at(4), at(5), at(6),
+            )
+        })?;
+        Ok(o.map(adopted))
     }
 
     /// The 8-bit checkpoint of a [rows, cols] matrix.

@@ -61,6 +61,26 @@ pub struct OptRow {
     pub n: usize,
 }
 
+/// orca_hip_be_residual_block
+#[repr(C)]
+pub struct OrcaHipBeResidualBlock {
+    pub post: c_int,
+    pub post_eps: f32,
+    pub post_weight: *mut OrcaHipStorage,
+    pub post_bias: *mut OrcaHipStorage,
+    pub next: c_int,
+    pub next_eps: f32,
+    pub next_weight: *mut OrcaHipStorage,
+    pub next_bias: *mut OrcaHipStorage,
+    pub gate: *mut OrcaHipStorage,
+    pub groups: usize,
+    pub residual_scale: f32,
+    pub block_scale: f32,
+    pub p: f64,
+    pub seed: u64,
+    pub offset: u64,
+}
+
 extern "C" {
     // ---- context and errors
     pub fn orca_hip_ctx_create(device: c_int, out: *mut *mut OrcaHipCtx) -> c_int;
@@ -518,6 +538,70 @@ extern "C" {
         dx: *mut *mut OrcaHipStorage,
         dw: *mut *mut OrcaHipStorage,
         db: *mut *mut OrcaHipStorage,
+    ) -> c_int;
+    pub fn orca_hip_be_norm(
+        be: *mut OrcaHipBackend,
+        x: *mut OrcaHipStorage,
+        rows: usize,
+        cols: usize,
+        kind: c_int,
+        eps: f32,
+        weight: *mut OrcaHipStorage,
+        bias: *mut OrcaHipStorage,
+        y: *mut *mut OrcaHipStorage,
+        y8: *mut *mut OrcaHipStorage,
+    ) -> c_int;
+    pub fn orca_hip_be_norm_backward(
+        be: *mut OrcaHipBackend,
+        dy: *mut OrcaHipStorage,
+        x: *mut OrcaHipStorage,
+        rows: usize,
+        cols: usize,
+        kind: c_int,
+        eps: f32,
+        weight: *mut OrcaHipStorage,
+        dx_add: *mut OrcaHipStorage,
+        dx: *mut *mut OrcaHipStorage,
+        dweight: *mut *mut OrcaHipStorage,
+        dbias: *mut *mut OrcaHipStorage,
+    ) -> c_int;
+    pub fn orca_hip_be_dropout(
+        be: *mut OrcaHipBackend,
+        x: *mut OrcaHipStorage,
+        rows: usize,
+        cols: usize,
+        p: f64,
+        seed: u64,
+        offset: u64,
+        y: *mut *mut OrcaHipStorage,
+    ) -> c_int;
+    pub fn orca_hip_be_residual_norm(
+        be: *mut OrcaHipBackend,
+        x: *mut OrcaHipStorage,
+        f: *mut OrcaHipStorage,
+        rows: usize,
+        cols: usize,
+        block: *const OrcaHipBeResidualBlock,
+        y: *mut *mut OrcaHipStorage,
+        u: *mut *mut OrcaHipStorage,
+        u_packed: *mut *mut OrcaHipStorage,
+    ) -> c_int;
+    pub fn orca_hip_be_residual_norm_backward(
+        be: *mut OrcaHipBackend,
+        dy: *mut OrcaHipStorage,
+        du: *mut OrcaHipStorage,
+        f: *mut OrcaHipStorage,
+        y: *mut OrcaHipStorage,
+        rows: usize,
+        cols: usize,
+        block: *const OrcaHipBeResidualBlock,
+        dx: *mut *mut OrcaHipStorage,
+        df: *mut *mut OrcaHipStorage,
+        dgate: *mut *mut OrcaHipStorage,
+        dpost_weight: *mut *mut OrcaHipStorage,
+        dpost_bias: *mut *mut OrcaHipStorage,
+        dnext_weight: *mut *mut OrcaHipStorage,
+        dnext_bias: *mut *mut OrcaHipStorage,
     ) -> c_int;
     pub fn orca_hip_be_act8_pack(
         be: *mut OrcaHipBackend,

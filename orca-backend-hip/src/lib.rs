@@ -11,5 +11,5 @@ pub mod error;
 pub mod ffi;
 pub mod storage;
 
-pub use backend::{Activation, HipBackend, Keep, LinearActOut};
+pub use backend::{Activation, HipBackend, Keep, LinearActOut, Norm, NormKind, ResidualBlock};
 pub use storage::HipStorage;

@@ -33,6 +33,7 @@ VIEW_CONTIGUOUS = 0
 VIEW_TRANSPOSED = 1
 
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+NORM_NONE, NORM_LAYER, NORM_RMS = range(3)
 
 EPI_NONE, EPI_BIAS, EPI_BIAS_RELU, EPI_RELU_MASK, EPI_BIAS_RELU_PRE, EPI_RELU_MASK_PRE = range(6)
 
@@ -86,6 +87,35 @@ class LinearSaved(ctypes.Structure):
                 ("dx_add", ctypes.c_void_p), ("ldadd", ctypes.c_size_t)]
 
 
+class NormParams(ctypes.Structure):
+    """orca_hip_norm_params."""
+    _fields_ = [("kind", ctypes.c_int), ("eps", ctypes.c_float), ("weight", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p)]
+
+
+class ResidualBlock(ctypes.Structure):
+    """orca_hip_residual_block."""
+    _fields_ = [("post", NormParams), ("next", NormParams), ("gate", ctypes.c_void_p), ("groups", ctypes.c_size_t),
+                ("ldgate", ctypes.c_size_t), ("residual_scale", ctypes.c_float), ("block_scale", ctypes.c_float),
+                ("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64)]
+
+
+class ResidualGrads(ctypes.Structure):
+    """orca_hip_residual_grads."""
+    _fields_ = [("dx", ctypes.c_void_p), ("lddx", ctypes.c_size_t), ("df", ctypes.c_void_p), ("lddf", ctypes.c_size_t),
+                ("dgate", ctypes.c_void_p), ("lddgate", ctypes.c_size_t), ("dpost_weight", ctypes.c_void_p),
+                ("dpost_bias", ctypes.c_void_p), ("dnext_weight", ctypes.c_void_p), ("dnext_bias", ctypes.c_void_p)]
+
+
+class BeResidualBlock(ctypes.Structure):
+    """orca_hip_be_residual_block: the same with storage handles."""
+    _fields_ = [("post", ctypes.c_int), ("post_eps", ctypes.c_float), ("post_weight", ctypes.c_void_p),
+                ("post_bias", ctypes.c_void_p), ("next", ctypes.c_int), ("next_eps", ctypes.c_float),
+                ("next_weight", ctypes.c_void_p), ("next_bias", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("groups", ctypes.c_size_t), ("residual_scale", ctypes.c_float), ("block_scale", ctypes.c_float),
+                ("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64)]
+
+
 class Optim(ctypes.Structure):
     _fields_ = [
         ("kind", ctypes.c_int),
@@ -123,6 +153,7 @@ _SZP = ctypes.POINTER(ctypes.c_size_t)
 _I = ctypes.c_int
 _F = ctypes.c_float
 _D = ctypes.c_double
+_U64 = ctypes.c_uint64
 
 _EW1 = [_P, _P, _SZP, _SZ, _I, _PP]
 _EW2 = [_P, _P, _P, _SZP, _SZ, _I, _PP]
@@ -187,6 +218,11 @@ SIGNATURES = {
     "orca_hip_trait_max_to_shape_backward": [_P, _P, _P, _P, _SZP, _SZ, _SZP, _SZ, _I, _PP],
     "orca_hip_be_linear_act": [_P, _P, _P, _P, _P, _SZ, _SZ, _SZ, _I, _PP, _PP, _PP, _PP],
     "orca_hip_be_linear_act_backward": [_P, _P, _P, _SZ, _SZ, _SZ, _I, _P, _P, _P, _P, _P, _PP, _PP, _PP],
+    "orca_hip_be_norm": [_P, _P, _SZ, _SZ, _I, _F, _P, _P, _PP, _PP],
+    "orca_hip_be_norm_backward": [_P, _P, _P, _SZ, _SZ, _I, _F, _P, _P, _PP, _PP, _PP],
+    "orca_hip_be_dropout": [_P, _P, _SZ, _SZ, _D, _U64, _U64, _PP],
+    "orca_hip_be_residual_norm": [_P, _P, _P, _SZ, _SZ, ctypes.POINTER(BeResidualBlock), _PP, _PP, _PP],
+    "orca_hip_be_residual_norm_backward": [_P, _P, _P, _P, _P, _SZ, _SZ, ctypes.POINTER(BeResidualBlock)] + [_PP] * 7,
     "orca_hip_be_act8_pack": [_P, _P, _SZ, _SZ, _PP],
     "orca_hip_be_act8_unpack": [_P, _P, _SZ, _SZ, _PP],
     "orca_hip_be_softmax_ce": [_P, _P, _P, _SZ, _SZ, _I, _PP, _PP],
@@ -251,6 +287,12 @@ SIGNATURES = {
     "orca_hip_max_to_shape_backward": [_P, _P, _P, _P, _SZP, _SZ, _SZP, _SZ, _I, _PP],
     "orca_hip_has_nan_or_inf": [_P, _P, _SZ, _I, ctypes.POINTER(_I)],
     "orca_hip_gemm": [_P, _I, _I, _SZ, _SZ, _SZ, _P, _SZ, _P, _SZ, _P, _SZ, ctypes.POINTER(Epilogue)],
+    "orca_hip_norm": [_P, _SZ, _SZ, _P, _SZ, ctypes.POINTER(NormParams), _P, _SZ, _P],
+    "orca_hip_norm_backward": [_P, _SZ, _SZ, _P, _SZ, _P, _SZ, ctypes.POINTER(NormParams), _P, _SZ, _P, _SZ, _P, _P],
+    "orca_hip_dropout": [_P, _SZ, _SZ, _P, _SZ, _D, _U64, _U64, _P, _SZ],
+    "orca_hip_residual_norm": [_P, _SZ, _SZ, _P, _SZ, _P, _SZ, ctypes.POINTER(ResidualBlock), _P, _SZ, _P, _SZ, _P],
+    "orca_hip_residual_norm_backward": [_P, _SZ, _SZ, _P, _SZ, _P, _SZ, _P, _SZ, _P, _SZ,
+                                        ctypes.POINTER(ResidualBlock), ctypes.POINTER(ResidualGrads)],
     "orca_hip_act8_size": [_SZ, _SZ, _SZP, _SZP],
     "orca_hip_act8_pack": [_P, _P, _SZ, _SZ, _SZ, _P],
     "orca_hip_act8_unpack": [_P, _P, _SZ, _SZ, _I, _P, _SZ],

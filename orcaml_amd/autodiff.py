@@ -119,6 +119,29 @@ class Autodiff:
             return run
         return self._record(primal, inputs, node)
 
+    def custom_pair(self, primals, inputs, backward):
+        """custom() for a node with two outputs, which later nodes read independently: backward((g0, g1), backend)
+        gets None for an output that no gradient reached and runs unless that is both."""
+        outs = [AdStorage(p) for p in primals]
+        if not self.grad_enabled:
+            return outs
+        ids = [self.tape.generate_id() for _ in outs]
+        wanted = tuple(s.node_id for s in inputs)
+        if all(i is None for i in wanted):
+            return outs
+
+        def run(tape, be):
+            g = [tape.grads.get(i) for i in ids]
+            if all(v is None for v in g):
+                return
+            for i, gi in zip(wanted, backward(g, be)):
+                if i is not None and gi is not None:
+                    tape.accumulate(i, gi, be)
+        self.tape.push_node(run)
+        for s, i in zip(outs, ids):
+            s.node_id = i
+        return outs
+
     def add(self, a, b, shape):
         primal = self.inner.add(a.primal, b.primal, shape)
 
@@ -536,6 +559,17 @@ class Module:
     def __init__(self):
         object.__setattr__(self, "_parameters", {})
         object.__setattr__(self, "_modules", {})
+        object.__setattr__(self, "training", True)
+
+    def train(self, mode: bool = True) -> "Module":
+        """Sets whether this module and those below it are in training (Dropout and ResidualNorm drop values then)."""
+        object.__setattr__(self, "training", bool(mode))
+        for m in self._modules.values():
+            m.train(mode)
+        return self
+
+    def eval(self) -> "Module":
+        return self.train(False)
 
     def __setattr__(self, name, value):
         if isinstance(value, Parameter):
@@ -695,6 +729,211 @@ class LinearAct(Linear):
         tensor was given another storage, or an update wrote this one in place."""
         s, of = x.storage.primal, getattr(x, "checkpoint_of", None)
         return x.checkpoint if of is not None and of() is s and not s.written else None
+
+
+def _rows_cols(t: Tensor, cols: int, op: str):
+    if not t.shape or t.shape[-1] != cols:
+        raise OrcaError(f"Shape mismatch during {op}: expected [..., {cols}], got {list(t.shape)}")
+    return _numel(t.shape[:-1]), cols
+
+
+def _vector(p: Parameter | None, cols: int, op: str):
+    """The storage of a weight or bias of [1, cols] (load_weights and optimizers replace parameters)."""
+    if p is None:
+        return None
+    if _numel(p.tensor.shape) != cols or p.tensor.shape[-1] != cols:
+        raise OrcaError(f"Shape mismatch during {op}: expected a weight of {[1, cols]}, got {list(p.tensor.shape)}")
+    return p.tensor.storage
+
+
+def _same_ad(ad: Autodiff, tensors) -> None:
+    if any(t is not None and t.ad is not ad for t in tensors):
+        raise OrcaError("Device mismatch: tensors must be on the same device")
+
+
+class _Norm(Module):
+    """A norm of the last dimension: weight [1, features] (ones where None) and an optional bias [1, features]."""
+
+    kind = "none"
+
+    def __init__(self, ad: Autodiff, features: int, weight: np.ndarray | None = None, bias: np.ndarray | None = None,
+                 eps: float = 1e-5, checkpoint: bool = False):
+        super().__init__()
+        if not hasattr(ad.inner, "norm"):
+            raise OrcaError(f"{type(self).__name__} needs a backend with norm")
+        self.features, self.eps, self.checkpoint = features, eps, checkpoint
+        w = np.ones(features, np.float32) if weight is None else np.asarray(weight, np.float32)
+        self.weight = Parameter(Tensor.from_numpy(ad, w.reshape(1, features), requires_grad=True))
+        self.bias = Parameter(Tensor.from_numpy(ad, np.asarray(bias, np.float32).reshape(1, features),
+                                                requires_grad=True)) if bias is not None else None
+
+    def forward(self, x: Tensor) -> Tensor:
+        op, ad, be, kind, eps = self.kind + "_norm", x.ad, x.ad.inner, self.kind, self.eps
+        M, N = _rows_cols(x, self.features, op)
+        w, b = _vector(self.weight, N, op), _vector(self.bias, N, op)
+        _same_ad(ad, [x, self.weight.tensor, self.bias.tensor if self.bias is not None else None])
+        inputs = [s for s in (x.storage, w, b) if s is not None]
+        record = ad.grad_enabled and any(s.node_id is not None for s in inputs)
+        y, y8 = be.norm(x.storage.primal, M, N, kind, eps, w.primal, b.primal if b else None,
+                        self.checkpoint and record)
+        xp, wp = x.storage.primal, w.primal
+        want = tuple(k for k, s in zip(("dx", "dweight", "dbias"), (x.storage, w, b))
+                     if s is not None and s.node_id is not None)
+        names = ("dx", "dweight", "dbias")[:len(inputs)]
+
+        def backward(g, be):
+            out = be.norm_backward(g, xp, M, N, kind, eps, wp, want=want)
+            return [out.get(k) for k in names]
+        t = Tensor(ad, ad.custom(y, inputs, backward), x.shape)
+        if y8 is not None:
+            t.checkpoint, t.checkpoint_of = y8, weakref.ref(y)
+        return t
+
+
+class LayerNorm(_Norm):
+    """(x - mean) / sqrt(variance + eps) * weight + bias over the last dimension, one kernel and one tape node
+    (orca_hip_norm; the reference composes it from trait ops).  checkpoint=True writes the output's 8-bit
+    checkpoint in the same pass, which a LinearAct(checkpoint=True) above takes as its input's."""
+
+    kind = "layer"
+
+
+class RMSNorm(_Norm):
+    """x / sqrt(mean(x^2) + eps) * weight + bias over the last dimension (orca_hip_norm); else as LayerNorm."""
+
+    kind = "rms"
+
+
+class _Draws:
+    """The numbers of a layer's dropout: every call in training takes the next offset under the layer's seed, so
+    that a run repeats from its seeds and no two calls share a mask.  Layers take different seeds."""
+
+    def __init__(self, seed: int):
+        if not 0 <= seed < 2 ** 64:
+            raise ValueError(f"a dropout's seed must be a number of 64 bits, got {seed}")
+        self.seed, self.calls = seed, 0
+
+    def next(self) -> int:
+        self.calls += 1
+        return self.calls - 1
+
+
+def _check_p(p: float) -> float:
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"a dropout's p must be from 0 to 1, got {p}")
+    return float(p)
+
+
+class Dropout(Module):
+    """In training x / (1 - p) where a value is kept and 0 elsewhere, after eval() x itself (orca_hip_dropout).
+    The mask is drawn from (seed, number of the call, place of the value) in the forward and again in the backward,
+    and never stored."""
+
+    def __init__(self, p: float = 0.5, seed: int = 0):
+        super().__init__()
+        self.p, self.draws = _check_p(p), _Draws(seed)
+
+    def forward(self, x: Tensor) -> Tensor:
+        if not self.training or self.p == 0.0:
+            return x
+        if not hasattr(x.ad.inner, "dropout"):
+            raise OrcaError("Dropout needs a backend with dropout")
+        M, N = _numel(x.shape[:-1]), x.shape[-1]
+        p, seed, offset = self.p, self.draws.seed, self.draws.next()
+        y = x.ad.inner.dropout(x.storage.primal, M, N, p, seed, offset)
+
+        def backward(g, be):
+            return [be.dropout(g, M, N, p, seed, offset)]
+        return Tensor(x.ad, x.ad.custom(y, (x.storage,), backward), x.shape)
+
+
+class ResidualNorm(Module):
+    """The joint of one residual block with the next, in one kernel and one tape node (orca_hip_residual_norm):
+
+        y = residual_scale * x + block_scale * gate * dropout(post(f)),   u = next(y)
+
+    called as joint(x, f, gate) on the residual stream x and a block's output f; gives (y, u), or y alone without a
+    next norm.  post and next are LayerNorm or RMSNorm modules over the same features, or None; next's `checkpoint`
+    goes for u.  The gate is a tensor of [..., features] whose leading dimensions have as many elements as x's, or
+    a divisor of that: each of its rows is for as many successive rows of x.  gate_weight gives the joint one row of
+    its own, trained with it (a scale a channel), in place of the argument.  y.grad() is the whole gradient of y, with
+    what came through u."""
+
+    def __init__(self, ad: Autodiff, features: int, post: _Norm | None = None, next: _Norm | None = None,
+                 gate_weight: np.ndarray | None = None, p: float = 0.0, seed: int = 0, residual_scale: float = 1.0,
+                 block_scale: float = 1.0):
+        super().__init__()
+        if not hasattr(ad.inner, "residual_norm"):
+            raise OrcaError("ResidualNorm needs a backend with residual_norm")
+        for n in (post, next):
+            if n is not None and n.features != features:
+                raise OrcaError(f"Shape mismatch during residual_norm: expected norms of {features} features, "
+                                f"got {n.features}")
+        if not (math.isfinite(residual_scale) and residual_scale != 0.0 and math.isfinite(block_scale)):
+            raise ValueError("a joint's scales must be finite, and residual_scale not 0")
+        self.features, self.p, self.draws = features, _check_p(p), _Draws(seed)
+        self.residual_scale, self.block_scale = residual_scale, block_scale
+        self.post, self.next = post, next
+        self.gate = Parameter(Tensor.from_numpy(ad, np.asarray(gate_weight, np.float32).reshape(1, features),
+                                                requires_grad=True)) if gate_weight is not None else None
+
+    def forward(self, x: Tensor, f: Tensor, gate: Tensor | None = None):
+        op, ad, be = "residual_norm", x.ad, x.ad.inner
+        M, N = _rows_cols(x, self.features, op)
+        if f.shape != x.shape:
+            raise OrcaError(f"Shape mismatch during {op}: expected {list(x.shape)}, got {list(f.shape)}")
+        groups = 1
+        if self.gate is not None:
+            if gate is not None:
+                raise OrcaError("residual_norm: a joint with a gate of its own takes no other")
+            _vector(self.gate, N, op)
+            gate = self.gate.tensor
+        elif gate is not None:
+            groups = _rows_cols(gate, N, op)[0]
+            if groups == 0 or M % groups:
+                raise OrcaError(f"Shape mismatch during {op}: expected a gate with a divisor of {M} rows, "
+                                f"got {list(gate.shape)}")
+        post, nxt = self.post, self.next
+        vectors = {k: _vector(p, N, op) for k, p in
+                   (("post_weight", post and post.weight), ("post_bias", post and post.bias),
+                    ("next_weight", nxt and nxt.weight), ("next_bias", nxt and nxt.bias))}
+        _same_ad(ad, [f, gate] + [p.tensor for n in (post, nxt) if n for p in (n.weight, n.bias) if p is not None])
+        p = self.p if self.training else 0.0
+        block = be.ResidualBlock(post=post.kind if post else "none", post_eps=post.eps if post else 0.0,
+                                 next=nxt.kind if nxt else "none", next_eps=nxt.eps if nxt else 0.0,
+                                 gate=gate.storage.primal if gate is not None else None, groups=groups,
+                                 residual_scale=self.residual_scale, block_scale=self.block_scale, p=p,
+                                 seed=self.draws.seed, offset=self.draws.next() if p else 0,
+                                 **{k: s.primal if s is not None else None for k, s in vectors.items()})
+        inputs = {"dx": x.storage, "df": f.storage, "dgate": gate.storage if gate is not None else None,
+                  **{"d" + k: s for k, s in vectors.items()}}
+        inputs = {k: s for k, s in inputs.items() if s is not None}
+        record = ad.grad_enabled and any(s.node_id is not None for s in inputs.values())
+        y, u, u8 = be.residual_norm(x.storage.primal, f.storage.primal, M, N, block,
+                                    nxt is not None and nxt.checkpoint and record)
+        want = tuple(k for k, s in inputs.items() if s.node_id is not None)
+        reads_f = any(k in want for k in ("dgate", "dpost_weight", "dpost_bias")) or ("df" in want and post is not None)
+        fp, yp = f.storage.primal if reads_f else None, y if nxt is not None else None
+        rs, names, node = self.residual_scale, tuple(inputs), {}  # the node holds no more of the operands than that
+
+        def backward(gy, gu, be):
+            asked = want if gu is not None else tuple(k for k in want if not k.startswith("dnext"))
+            # dx is asked for in any case: it is y's own gradient, scaled
+            out = be.residual_norm_backward(gy, gu, fp, yp, M, N, block, want=tuple({*asked, "dx"}))
+            total = out["dx"] if rs == 1.0 else be.mul_scalar(out["dx"], 1.0 / rs, (M, N))
+            ad.tape.grads[node["y"]] = total
+            return [out.get(k) if k in want else None for k in names]
+
+        if nxt is None:
+            ys = ad.custom(y, list(inputs.values()), lambda g, be: backward(g, None, be))
+            node["y"] = ys.node_id
+            return Tensor(ad, ys, x.shape)
+        ys, us = ad.custom_pair((y, u), list(inputs.values()), lambda g, be: backward(*g, be))
+        node["y"] = ys.node_id
+        ty, tu = Tensor(ad, ys, x.shape), Tensor(ad, us, x.shape)
+        if u8 is not None:
+            tu.checkpoint, tu.checkpoint_of = u8, weakref.ref(u)
+        return ty, tu
 
 
 class ReLU(Module):
@@ -1068,5 +1307,6 @@ def argmax_rows(logits: np.ndarray) -> np.ndarray:
     return out
 
 
-__all__ = ["Autodiff", "Tensor", "Tape", "no_grad", "Linear", "LinearAct", "ReLU", "Sequential", "CrossEntropyLoss", "MSELoss",
+__all__ = ["Autodiff", "Tensor", "Tape", "no_grad", "Linear", "LinearAct", "LayerNorm", "RMSNorm", "Dropout",
+           "ResidualNorm", "ReLU", "Sequential", "CrossEntropyLoss", "MSELoss",
            "SGD", "AdamW", "Parameter", "Module", "build_mlp", "argmax_rows", "OrcaError", "math"]

@@ -135,6 +135,24 @@ class Act8:
         return b.value
 
 
+class ResidualBlock:
+    """The parameters of the joint of two residual blocks (include/orca_hip.h, orca_hip_residual_block):
+    y = residual_scale x + block_scale gate dropout(post(f)), u = next(y).  post and next are "none", "layer" or
+    "rms", their weights and biases and the gate [groups, cols] storages or None."""
+
+    __slots__ = ("post", "post_eps", "post_weight", "post_bias", "next", "next_eps", "next_weight", "next_bias", "gate",
+                 "groups", "residual_scale", "block_scale", "p", "seed", "offset")
+
+    def __init__(self, post: str = "none", post_eps: float = 1e-5, post_weight: HipStorage | None = None,
+                 post_bias: HipStorage | None = None, next: str = "none", next_eps: float = 1e-5,
+                 next_weight: HipStorage | None = None, next_bias: HipStorage | None = None,
+                 gate: HipStorage | None = None, groups: int = 1, residual_scale: float = 1.0,
+                 block_scale: float = 1.0, p: float = 0.0, seed: int = 0, offset: int = 0):
+        for name, value in list(locals().items()):
+            if name != "self":
+                setattr(self, name, value)
+
+
 class HipBackend:
     """Drop-in for `GpuBackend` (orca-backend-gpu/src/backend.rs:45-50): an `orca_hip_backend`
     on a context.  The switches select the library's planning (include/orca_hip.h
@@ -449,6 +467,90 @@ class HipBackend:
         _lib.call("orca_hip_be_linear_act_backward", self.handle, self._handle(dy, "linear_act_backward (dy)"),
                   self._handle(w, "linear_act_backward (weight)"), M, N, K, act, *zs, *xs,
                   self._handle(dx_add, "linear_act_backward (dx_add)"), p.get("dx"), p.get("dw"), p.get("db"))
+        return {k: self._wrap(v.value) for k, v in out.items()}
+
+    # ---- norms of rows, dropout, and the joint of two residual blocks ----
+    ResidualBlock = ResidualBlock
+    NORMS = {"none": _lib.NORM_NONE, "layer": _lib.NORM_LAYER, "rms": _lib.NORM_RMS}
+
+    def _norm(self, name: str) -> int:
+        if name not in self.NORMS:
+            raise ValueError(f"unknown norm {name!r}: one of {', '.join(self.NORMS)}")
+        return self.NORMS[name]
+
+    @staticmethod
+    def _word64(value: int, what: str) -> int:
+        if not 0 <= value < 2 ** 64:
+            raise ValueError(f"{what} must be a number of 64 bits, got {value}")
+        return value
+
+    def norm(self, x: HipStorage, rows: int, cols: int, kind: str, eps: float = 1e-5,
+             weight: HipStorage | None = None, bias: HipStorage | None = None, checkpoint: bool = False):
+        """(y, y8): the norm of each row of [rows, cols] (orca_hip_be_norm) and, if checkpoint, its 8-bit
+        checkpoint (else None)."""
+        y, y8 = _VP(), _VP()
+        _lib.call("orca_hip_be_norm", self.handle, self._handle(x, "norm (x)"), rows, cols, self._norm(kind), eps,
+                  self._handle(weight, "norm (weight)"), self._handle(bias, "norm (bias)"), _byref(y),
+                  _byref(y8) if checkpoint else None)
+        return self._wrap(y.value), Act8(self._wrap(y8.value), rows, cols) if checkpoint else None
+
+    def norm_backward(self, dy: HipStorage, x: HipStorage, rows: int, cols: int, kind: str, eps: float = 1e-5,
+                      weight: HipStorage | None = None, dx_add: HipStorage | None = None,
+                      want: tuple = ("dx", "dweight", "dbias")) -> dict:
+        """The gradients that `want` names (orca_hip_be_norm_backward); dx_add is added to dx."""
+        out = self._wanted("norm_backward", want, ("dx", "dweight", "dbias"))
+        p = {k: _byref(v) for k, v in out.items()}
+        _lib.call("orca_hip_be_norm_backward", self.handle, self._handle(dy, "norm_backward (dy)"),
+                  self._handle(x, "norm_backward (x)"), rows, cols, self._norm(kind), eps,
+                  self._handle(weight, "norm_backward (weight)"), self._handle(dx_add, "norm_backward (dx_add)"),
+                  p.get("dx"), p.get("dweight"), p.get("dbias"))
+        return {k: self._wrap(v.value) for k, v in out.items()}
+
+    @staticmethod
+    def _wanted(op: str, want: tuple, names: tuple) -> dict:
+        if not set(want) <= set(names):
+            raise ValueError(f"{op} cannot give {sorted(set(want) - set(names))}")
+        return {k: _VP() for k in want}
+
+    def dropout(self, x: HipStorage, rows: int, cols: int, p: float, seed: int, offset: int) -> HipStorage:
+        """x / (1 - p) where the numbers of (seed, offset) keep a value, else 0 (orca_hip_be_dropout).  The gradient
+        of x is the same call on that of y."""
+        return self._out("orca_hip_be_dropout", self._handle(x, "dropout"), rows, cols, p,
+                         self._word64(seed, "a dropout's seed"), self._word64(offset, "a dropout's offset"))
+
+    def _block(self, b: ResidualBlock):
+        return _lib.BeResidualBlock(
+            post=self._norm(b.post), post_eps=b.post_eps, post_weight=self._handle(b.post_weight, "post weight"),
+            post_bias=self._handle(b.post_bias, "post bias"), next=self._norm(b.next), next_eps=b.next_eps,
+            next_weight=self._handle(b.next_weight, "next weight"), next_bias=self._handle(b.next_bias, "next bias"),
+            gate=self._handle(b.gate, "gate"), groups=b.groups, residual_scale=b.residual_scale,
+            block_scale=b.block_scale, p=b.p, seed=self._word64(b.seed, "a dropout's seed"),
+            offset=self._word64(b.offset, "a dropout's offset"))
+
+    def residual_norm(self, x: HipStorage, f: HipStorage, rows: int, cols: int, block: ResidualBlock,
+                      checkpoint: bool = False):
+        """(y, u, u8) of the joint of two blocks (orca_hip_be_residual_norm): u is None without a next norm, u8
+        without `checkpoint`."""
+        b, y, u, u8 = self._block(block), _VP(), _VP(), _VP()
+        has_u = b.next != _lib.NORM_NONE
+        _lib.call("orca_hip_be_residual_norm", self.handle, self._handle(x, "residual_norm (x)"),
+                  self._handle(f, "residual_norm (f)"), rows, cols, _byref(b), _byref(y), _byref(u) if has_u else None,
+                  _byref(u8) if checkpoint else None)
+        return (self._wrap(y.value), self._wrap(u.value) if has_u else None,
+                Act8(self._wrap(u8.value), rows, cols) if checkpoint else None)
+
+    RESIDUAL_GRADS = ("dx", "df", "dgate", "dpost_weight", "dpost_bias", "dnext_weight", "dnext_bias")
+
+    def residual_norm_backward(self, dy: HipStorage | None, du: HipStorage | None, f: HipStorage | None,
+                               y: HipStorage | None, rows: int, cols: int, block: ResidualBlock,
+                               want: tuple = ("dx", "df")) -> dict:
+        """The gradients that `want` names, of RESIDUAL_GRADS (orca_hip_be_residual_norm_backward)."""
+        out = self._wanted("residual_norm_backward", want, self.RESIDUAL_GRADS)
+        b, p = self._block(block), {k: _byref(v) for k, v in out.items()}
+        op = "residual_norm_backward"
+        _lib.call("orca_hip_be_residual_norm_backward", self.handle, self._handle(dy, op), self._handle(du, op),
+                  self._handle(f, op), self._handle(y, op), rows, cols, _byref(b),
+                  *[p.get(k) for k in self.RESIDUAL_GRADS])
         return {k: self._wrap(v.value) for k, v in out.items()}
 
     # ---- flat arenas and one-launch optimizer passes ----

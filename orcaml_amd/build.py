@@ -18,8 +18,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG_DIR, "csrc")
 BUILD_DIR = os.path.join(PKG_DIR, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "liborca_hip.so")
-SOURCES = ["runtime_host.cpp", "storage.cpp", "linear_be.cpp", "runtime.hip", "ops.hip", "gemm.hip", "fused.hip", "head.hip",
-           "mlp.hip", "ewprog.hip", "act8.hip", "linear_act.hip"]
+SOURCES = ["runtime_host.cpp", "storage.cpp", "linear_be.cpp", "norm_be.cpp", "runtime.hip", "ops.hip", "gemm.hip",
+           "fused.hip", "head.hip", "mlp.hip", "ewprog.hip", "act8.hip", "linear_act.hip", "norm.hip", "dropout.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 

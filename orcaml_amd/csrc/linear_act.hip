@@ -7,14 +7,12 @@
 
 #include "act8.hpp"
 #include "activation.hpp"
+#include "operand.hpp"
 #include "quad.hpp"
 #include "runtime.hpp"
 #include "split_product.hpp"
 
 namespace orca_hip {
-
-void act8_aligned(const void* packed, const char* what);
-
 namespace {
 
 // What becomes of a product: z = acc + bias, y = act(z) + residual.  The residual may be y itself.
@@ -538,43 +536,6 @@ constexpr double kInsideWork = 2.5e7, kInsideWorkPlain = 3e8;
 // checkpoint; the launch that makes them apart takes this long.
 constexpr double kSlopeLaunch = 4.0;
 
-void check_ld(const char* what, size_t ld, size_t cols) {
-  if (ld > size_t(1) << kMaxLdBits)
-    fail_shape(what, "a leading dimension of at most 2^" + std::to_string(kMaxLdBits), std::to_string(ld));
-  if (ld < cols) fail_shape(what, "a leading dimension of at least " + std::to_string(cols), std::to_string(ld));
-}
-void check_sizes(const char* op, size_t M, size_t N, size_t K) {
-  for (size_t v : {M, N, K})
-    if (v >> kMaxSizeBits) fail_shape(op, "sizes below 2^" + std::to_string(kMaxSizeBits), std::to_string(v));
-}
-// An operand's rows of `width` bytes, `ld` bytes apart (one row: a contiguous buffer).
-struct Span {
-  const void* p;
-  size_t rows, width, ld;
-  size_t bytes() const { return rows && width ? (rows - 1) * ld + width : 0; }
-};
-Span matrix_span(const void* p, size_t rows, size_t cols, size_t ld) { return Span{p, rows, 4 * cols, 4 * ld}; }
-Span buffer_span(const void* p, size_t bytes) { return Span{p, 1, bytes, bytes}; }
-// A result must not lie in what the call reads, or in another result.  Columns of one matrix beside each
-// other (the same ld) are apart.
-void check_apart(const char* op, const Span& out, const Span& in) {
-  const auto a = reinterpret_cast<uintptr_t>(out.p), b = reinterpret_cast<uintptr_t>(in.p);
-  if (!out.p || !in.p || !out.bytes() || !in.bytes() || a >= b + in.bytes() || b >= a + out.bytes()) return;
-  if (out.ld == in.ld && out.ld) {
-    const size_t d = (a < b ? b - a : out.ld - (a - b) % out.ld) % out.ld;  // from out's columns to in's
-    if (d >= out.width && out.ld - d >= in.width) return;
-  }
-  fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": an output overlaps another operand");
-}
-// A workspace goes back to the context's allocator when the call returns: a captured graph would write
-// it at every replay, whoever has it then.
-std::unique_ptr<Scratch> workspace(orca_hip_ctx* ctx, size_t bytes, const char* op) {
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  ORCA_HIP_CHECK(hipStreamIsCapturing(ctx->stream, &status));
-  if (status != hipStreamCaptureStatusNone)
-    fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": needs a workspace, which a captured graph cannot keep");
-  return std::make_unique<Scratch>(ctx, bytes);
-}
 void check_act(const char* op, int act) {
   if (act < ORCA_HIP_ACT_NONE || act > ORCA_HIP_ACT_SILU)
     fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": unknown activation " + std::to_string(act));
@@ -591,7 +552,7 @@ int orca_hip_linear_act(orca_hip_ctx* ctx, size_t M, size_t N, size_t K, const f
                         size_t ldw, float* Y, size_t ldy, const orca_hip_linear_epilogue* epi) {
   return guard([&] {
     const char* op = "linear_act";
-    check_sizes(op, M, N, K);
+    check_sizes(op, {M, N, K});
     check_ld("linear_act (x)", ldx, K);
     check_ld("linear_act (weight)", ldw, N);
     check_ld("linear_act (y)", ldy, N);
@@ -678,7 +639,7 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
                                  size_t lddx, float* dW, size_t lddw, float* db) {
   return guard([&] {
     const char* op = "linear_act_backward";
-    check_sizes(op, M, N, K);
+    check_sizes(op, {M, N, K});
     const orca_hip_linear_saved none{};
     const orca_hip_linear_saved& s = saved ? *saved : none;
     check_act(op, s.act);

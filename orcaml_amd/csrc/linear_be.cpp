@@ -1,27 +1,16 @@
 // The fused Linear and the 8-bit checkpoints on storages (orca_hip_be_linear_act and its
 // neighbours): the buffer-level calls under the backend's lock, with contiguous operands.
 #include "act8.hpp"
+#include "operand.hpp"
 #include "runtime.hpp"
 
 using namespace orca_hip;
-
-namespace {
-
-// Elements of a matrix, and of a checkpoint's storage; of sizes that the calls refuse, a number that no storage has.
-size_t count(size_t rows, size_t cols) {
-  return rows >> kMaxSizeBits || cols >> kMaxSizeBits ? SIZE_MAX : rows * cols;
-}
-size_t packed_count(size_t rows, size_t cols) {
-  return count(rows, cols) == SIZE_MAX ? SIZE_MAX : (act8_layout(rows, cols).bytes + 3) / 4;
-}
-
-}  // namespace
 
 extern "C" {
 
 int orca_hip_be_act8_pack(orca_hip_backend* be, orca_hip_storage* x, size_t rows, size_t cols,
                           orca_hip_storage** out) {
-  return be_run(be, {{x, count(rows, cols), "act8_pack"}}, {{packed_count(rows, cols), out}},
+  return be_run(be, {{x, element_count(rows, cols), "act8_pack"}}, {{packed_count(rows, cols), out}},
                 [&](orca_hip_ctx* ctx, float* const* i, float* const* o) {
                   return orca_hip_act8_pack(ctx, i[0], rows, cols, cols, o[0]);
                 });
@@ -29,7 +18,7 @@ int orca_hip_be_act8_pack(orca_hip_backend* be, orca_hip_storage* x, size_t rows
 
 int orca_hip_be_act8_unpack(orca_hip_backend* be, orca_hip_storage* packed, size_t rows, size_t cols,
                             orca_hip_storage** out) {
-  return be_run(be, {{packed, packed_count(rows, cols), "act8_unpack"}}, {{count(rows, cols), out}},
+  return be_run(be, {{packed, packed_count(rows, cols), "act8_unpack"}}, {{element_count(rows, cols), out}},
                 [&](orca_hip_ctx* ctx, float* const* i, float* const* o) {
                   return orca_hip_act8_unpack(ctx, i[0], rows, cols, ORCA_HIP_F32, o[0], cols);
                 });
@@ -38,10 +27,10 @@ int orca_hip_be_act8_unpack(orca_hip_backend* be, orca_hip_storage* packed, size
 int orca_hip_be_linear_act(orca_hip_backend* be, orca_hip_storage* x, orca_hip_storage* w, orca_hip_storage* bias,
                            orca_hip_storage* residual, size_t M, size_t N, size_t K, int act, orca_hip_storage** y,
                            orca_hip_storage** z, orca_hip_storage** z8, orca_hip_storage** y8) {
-  const size_t mn = count(M, N), packed = packed_count(M, N);
+  const size_t mn = element_count(M, N), packed = packed_count(M, N);
   return be_run(be,
-                {{x, count(M, K), "linear_act (x)"},
-                 {w, count(K, N), "linear_act (weight)"},
+                {{x, element_count(M, K), "linear_act (x)"},
+                 {w, element_count(K, N), "linear_act (weight)"},
                  {bias, N, "linear_act (bias)", true},
                  {residual, mn, "linear_act (residual)", true}},
                 {{mn, y}, {mn, z, true}, {packed, z8, true}, {packed, y8, true}},
@@ -63,7 +52,7 @@ int orca_hip_be_linear_act_backward(orca_hip_backend* be, orca_hip_storage* dy, 
                                     size_t N, size_t K, int act, orca_hip_storage* z, orca_hip_storage* z8,
                                     orca_hip_storage* x, orca_hip_storage* x8, orca_hip_storage* dx_add,
                                     orca_hip_storage** dx, orca_hip_storage** dw, orca_hip_storage** db) {
-  const size_t mn = count(M, N), mk = count(M, K), kn = count(K, N);
+  const size_t mn = element_count(M, N), mk = element_count(M, K), kn = element_count(K, N);
   return be_run(be,
                 {{dy, mn, "linear_act_backward (dy)"},
                  {w, kn, "linear_act_backward (weight)"},

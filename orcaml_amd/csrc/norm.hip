@@ -1,0 +1,777 @@
+// Norms of rows and the joint of two residual blocks, with their backward passes (orca_hip_norm,
+// orca_hip_residual_norm and their _backward).
+//
+// The formulas, for a row v of n values: unit(v) = (v - mean) r with r = 1 / sqrt(mean((v - mean)^2) + eps), or v r
+// with r = 1 / sqrt(mean(v^2) + eps).  norm(v) = unit(v) w + b.  Its backward, with e = dv w:
+// r (e - mean(e) - unit mean(e unit)), without mean(e) for the mean square; dw = sum dv unit, db = sum dv.
+// The joint: y = s x + t gate drop(post(f)), u = next(y).  Its backward: g = dy + next's of du, dx = s g,
+// dv = t gate keep g, df = post's of dv, dgate = sum over the gate row's rows of t keep g post(f).
+//
+// The backward takes the statistics again from the rows that it reads anyway, and draws the dropout's numbers
+// again: nothing is kept between the passes.  Everything is bound by HBM.  Means and sums are fp32: a variance is
+// taken around the row's mean, corrected by what that mean was off by (sum of the differences), so that a large
+// common part of a row costs no digits.  Sums over rows run per block in row order, then over the blocks'
+// partial sums in a second launch: no atomics, the same bits every time.
+#include <algorithm>
+#include <cmath>
+#include <memory>
+#include <string>
+
+#include "act8.hpp"
+#include "ce_row.hpp"
+#include "operand.hpp"
+#include "philox.hpp"
+#include "quad.hpp"
+#include "runtime.hpp"
+#include "slab.hpp"
+
+namespace orca_hip {
+namespace {
+
+struct Norm {
+  int kind = ORCA_HIP_NORM_NONE;
+  float eps = 0.0f;
+  const float* w = nullptr;  // null: ones
+  const float* b = nullptr;  // null: zeros
+};
+
+struct NormForward {
+  int64_t rows, cols;
+  const float* x;
+  int64_t ldx;
+  const float* f;  // the block's output (a norm alone has none: y is x then, and not written)
+  int64_t ldf;
+  float* y;
+  int64_t ldy;
+  float* u;
+  int64_t ldu;
+  Act8 u8;
+  Norm post, next;
+  const float* gate;
+  int64_t ldgate, gate_rows;  // rows of f for each of the gate's
+  float rs, bs;
+  Dropout drop;
+};
+
+// Sums over the rows that a backward gives.
+enum { kSumGate, kSumPostW, kSumPostB, kSumNextW, kSumNextB, kSums };
+
+struct NormBackward {
+  int64_t rows, cols;
+  const float* dy;  // may be null
+  int64_t lddy;
+  const float* du;  // null: nothing through u
+  int64_t lddu;
+  const float* f;
+  int64_t ldf;
+  const float* y;
+  int64_t ldy;
+  Norm post, next;
+  const float* gate;
+  int64_t ldgate, gate_rows;
+  float rs, bs;
+  Dropout drop;
+  float* dx;
+  int64_t lddx;
+  float* df;
+  int64_t lddf;
+  float* dgate;
+  int64_t lddgate;
+  // A block adds up whole pieces of rows: per_group pieces of piece_rows rows for each of `groups` groups of
+  // group_rows (one group but where each row of the gate has its own sum).
+  int64_t group_rows, groups, per_group, piece_rows;
+  bool gate_each;     // the gate's gradient row by row, without a sum
+  bool gate_grouped;  // its sums are those of the groups
+  float* sum[kSums];  // where a sum goes: the result itself (one block), or a block's first partial sum
+  int64_t sum_step;   // from one block's to the next one's
+  float* stats;       // [rows][8] (norm_stats_kernel)
+};
+
+// ---------------------------------------------------------------- rows
+// A row is held by NW waves.  One barrier a sum: successive ones take turns in LDS.
+template <int NW>
+struct Team {
+  float* lds;  // 2 x NW x 4 floats
+  int turn = 0;
+  template <int N>
+  __device__ __forceinline__ void sum(float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if constexpr (NW > 1) {
+      float* p = lds + turn * (NW * 4);
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i * NW + (threadIdx.x >> 6)] = v[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[i] = p[i * NW];
+#pragma unroll
+        for (int k = 1; k < NW; ++k) v[i] += p[i * NW + k];
+      }
+    }
+  }
+};
+
+// unit = ((v - mean) - rest) r
+struct Stats {
+  float mean, rest, r;
+  __device__ __forceinline__ float unit(float v) const { return ((v - mean) - rest) * r; }
+};
+
+__device__ __forceinline__ floatx4 splat(float v) { return floatx4{v, v, v, v}; }
+__device__ __forceinline__ floatx4 load4(const float* row, int64_t c, int64_t cols) {
+  if (c + 4 <= cols) return *reinterpret_cast<const floatx4_u*>(row + c);
+  floatx4 v = splat(0.0f);
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (c + j < cols) v[j] = row[c + j];
+  return v;
+}
+__device__ __forceinline__ void store4(float* row, int64_t c, int64_t cols, floatx4 v) {
+  if (c + 4 <= cols) {
+    *reinterpret_cast<floatx4_u*>(row + c) = v;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+    if (c + j < cols) row[c + j] = v[j];
+}
+__device__ __forceinline__ floatx4 weight4(const float* w, int64_t c, int64_t cols, float none) {
+  return w ? load4(w, c, cols) : splat(none);
+}
+
+// ---------------------------------------------------------------- rows of any length
+constexpr int kStream = 256;  // threads of a block, 4 columns each at a time
+
+__device__ __forceinline__ Stats stream_stats(const Norm& n, const float* row, int64_t cols, Team<4>& team) {
+  Stats s{0.0f, 0.0f, 0.0f};
+  const float count = (float)cols;
+  if (n.kind == ORCA_HIP_NORM_LAYER) {
+    float t[1] = {0.0f};
+    for (int64_t c = threadIdx.x * 4; c < cols; c += kStream * 4) {
+      const floatx4 v = load4(row, c, cols);
+      t[0] += (v.x + v.y) + (v.z + v.w);
+    }
+    team.sum(t);
+    s.mean = t[0] / count;
+  }
+  float t[2] = {0.0f, 0.0f};
+  for (int64_t c = threadIdx.x * 4; c < cols; c += kStream * 4) {
+    const floatx4 v = load4(row, c, cols);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d = c + j < cols ? v[j] - s.mean : 0.0f;
+      t[0] += d;
+      t[1] = fmaf(d, d, t[1]);
+    }
+  }
+  team.sum(t);
+  float var = t[1] / count;
+  if (n.kind == ORCA_HIP_NORM_LAYER) {
+    s.rest = t[0] / count;
+    var = fmaxf(fmaf(-s.rest, s.rest, var), 0.0f);
+  }
+  s.r = 1.0f / sqrtf(var + n.eps);
+  return s;
+}
+
+template <bool JOINT>
+__global__ void __launch_bounds__(kStream) norm_stream_kernel(NormForward a) {
+  __shared__ float lds[2 * 4 * 4];
+  Team<4> team{lds};
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float* y = a.x + row * a.ldx;
+    if (JOINT) {
+      const float *x = y, *f = a.f + row * a.ldf, *gate = a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr;
+      float* out = a.y + row * a.ldy;
+      Stats s{0.0f, 0.0f, 1.0f};
+      if (a.post.kind != ORCA_HIP_NORM_NONE) s = stream_stats(a.post, f, a.cols, team);
+      for (int64_t c = threadIdx.x * 4; c < a.cols; c += kStream * 4) {
+        floatx4 v = load4(f, c, a.cols);
+        if (a.post.kind != ORCA_HIP_NORM_NONE) {
+          const floatx4 w = weight4(a.post.w, c, a.cols, 1.0f), b = weight4(a.post.b, c, a.cols, 0.0f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = fmaf(s.unit(v[j]), w[j], b[j]);
+        }
+        const floatx4 g = weight4(gate, c, a.cols, 1.0f), xv = load4(x, c, a.cols);
+        Words words{};
+        if (a.drop.on) words = dropout_words(a.drop, row, c / 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float t = v[j] * (g[j] * (a.bs * a.drop.scale));
+          v[j] = fmaf(a.rs, xv[j], !a.drop.on || dropout_keeps(a.drop, words, j) ? t : 0.0f);
+        }
+        store4(out, c, a.cols, v);
+      }
+      y = out;  // a thread reads back what it wrote itself
+    }
+    if (a.next.kind == ORCA_HIP_NORM_NONE) continue;
+    const Stats s = stream_stats(a.next, y, a.cols, team);
+    float* u = a.u + row * a.ldu;
+    for (int64_t c0 = 0; c0 < a.cols; c0 += kStream * 4) {
+      const int64_t c = c0 + threadIdx.x * 4;
+      floatx4 v = splat(0.0f);
+      if (c < a.cols) {
+        v = load4(y, c, a.cols);
+        const floatx4 w = weight4(a.next.w, c, a.cols, 1.0f), b = weight4(a.next.b, c, a.cols, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = fmaf(s.unit(v[j]), w[j], b[j]);
+        store4(u, c, a.cols, v);
+      }
+      if (a.u8.codes) {
+        const Quad q = quad_of(c, a.cols);
+        const uint32_t byte = quad_byte(v, q);
+        if (q.have > 0) {
+          store_codes(a.u8.codes + row * a.u8.cols, q, v, byte);
+          if ((threadIdx.x & 7) == 0) a.u8.scales[q.group * a.u8.ld + row] = (uint8_t)byte;
+        }
+      }
+    }
+  }
+}
+
+// What a backward needs to know of each row: (mean, r, mean(e), mean(e unit)) of the next norm, then of the post
+// norm.
+__global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, bool block) {
+  __shared__ float lds[2 * 4 * 4];
+  Team<4> team{lds};
+  const float count = (float)a.cols;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float *y = a.y + row * a.ldy, *du = a.du + row * a.lddu, *dy = a.dy + row * a.lddy;
+    Stats sy{0.0f, 0.0f, 0.0f};
+    float c1 = 0.0f, c2 = 0.0f;
+    if (a.du) {
+      sy = stream_stats(a.next, y, a.cols, team);
+      sy.mean += sy.rest;
+      sy.rest = 0.0f;
+      float t[2] = {0.0f, 0.0f};
+      for (int64_t c = threadIdx.x * 4; c < a.cols; c += kStream * 4) {
+        const floatx4 v = load4(y, c, a.cols), d = load4(du, c, a.cols), w = weight4(a.next.w, c, a.cols, 1.0f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (c + j >= a.cols) break;
+          const float e = d[j] * w[j];
+          t[0] += e;
+          t[1] = fmaf(e, sy.unit(v[j]), t[1]);
+        }
+      }
+      team.sum(t);
+      c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? t[0] / count : 0.0f;
+      c2 = t[1] / count;
+    }
+    Stats sf{0.0f, 0.0f, 0.0f};
+    float p1 = 0.0f, p2 = 0.0f;
+    if (block && a.post.kind != ORCA_HIP_NORM_NONE) {
+      const float *f = a.f + row * a.ldf, *gate = a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr;
+      sf = stream_stats(a.post, f, a.cols, team);
+      sf.mean += sf.rest;
+      sf.rest = 0.0f;
+      float t[2] = {0.0f, 0.0f};
+      for (int64_t c = threadIdx.x * 4; c < a.cols; c += kStream * 4) {
+        floatx4 g = splat(0.0f);
+        if (a.dy) g = load4(dy, c, a.cols);
+        if (a.du) {
+          const floatx4 v = load4(y, c, a.cols), d = load4(du, c, a.cols), w = weight4(a.next.w, c, a.cols, 1.0f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) g[j] += sy.r * (fmaf(-sy.unit(v[j]), c2, d[j] * w[j]) - c1);
+        }
+        const floatx4 v = load4(f, c, a.cols), w = weight4(a.post.w, c, a.cols, 1.0f);
+        const floatx4 gt = weight4(gate, c, a.cols, 1.0f);
+        Words words{};
+        if (a.drop.on) words = dropout_words(a.drop, row, c / 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (c + j >= a.cols) break;
+          const bool kept = !a.drop.on || dropout_keeps(a.drop, words, j);
+          const float e = kept ? g[j] * (a.bs * a.drop.scale) * gt[j] * w[j] : 0.0f;
+          t[0] += e;
+          t[1] = fmaf(e, sf.unit(v[j]), t[1]);
+        }
+      }
+      team.sum(t);
+      p1 = a.post.kind == ORCA_HIP_NORM_LAYER ? t[0] / count : 0.0f;
+      p2 = t[1] / count;
+    }
+    if (threadIdx.x == 0) {
+      floatx4* s = reinterpret_cast<floatx4*>(a.stats + row * 8);
+      s[0] = floatx4{sy.mean, sy.r, c1, c2};
+      s[1] = floatx4{sf.mean, sf.r, p1, p2};
+    }
+  }
+}
+
+// The gradients, a block for 1024 columns (blockIdx.x) and a piece of rows, from the rows' statistics.
+__global__ void __launch_bounds__(kStream) norm_strip_kernel(NormBackward a, bool block) {
+  const int64_t c = ((int64_t)blockIdx.x * kStream + threadIdx.x) * 4;
+  if (c >= a.cols) return;
+  const floatx4 zero = splat(0.0f);
+  const floatx4 wn = weight4(a.next.w, c, a.cols, 1.0f), wp = weight4(a.post.w, c, a.cols, 1.0f);
+  const floatx4 bp = weight4(a.post.b, c, a.cols, 0.0f);
+  const bool post = a.post.kind != ORCA_HIP_NORM_NONE;
+  floatx4 sum[kSums] = {zero, zero, zero, zero, zero};
+  for (int64_t unit = blockIdx.y; unit < a.groups * a.per_group; unit += gridDim.y) {
+    const int64_t group = unit / a.per_group, r0 = group * a.group_rows + unit % a.per_group * a.piece_rows;
+    const int64_t r1 = min(r0 + a.piece_rows, (group + 1) * a.group_rows);
+    for (int64_t row = r0; row < r1; ++row) {
+      floatx4 s[2] = {zero, zero};
+      if (a.stats) {
+        s[0] = reinterpret_cast<const floatx4*>(a.stats + row * 8)[0];
+        s[1] = reinterpret_cast<const floatx4*>(a.stats + row * 8)[1];
+      }
+      floatx4 g = zero;
+      if (a.dy) g = load4(a.dy + row * a.lddy, c, a.cols);
+      if (a.du) {
+        const floatx4 v = load4(a.y + row * a.ldy, c, a.cols), d = load4(a.du + row * a.lddu, c, a.cols);
+        const Stats sy{s[0].x, 0.0f, s[0].y};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float unit = sy.unit(v[j]);
+          g[j] += sy.r * (fmaf(-unit, s[0].w, d[j] * wn[j]) - s[0].z);
+          sum[kSumNextW][j] = fmaf(d[j], unit, sum[kSumNextW][j]);
+          sum[kSumNextB][j] += d[j];
+        }
+      }
+      if (a.dx) store4(a.dx + row * a.lddx, c, a.cols, floatx4{g.x * a.rs, g.y * a.rs, g.z * a.rs, g.w * a.rs});
+      if (!block) continue;
+      floatx4 v = zero, unit = zero, dv, each;
+      if (a.f) v = load4(a.f + row * a.ldf, c, a.cols);
+      if (post) {
+        const Stats sf{s[1].x, 0.0f, s[1].y};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          unit[j] = sf.unit(v[j]);
+          v[j] = fmaf(unit[j], wp[j], bp[j]);
+        }
+      }
+      const floatx4 gate = weight4(a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr, c, a.cols, 1.0f);
+      Words words{};
+      if (a.drop.on) words = dropout_words(a.drop, row, c / 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool kept = !a.drop.on || dropout_keeps(a.drop, words, j);
+        dv[j] = kept ? g[j] * (a.bs * a.drop.scale) : 0.0f;
+        each[j] = kept ? dv[j] * v[j] : 0.0f;
+        sum[kSumGate][j] += each[j];
+        dv[j] *= gate[j];
+        sum[kSumPostB][j] += dv[j];
+        if (post) {
+          sum[kSumPostW][j] = fmaf(dv[j], unit[j], sum[kSumPostW][j]);
+          dv[j] = s[1].y * (fmaf(-unit[j], s[1].w, dv[j] * wp[j]) - s[1].z);
+        }
+      }
+      if (a.gate_each) store4(a.dgate + row * a.lddgate, c, a.cols, each);
+      if (a.df) store4(a.df + row * a.lddf, c, a.cols, dv);
+    }
+    if (a.gate_grouped && a.per_group == 1 && a.dgate) {
+      store4(a.dgate + group * a.lddgate, c, a.cols, sum[kSumGate]);
+      sum[kSumGate] = zero;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kSums; ++i)
+    if (a.sum[i]) store4(a.sum[i] + blockIdx.y * a.sum_step, c, a.cols, sum[i]);
+}
+
+// ---------------------------------------------------------------- the blocks' partial sums
+struct NormFinish {
+  int64_t cols, blocks, step;  // of the partial sums; `step` floats from one block's to the next one's
+  int count;                   // sums over all blocks
+  const float* from[kSums];
+  float* to[kSums];
+  const float* gate_from;  // and over each group's blocks
+  float* dgate;
+  int64_t lddgate, groups, per_group;
+};
+// A block adds up 64 columns: 16 threads of four columns, 16 of each for every 16th partial sum.
+__global__ void __launch_bounds__(256) norm_finish_kernel(NormFinish a) {
+  __shared__ floatx4 lds[16][16];
+  const int q = threadIdx.x & 15, k = threadIdx.x >> 4;
+  const int64_t c = ((int64_t)blockIdx.x * 16 + q) * 4;
+  for (int64_t i = blockIdx.y; i < a.count + a.groups; i += gridDim.y) {
+    const int64_t group = i - a.count;
+    const float* from = group < 0 ? a.from[i] : a.gate_from + group * a.per_group * a.step;
+    float* to = group < 0 ? a.to[i] : a.dgate + group * a.lddgate;
+    const int64_t blocks = group < 0 ? a.blocks : a.per_group;
+    floatx4 t = splat(0.0f);
+    if (c < a.cols)
+      for (int64_t b = k; b < blocks; b += 16) t += load4(from + b * a.step, c, a.cols);
+    lds[k][q] = t;
+    __syncthreads();
+    if (k == 0 && c < a.cols) {
+#pragma unroll
+      for (int j = 1; j < 16; ++j) t += lds[j][q];
+      store4(to, c, a.cols, t);
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- host
+void check_norm(const char* op, const orca_hip_norm_params& n, bool none) {
+  if (n.kind < (none ? ORCA_HIP_NORM_NONE : ORCA_HIP_NORM_LAYER) || n.kind > ORCA_HIP_NORM_RMS)
+    fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": unknown norm " + std::to_string(n.kind));
+  if (n.kind != ORCA_HIP_NORM_NONE && !(n.eps >= 0.0f && n.eps < INFINITY))
+    fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": eps must be a finite number from 0 on");
+}
+Norm norm_of(const orca_hip_norm_params& n) {
+  Norm r;
+  r.kind = n.kind;
+  if (n.kind == ORCA_HIP_NORM_NONE) return r;
+  r.eps = n.eps;
+  r.w = n.weight;
+  r.b = n.bias;
+  return r;
+}
+void check_block(const char* op, size_t rows, size_t cols, const orca_hip_residual_block& b) {
+  check_norm(op, b.post, true);
+  check_norm(op, b.next, true);
+  if (!(b.p >= 0.0 && b.p <= 1.0))
+    fail(ORCA_HIP_ERR_INTERNAL, std::string(op) + ": a dropout's p must be from 0 to 1");
+  if (!b.gate) return;
+  if (!b.groups || b.groups >> kMaxSizeBits || rows % b.groups)
+    fail_shape(op, "a number of gate rows that divides " + std::to_string(rows), std::to_string(b.groups));
+  check_ld((std::string(op) + " (gate)").c_str(), b.ldgate, cols);
+}
+Span vector_span(const float* p, size_t cols) { return buffer_span(p, 4 * cols); }
+
+// The operands of a call with what they are, for the checks that each call makes.
+struct Operand {
+  Span span;
+  const char* what;
+};
+void check_operands(orca_hip_ctx* ctx, const char* op, std::initializer_list<Operand> operands) {
+  for (const Operand& o : operands)
+    check_extent(ctx, o.span.p, o.span.bytes(), (std::string(op) + " (" + o.what + ")").c_str());
+}
+
+constexpr unsigned kMaxBlocks = 1u << 20;  // of 256 threads and more; the kernels step over the rest
+
+void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
+  const dim3 grid((unsigned)std::min<int64_t>(a.rows, kMaxBlocks));
+  if (joint)
+    hipLaunchKernelGGL(norm_stream_kernel<true>, grid, dim3(kStream), 0, ctx->stream, a);
+  else
+    hipLaunchKernelGGL(norm_stream_kernel<false>, grid, dim3(kStream), 0, ctx->stream, a);
+  ORCA_HIP_CHECK(hipGetLastError());
+}
+
+void launch_finish(orca_hip_ctx* ctx, const NormFinish& f) {
+  const int64_t outs = f.count + f.groups;
+  if (!outs) return;
+  hipLaunchKernelGGL(norm_finish_kernel, dim3((unsigned)((f.cols + 63) / 64), (unsigned)std::min<int64_t>(outs, 32768)),
+                     dim3(256), 0, ctx->stream, f);
+  ORCA_HIP_CHECK(hipGetLastError());
+}
+
+// Runs a backward; `to` are the results of the sums (null: not wanted).  dgate has `gate_rows` rows.
+void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSums], int64_t gate_rows, const char* op) {
+  if (!a.rows) {  // sums of nothing
+    NormFinish fin{};
+    fin.cols = a.cols;
+    for (int i = 0; i < kSums; ++i)
+      if (to[i] && i != kSumGate) fin.to[fin.count++] = to[i];
+    if (to[kSumGate]) {
+      fin.dgate = to[kSumGate];
+      fin.lddgate = a.lddgate;
+      fin.groups = gate_rows;
+    }
+    return launch_finish(ctx, fin);
+  }
+  a.gate_rows = gate_rows ? a.rows / gate_rows : a.rows;
+  a.gate_each = to[kSumGate] && a.gate_rows == 1;
+  const bool gate_sum = to[kSumGate] && !a.gate_each;
+  // by the gate's rows also where their gradient is not wanted: the other sums then have the same bits
+  a.gate_grouped = a.gate_rows != 1 && a.gate_rows != a.rows;
+  a.groups = a.gate_grouped ? a.rows / a.gate_rows : 1;
+  a.group_rows = a.gate_grouped ? a.gate_rows : a.rows;
+  const bool block = a.df || to[kSumGate] || to[kSumPostW] || to[kSumPostB];
+  const int64_t strips = (a.cols + kStream * 4 - 1) / (kStream * 4);
+  int64_t blocks = std::max<int64_t>(1, 2 * ctx->num_cus / strips);
+  if (a.groups >= blocks) {
+    a.per_group = 1;
+    a.piece_rows = a.group_rows;
+  } else {
+    a.piece_rows = std::max<int64_t>(16, (a.group_rows * a.groups + blocks - 1) / blocks);
+    a.per_group = (a.group_rows + a.piece_rows - 1) / a.piece_rows;
+    blocks = a.groups * a.per_group;
+  }
+  // slots of the partial sums
+  NormFinish fin{};
+  fin.cols = a.cols;
+  fin.blocks = blocks;
+  fin.per_group = a.per_group;
+  const bool direct = blocks == 1;
+  const bool gate_slot = gate_sum && !(a.gate_grouped && a.per_group == 1);
+  int slots = 0;
+  int slot[kSums];
+  for (int i = 0; i < kSums; ++i) slot[i] = to[i] && (i != kSumGate || gate_slot) ? slots++ : -1;
+  std::unique_ptr<Scratch> ws, stats;
+  const size_t step = (size_t)slots * a.cols;
+  if (!direct && slots) ws = workspace(ctx, sizeof(float) * step * blocks, op);
+  a.sum_step = direct ? 0 : (int64_t)step;
+  fin.step = (int64_t)step;
+  for (int i = 0; i < kSums; ++i) {
+    a.sum[i] = nullptr;
+    if (slot[i] < 0) continue;
+    float* out = to[i];
+    float* p = ws ? ws->as<float>() + (size_t)slot[i] * a.cols : nullptr;
+    a.sum[i] = direct ? out : p;
+    if (i == kSumGate && a.gate_grouped) {
+      fin.gate_from = p;
+      fin.dgate = out;
+      fin.lddgate = a.lddgate;
+      fin.groups = a.groups;
+    } else {
+      fin.from[fin.count] = p;
+      fin.to[fin.count++] = out;
+    }
+  }
+  if (a.du || (block && a.post.kind != ORCA_HIP_NORM_NONE)) {
+    stats = workspace(ctx, sizeof(float) * 8 * a.rows, op);
+    a.stats = stats->as<float>();
+    hipLaunchKernelGGL(norm_stats_kernel, dim3((unsigned)std::min<int64_t>(a.rows, kMaxBlocks)), dim3(kStream), 0,
+                       ctx->stream, a, block);
+    ORCA_HIP_CHECK(hipGetLastError());
+  }
+  hipLaunchKernelGGL(norm_strip_kernel, dim3((unsigned)strips, (unsigned)blocks), dim3(kStream), 0, ctx->stream, a,
+                     block);
+  ORCA_HIP_CHECK(hipGetLastError());
+  if (!direct) launch_finish(ctx, fin);
+}
+
+}  // namespace
+}  // namespace orca_hip
+
+using namespace orca_hip;
+
+extern "C" {
+
+int orca_hip_norm(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* x, size_t ldx,
+                  const orca_hip_norm_params* norm, float* y, size_t ldy, void* y8) {
+  return guard([&] {
+    const char* op = "norm";
+    check_sizes(op, {rows, cols});
+    if (!norm) fail(ORCA_HIP_ERR_INTERNAL, "norm: null parameters");
+    check_norm(op, *norm, false);
+    check_ld("norm (x)", ldx, cols);
+    check_ld("norm (y)", ldy, cols);
+    if (rows && cols && (!x || !y)) fail(ORCA_HIP_ERR_INTERNAL, "norm: null operand");
+    const Span xs = matrix_span(x, rows, cols, ldx), ys = matrix_span(y, rows, cols, ldy),
+               ws = vector_span(norm->weight, cols), bs = vector_span(norm->bias, cols),
+               y8s = buffer_span(y8, act8_layout(rows, cols).bytes);
+    for (const Span& in : {ws, bs}) check_apart(op, ys, in);
+    for (const Span& in : {xs, ws, bs}) check_apart(op, y8s, in);
+    if (x != y || ldx != ldy) check_apart(op, ys, xs);  // y over x, row by row, is in order
+    check_apart(op, y8s, ys);
+    act8_aligned(y8, op);
+    bind(ctx);
+    if (!rows || !cols) return;
+    check_operands(ctx, op, {{xs, "x"}, {ws, "weight"}, {bs, "bias"}, {ys, "y"}, {y8s, "y8"}});
+    NormForward a{};
+    a.rows = (int64_t)rows;
+    a.cols = (int64_t)cols;
+    a.x = x;
+    a.ldx = (int64_t)ldx;
+    a.u = y;
+    a.ldu = (int64_t)ldy;
+    a.u8 = act8_at(y8, rows, cols);
+    a.next = norm_of(*norm);
+    ProfScope prof(ctx, op, 7.0 * rows * cols, 8.0 * rows * cols + (double)(y8 ? y8s.bytes() : 0));
+    launch_forward(ctx, a, false);
+  });
+}
+
+int orca_hip_norm_backward(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* dy, size_t lddy, const float* x,
+                           size_t ldx, const orca_hip_norm_params* norm, const float* dx_add, size_t ldadd, float* dx,
+                           size_t lddx, float* dweight, float* dbias) {
+  return guard([&] {
+    const char* op = "norm_backward";
+    check_sizes(op, {rows, cols});
+    if (!norm) fail(ORCA_HIP_ERR_INTERNAL, "norm_backward: null parameters");
+    check_norm(op, *norm, false);
+    check_ld("norm_backward (dy)", lddy, cols);
+    check_ld("norm_backward (x)", ldx, cols);
+    if (dx) check_ld("norm_backward (dx)", lddx, cols);
+    if (dx && dx_add) check_ld("norm_backward (dx_add)", ldadd, cols);
+    if (rows && cols && (!dy || !x)) fail(ORCA_HIP_ERR_INTERNAL, "norm_backward: null operand");
+    const Span dys = matrix_span(dy, rows, cols, lddy), xs = matrix_span(x, rows, cols, ldx),
+               ws = vector_span(norm->weight, cols), add = matrix_span(dx ? dx_add : nullptr, rows, cols, ldadd),
+               dxs = matrix_span(dx, rows, cols, lddx), dws = vector_span(dweight, cols), dbs = vector_span(dbias, cols);
+    const Span outs[3] = {dxs, dws, dbs};
+    for (int i = 0; i < 3; ++i) {
+      for (const Span& in : {dys, xs, ws}) check_apart(op, outs[i], in);
+      // dx over dx_add, row by row, is in order (a gradient added up in place)
+      if (!(i == 0 && dx_add == dx && ldadd == lddx)) check_apart(op, outs[i], add);
+      for (int j = 0; j < i; ++j) check_apart(op, outs[i], outs[j]);
+    }
+    bind(ctx);
+    check_operands(ctx, op, {{dys, "dy"}, {xs, "x"}, {ws, "weight"}, {add, "dx_add"}, {dxs, "dx"}, {dws, "dweight"},
+                             {dbs, "dbias"}});
+    if (!cols || (!dx && !dweight && !dbias)) return;
+    NormBackward a{};
+    a.rows = (int64_t)rows;
+    a.cols = (int64_t)cols;
+    a.dy = static_cast<const float*>(add.p);
+    a.lddy = (int64_t)ldadd;
+    a.du = dy;
+    a.lddu = (int64_t)lddy;
+    a.y = x;
+    a.ldy = (int64_t)ldx;
+    a.next = norm_of(*norm);
+    a.rs = 1.0f;
+    a.dx = dx;
+    a.lddx = (int64_t)lddx;
+    float* const to[kSums] = {nullptr, nullptr, nullptr, dweight, dbias};
+    ProfScope prof(ctx, op, 16.0 * rows * cols, 4.0 * (2 + (dx != nullptr) + (add.p != nullptr)) * rows * cols);
+    launch_backward(ctx, a, to, 0, op);
+  });
+}
+
+int orca_hip_residual_norm(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* x, size_t ldx, const float* f,
+                           size_t ldf, const orca_hip_residual_block* block, float* y, size_t ldy, float* u,
+                           size_t ldu, void* u8) {
+  return guard([&] {
+    const char* op = "residual_norm";
+    check_sizes(op, {rows, cols});
+    if (!block) fail(ORCA_HIP_ERR_INTERNAL, "residual_norm: null parameters");
+    const orca_hip_residual_block& p = *block;
+    check_block(op, rows, cols, p);
+    const bool next = p.next.kind != ORCA_HIP_NORM_NONE;
+    check_ld("residual_norm (x)", ldx, cols);
+    check_ld("residual_norm (f)", ldf, cols);
+    check_ld("residual_norm (y)", ldy, cols);
+    if (next) check_ld("residual_norm (u)", ldu, cols);
+    if (!next && (u || u8)) fail(ORCA_HIP_ERR_INTERNAL, "residual_norm: u without a next norm");
+    if (rows && cols && (!x || !f || !y || (next && !u))) fail(ORCA_HIP_ERR_INTERNAL, "residual_norm: null operand");
+    const Norm post = norm_of(p.post), nx = norm_of(p.next);
+    const Span xs = matrix_span(x, rows, cols, ldx), fs = matrix_span(f, rows, cols, ldf),
+               ys = matrix_span(y, rows, cols, ldy), us = matrix_span(u, rows, cols, ldu),
+               u8s = buffer_span(u8, act8_layout(rows, cols).bytes),
+               gate = matrix_span(p.gate, p.gate ? p.groups : 0, cols, p.ldgate), pw = vector_span(post.w, cols),
+               pb = vector_span(post.b, cols), nw = vector_span(nx.w, cols), nb = vector_span(nx.b, cols);
+    const Span outs[3] = {ys, us, u8s};
+    for (int i = 0; i < 3; ++i) {
+      for (const Span& in : {fs, gate, pw, pb, nw, nb}) check_apart(op, outs[i], in);
+      // y over x, element by element, is in order
+      if (!(i == 0 && x == y && ldx == ldy)) check_apart(op, outs[i], xs);
+      for (int j = 0; j < i; ++j) check_apart(op, outs[i], outs[j]);
+    }
+    act8_aligned(u8, op);
+    bind(ctx);
+    if (!rows || !cols) return;
+    check_operands(ctx, op, {{xs, "x"}, {fs, "f"}, {gate, "gate"}, {pw, "post weight"}, {pb, "post bias"},
+                             {nw, "next weight"}, {nb, "next bias"}, {ys, "y"}, {us, "u"}, {u8s, "u8"}});
+    NormForward a{};
+    a.rows = (int64_t)rows;
+    a.cols = (int64_t)cols;
+    a.x = x;
+    a.ldx = (int64_t)ldx;
+    a.f = f;
+    a.ldf = (int64_t)ldf;
+    a.y = y;
+    a.ldy = (int64_t)ldy;
+    a.u = u;
+    a.ldu = (int64_t)ldu;
+    a.u8 = act8_at(u8, rows, cols);
+    a.post = post;
+    a.next = nx;
+    a.gate = p.gate;
+    a.ldgate = (int64_t)p.ldgate;
+    a.gate_rows = p.gate ? (int64_t)(rows / p.groups) : 1;
+    a.rs = p.residual_scale;
+    a.bs = p.block_scale;
+    a.drop = dropout_of(p.p, p.seed, p.offset);
+    ProfScope prof(ctx, op, 12.0 * rows * cols, 4.0 * (3 + next) * rows * cols + (double)(u8 ? u8s.bytes() : 0));
+    launch_forward(ctx, a, true);
+  });
+}
+
+int orca_hip_residual_norm_backward(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* dy, size_t lddy,
+                                    const float* du, size_t lddu, const float* f, size_t ldf, const float* y,
+                                    size_t ldy, const orca_hip_residual_block* block,
+                                    const orca_hip_residual_grads* grads) {
+  return guard([&] {
+    const char* op = "residual_norm_backward";
+    check_sizes(op, {rows, cols});
+    if (!block || !grads) fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: null parameters");
+    const orca_hip_residual_block& p = *block;
+    const orca_hip_residual_grads& o = *grads;
+    check_block(op, rows, cols, p);
+    const bool post = p.post.kind != ORCA_HIP_NORM_NONE;
+    if (du && p.next.kind == ORCA_HIP_NORM_NONE)
+      fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: du without a next norm");
+    if (!du && (o.dnext_weight || o.dnext_bias))
+      fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: the next norm's gradients need du");
+    if (!post && (o.dpost_weight || o.dpost_bias))
+      fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: gradients of a post norm that is not there");
+    if (o.dgate && !p.gate) fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: a gradient without its gate");
+    const bool through = o.df || o.dgate || o.dpost_weight || o.dpost_bias;  // something of the block is wanted
+    const bool reads_f = (through && post) || o.dgate;
+    if (rows && cols && !dy && !du) fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: one of dy and du is needed");
+    if (rows && cols && ((du && !y) || (reads_f && !f)))
+      fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: null operand");
+    if (dy) check_ld("residual_norm_backward (dy)", lddy, cols);
+    if (du) check_ld("residual_norm_backward (du)", lddu, cols);
+    if (du) check_ld("residual_norm_backward (y)", ldy, cols);
+    if (reads_f) check_ld("residual_norm_backward (f)", ldf, cols);
+    if (o.dx) check_ld("residual_norm_backward (dx)", o.lddx, cols);
+    if (o.df) check_ld("residual_norm_backward (df)", o.lddf, cols);
+    if (o.dgate) check_ld("residual_norm_backward (dgate)", o.lddgate, cols);
+    const Norm pn = norm_of(p.post), nx = norm_of(p.next);
+    const Span dys = matrix_span(dy, rows, cols, lddy), dus = matrix_span(du, rows, cols, lddu),
+               fs = matrix_span(reads_f ? f : nullptr, rows, cols, ldf),
+               ys = matrix_span(du ? y : nullptr, rows, cols, ldy),
+               gate = matrix_span(p.gate, p.gate ? p.groups : 0, cols, p.ldgate), pw = vector_span(pn.w, cols),
+               pb = vector_span(pn.b, cols), nw = vector_span(nx.w, cols),
+               dxs = matrix_span(o.dx, rows, cols, o.lddx), dfs = matrix_span(o.df, rows, cols, o.lddf),
+               dgs = matrix_span(o.dgate, o.dgate ? p.groups : 0, cols, o.lddgate),
+               dpw = vector_span(o.dpost_weight, cols), dpb = vector_span(o.dpost_bias, cols),
+               dnw = vector_span(o.dnext_weight, cols), dnb = vector_span(o.dnext_bias, cols);
+    const Span outs[7] = {dxs, dfs, dgs, dpw, dpb, dnw, dnb};
+    for (int i = 0; i < 7; ++i) {
+      for (const Span& in : {dus, fs, ys, gate, pw, pb, nw}) check_apart(op, outs[i], in);
+      // dx over dy, element by element, is in order
+      if (!(i == 0 && o.dx == dy && o.lddx == lddy)) check_apart(op, outs[i], dys);
+      for (int j = 0; j < i; ++j) check_apart(op, outs[i], outs[j]);
+    }
+    bind(ctx);
+    check_operands(ctx, op, {{dys, "dy"}, {dus, "du"}, {fs, "f"}, {ys, "y"}, {gate, "gate"}, {pw, "post weight"},
+                             {pb, "post bias"}, {nw, "next weight"}, {dxs, "dx"}, {dfs, "df"}, {dgs, "dgate"},
+                             {dpw, "dpost_weight"}, {dpb, "dpost_bias"}, {dnw, "dnext_weight"}, {dnb, "dnext_bias"}});
+    if (!cols || (!through && !o.dx && !o.dnext_weight && !o.dnext_bias)) return;
+    NormBackward a{};
+    a.rows = (int64_t)rows;
+    a.cols = (int64_t)cols;
+    a.dy = dy;
+    a.lddy = (int64_t)lddy;
+    a.du = du;
+    a.lddu = (int64_t)lddu;
+    a.f = static_cast<const float*>(fs.p);
+    a.ldf = (int64_t)ldf;
+    a.y = y;
+    a.ldy = (int64_t)ldy;
+    a.post = pn;
+    a.next = nx;
+    a.gate = p.gate;
+    a.ldgate = (int64_t)p.ldgate;
+    a.rs = p.residual_scale;
+    a.bs = p.block_scale;
+    a.drop = dropout_of(p.p, p.seed, p.offset);
+    a.dx = o.dx;
+    a.lddx = (int64_t)o.lddx;
+    a.df = o.df;
+    a.lddf = (int64_t)o.lddf;
+    a.dgate = o.dgate;
+    a.lddgate = (int64_t)o.lddgate;
+    float* const to[kSums] = {o.dgate, o.dpost_weight, o.dpost_bias, o.dnext_weight, o.dnext_bias};
+    ProfScope prof(ctx, op, 32.0 * rows * cols,
+                   4.0 * ((dy != nullptr) + 2 * (du != nullptr) + reads_f + (o.dx != nullptr) + (o.df != nullptr)) *
+                       rows * cols);
+    launch_backward(ctx, a, to, p.gate ? (int64_t)p.groups : 0, op);
+  });
+}
+
+}  // extern "C"
