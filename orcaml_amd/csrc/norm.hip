@@ -375,6 +375,331 @@ __global__ void __launch_bounds__(kStream) norm_strip_kernel(NormBackward a, boo
     if (a.sum[i]) store4(a.sum[i] + blockIdx.y * a.sum_step, c, a.cols, sum[i]);
 }
 
+// ---------------------------------------------------------------- rows in registers
+// A row of up to T x Q x 4 values held by T = 64 NW threads, Q quads of neighbouring columns each, quads T apart.
+// One wave (NW = 1): blocks of four waves with a row each, and no barrier.
+template <int NW>
+constexpr int kRowThreads = NW == 1 ? 256 : 64 * NW;
+
+template <int NW, int Q>
+struct RowCols {
+  static constexpr int T = 64 * NW;
+  int cols, c0;
+  bool full, ragged;  // every thread has all its columns; quads are cut off at the end
+  uint32_t at[Q];     // where a quad's load starts, in bytes (32 bits and a uniform row: no 64-bit address a lane)
+  __device__ __forceinline__ explicit RowCols(int64_t n)
+      : cols((int)n), c0((int)(threadIdx.x % T) * 4), full((int)n == T * Q * 4), ragged((n & 3) != 0) {
+    // Loads are moved back into the row at its end, so that none waits behind a branch; settle() then shifts the
+    // values into place, with zeros for what does not exist.
+#pragma unroll
+    for (int i = 0; i < Q; ++i) at[i] = 4u * (uint32_t)min(c(i), cols - 4);
+  }
+  __device__ __forceinline__ int c(int i) const { return c0 + i * T * 4; }
+  // How many of a quad's columns exist (or a number beyond 0 .. 4).  Opaque: the compiler would else keep the
+  // comparisons of a whole row, two scalar registers each, and spill them.
+  __device__ __forceinline__ int have(int i) const {
+    int h = cols - c(i);
+    asm volatile("" : "+v"(h));
+    return h;
+  }
+  __device__ __forceinline__ floatx4 load(const float* row, int i) const {
+    return *reinterpret_cast<const floatx4_u*>(reinterpret_cast<const char*>(row) + at[i]);
+  }
+  __device__ __forceinline__ void settle(floatx4& v, int i) const {
+    if (full) return;
+    const int h = have(i);
+    if (ragged) v = shift_down(v, h > 0 && h < 4 ? 4 - h : 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < h ? v[j] : 0.0f;
+  }
+  __device__ __forceinline__ void load_row(const float* row, floatx4 (&v)[Q]) const {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) v[i] = load(row, i);
+  }
+  __device__ __forceinline__ void settle_row(floatx4 (&v)[Q]) const {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) settle(v[i], i);
+  }
+  // A weight's values in the row's columns (`none` where there is no weight).
+  __device__ __forceinline__ void load_weight(const float* w, float none, floatx4 (&v)[Q]) const {
+    if (!w) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) v[i] = splat(none);
+      return;
+    }
+    load_row(w, v);
+    settle_row(v);
+  }
+  __device__ __forceinline__ void store(float* row, int i, floatx4 v) const {
+    float* p = reinterpret_cast<float*>(reinterpret_cast<char*>(row) + 4u * (uint32_t)c(i));
+    const int h = have(i);
+    if (h >= 4) {
+      *reinterpret_cast<floatx4_u*>(p) = v;
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < h) p[j] = v[j];
+  }
+  // Bit 4 i + j: the dropout keeps column c(i) + j.
+  __device__ __forceinline__ uint32_t kept(const Dropout& d, int64_t row) const {
+    static_assert(Q <= 8, "a word has 32 bits");
+    if (!d.on) return 0xffffffffu;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      const Words w = dropout_words(d, row, c(i) >> 2);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bits |= (uint32_t)dropout_keeps(d, w, j) << (4 * i + j);
+    }
+    return bits;
+  }
+};
+
+template <int NW, int Q>
+__device__ __forceinline__ Stats row_stats(const Norm& n, const floatx4 (&v)[Q], const RowCols<NW, Q>& rc,
+                                           Team<NW>& team) {
+  Stats s{0.0f, 0.0f, 0.0f};
+  const float count = (float)rc.cols;
+  if (n.kind == ORCA_HIP_NORM_LAYER) {
+    float t[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < Q; ++i) t[0] += (v[i].x + v[i].y) + (v[i].z + v[i].w);
+    team.sum(t);
+    s.mean = t[0] / count;
+  }
+  float t[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < Q; ++i) {
+    const int h = rc.have(i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float d = j < h ? v[i][j] - s.mean : 0.0f;
+      t[0] += d;
+      t[1] = fmaf(d, d, t[1]);
+    }
+  }
+  team.sum(t);
+  float var = t[1] / count;
+  if (n.kind == ORCA_HIP_NORM_LAYER) {
+    s.rest = t[0] / count;
+    var = fmaxf(fmaf(-s.rest, s.rest, var), 0.0f);
+  }
+  s.r = 1.0f / sqrtf(var + n.eps);
+  return s;
+}
+
+template <int NW, int Q, bool JOINT>
+__global__ void __launch_bounds__(kRowThreads<NW>) norm_rows_kernel(NormForward a) {
+  __shared__ float lds[2 * NW * 4];
+  Team<NW> team{lds};
+  const RowCols<NW, Q> rc(a.cols);
+  const int64_t first = NW == 1 ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+  for (int64_t row = first; row < a.rows; row += (int64_t)gridDim.x * (NW == 1 ? 4 : 1)) {
+    floatx4 v[Q], w[Q], b[Q];
+    rc.load_row(a.x + row * a.ldx, v);
+    if (JOINT) {
+      floatx4 f[Q];
+      rc.load_row(a.f + row * a.ldf, f);
+      const uint32_t kept = rc.kept(a.drop, row);
+      rc.settle_row(f);
+      if (a.post.kind != ORCA_HIP_NORM_NONE) {
+        rc.load_weight(a.post.w, 1.0f, w);
+        rc.load_weight(a.post.b, 0.0f, b);
+        const Stats s = row_stats<NW, Q>(a.post, f, rc, team);
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f[i][j] = fmaf(s.unit(f[i][j]), w[i][j], b[i][j]);
+      }
+      rc.load_weight(a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr, 1.0f, w);
+      const float k = a.bs * a.drop.scale;
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        rc.settle(v[i], i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float t = f[i][j] * (w[i][j] * k);
+          v[i][j] = fmaf(a.rs, v[i][j], kept >> (4 * i + j) & 1 ? t : 0.0f);
+        }
+        rc.store(a.y + row * a.ldy, i, v[i]);
+        if (!rc.full) {  // zeros again behind the row, where a bias may have stood
+          const int h = rc.have(i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[i][j] = j < h ? v[i][j] : 0.0f;
+        }
+      }
+    } else {
+      rc.settle_row(v);
+    }
+    if (a.next.kind == ORCA_HIP_NORM_NONE) continue;
+    rc.load_weight(a.next.w, 1.0f, w);
+    rc.load_weight(a.next.b, 0.0f, b);
+    const Stats s = row_stats<NW, Q>(a.next, v, rc, team);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = fmaf(s.unit(v[i][j]), w[i][j], b[i][j]);
+      rc.store(a.u + row * a.ldu, i, v[i]);
+      if (a.u8.codes) {
+        const Quad q = quad_of(rc.c(i), a.cols);
+        const uint32_t byte = quad_byte(v[i], q);
+        if (q.have > 0) {
+          store_codes(a.u8.codes + row * a.u8.cols, q, v[i], byte);
+          if ((threadIdx.x & 7) == 0) a.u8.scales[q.group * a.u8.ld + row] = (uint8_t)byte;
+        }
+      }
+    }
+  }
+}
+
+// The whole backward of the rows of a block's pieces: NEXT: a gradient through u; BLOCK: the gradients of the
+// block; POST: its output is normed.
+template <int NW, int Q, bool NEXT, bool BLOCK, bool POST>
+__global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBackward a) {
+  constexpr int T = 64 * NW, TEAMS = kRowThreads<NW> / T;
+  __shared__ float lds[2 * NW * 4];
+  __shared__ floatx4 sums_lds[TEAMS > 1 ? TEAMS * T * Q : 1];
+  Team<NW> team{lds};
+  const RowCols<NW, Q> rc(a.cols);
+  const int tm = NW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, t = threadIdx.x % T;
+  const float count = (float)a.cols, k = a.bs * a.drop.scale;
+  floatx4 sum[kSums][Q];
+#pragma unroll
+  for (int n = 0; n < kSums; ++n)
+#pragma unroll
+    for (int i = 0; i < Q; ++i) sum[n][i] = splat(0.0f);
+  // the block's teams' sums, added up, to `out`
+  const auto flush = [&](floatx4 (&v)[Q], float* out) {
+    if constexpr (TEAMS > 1) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) sums_lds[(tm * Q + i) * T + t] = v[i];
+      __syncthreads();
+      if (tm == 0) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+          floatx4 s = v[i];
+#pragma unroll
+          for (int m = 1; m < TEAMS; ++m) s += sums_lds[(m * Q + i) * T + t];
+          rc.store(out, i, s);
+        }
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) rc.store(out, i, v[i]);
+    }
+  };
+  for (int64_t unit = blockIdx.x; unit < a.groups * a.per_group; unit += gridDim.x) {
+    const int64_t group = unit / a.per_group, r0 = group * a.group_rows + unit % a.per_group * a.piece_rows;
+    const int64_t r1 = min(r0 + a.piece_rows, (group + 1) * a.group_rows);
+    for (int64_t row = r0 + tm; row < r1; row += TEAMS) {
+      floatx4 g[Q], v[Q], d[Q], w[Q];
+      if (a.dy)
+        rc.load_row(a.dy + row * a.lddy, g);
+      else
+#pragma unroll
+        for (int i = 0; i < Q; ++i) g[i] = splat(0.0f);
+      if (NEXT) {
+        rc.load_row(a.y + row * a.ldy, v);
+        rc.load_row(a.du + row * a.lddu, d);
+      }
+      floatx4 f[Q];
+      if (BLOCK && a.f) rc.load_row(a.f + row * a.ldf, f);
+      if (a.dy) rc.settle_row(g);
+      if (NEXT) {
+        rc.settle_row(v);
+        rc.settle_row(d);
+        rc.load_weight(a.next.w, 1.0f, w);
+        Stats s = row_stats<NW, Q>(a.next, v, rc, team);
+        float e[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[i][j] = s.unit(v[i][j]);
+            sum[kSumNextW][i][j] = fmaf(d[i][j], v[i][j], sum[kSumNextW][i][j]);
+            sum[kSumNextB][i][j] += d[i][j];
+            d[i][j] *= w[i][j];
+            e[0] += d[i][j];
+            e[1] = fmaf(d[i][j], v[i][j], e[1]);
+          }
+        }
+        team.sum(e);
+        const float c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? e[0] / count : 0.0f, c2 = e[1] / count;
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) g[i][j] = fmaf(s.r, fmaf(-v[i][j], c2, d[i][j]) - c1, g[i][j]);
+      }
+      if (a.dx) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+          rc.store(a.dx + row * a.lddx, i, floatx4{g[i].x * a.rs, g[i].y * a.rs, g[i].z * a.rs, g[i].w * a.rs});
+      }
+      if (!BLOCK) continue;
+      const uint32_t kept = rc.kept(a.drop, row);
+      rc.load_weight(a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr, 1.0f, w);
+      if (a.f)
+        rc.settle_row(f);
+      else
+#pragma unroll
+        for (int i = 0; i < Q; ++i) f[i] = splat(0.0f);
+      Stats s{0.0f, 0.0f, 0.0f};
+      float e[2] = {0.0f, 0.0f};
+      if (POST) {
+        s = row_stats<NW, Q>(a.post, f, rc, team);
+        rc.load_weight(a.post.w, 1.0f, v);
+        rc.load_weight(a.post.b, 0.0f, d);
+      }
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        floatx4 each;
+        const int h = rc.have(i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool on = (kept >> (4 * i + j) & 1) && j < h;
+          if (POST) f[i][j] = s.unit(f[i][j]);
+          const float out = POST ? fmaf(f[i][j], v[i][j], d[i][j]) : f[i][j];
+          float dv = on ? g[i][j] * k : 0.0f;
+          each[j] = on ? dv * out : 0.0f;
+          sum[kSumGate][i][j] += each[j];
+          dv *= w[i][j];
+          if (POST) {
+            sum[kSumPostW][i][j] = fmaf(dv, f[i][j], sum[kSumPostW][i][j]);
+            sum[kSumPostB][i][j] += dv;
+            dv *= v[i][j];
+            e[0] += dv;
+            e[1] = fmaf(dv, f[i][j], e[1]);
+          }
+          g[i][j] = dv;
+        }
+        if (a.gate_each) rc.store(a.dgate + row * a.lddgate, i, each);
+      }
+      if (POST) {
+        team.sum(e);
+        const float c1 = a.post.kind == ORCA_HIP_NORM_LAYER ? e[0] / count : 0.0f, c2 = e[1] / count;
+#pragma unroll
+        for (int i = 0; i < Q; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) g[i][j] = s.r * (fmaf(-f[i][j], c2, g[i][j]) - c1);
+      }
+      if (a.df) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) rc.store(a.df + row * a.lddf, i, g[i]);
+      }
+    }
+    if (BLOCK && a.gate_grouped && a.per_group == 1 && a.dgate) {
+      flush(sum[kSumGate], a.dgate + group * a.lddgate);
+#pragma unroll
+      for (int i = 0; i < Q; ++i) sum[kSumGate][i] = splat(0.0f);
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kSums; ++n)
+    if (a.sum[n]) flush(sum[n], a.sum[n] + blockIdx.x * a.sum_step);
+}
+
 // ---------------------------------------------------------------- the blocks' partial sums
 struct NormFinish {
   int64_t cols, blocks, step;  // of the partial sums; `step` floats from one block's to the next one's
@@ -449,13 +774,54 @@ void check_operands(orca_hip_ctx* ctx, const char* op, std::initializer_list<Ope
 
 constexpr unsigned kMaxBlocks = 1u << 20;  // of 256 threads and more; the kernels step over the rest
 
+// Rows of up to 8192 values stay in registers; longer ones, and rows shorter than a quad, are gone over in passes.
+constexpr int64_t kMaxRegisterRow = 8192;
+// Calls f with the waves of a row and the quads of a thread, as template arguments.
+template <class F>
+void with_row_shape(int64_t cols, F f) {
+  using std::integral_constant;
+  if (cols <= 256) return f(integral_constant<int, 1>(), integral_constant<int, 1>());
+  if (cols <= 512) return f(integral_constant<int, 1>(), integral_constant<int, 2>());
+  if (cols <= 1024) return f(integral_constant<int, 1>(), integral_constant<int, 4>());
+  if (cols <= 2048) return f(integral_constant<int, 4>(), integral_constant<int, 2>());
+  if (cols <= 4096) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
+  return f(integral_constant<int, 8>(), integral_constant<int, 4>());
+}
+bool in_registers(int64_t cols) { return cols >= 4 && cols <= kMaxRegisterRow; }
+
 void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
-  const dim3 grid((unsigned)std::min<int64_t>(a.rows, kMaxBlocks));
-  if (joint)
-    hipLaunchKernelGGL(norm_stream_kernel<true>, grid, dim3(kStream), 0, ctx->stream, a);
-  else
-    hipLaunchKernelGGL(norm_stream_kernel<false>, grid, dim3(kStream), 0, ctx->stream, a);
+  if (in_registers(a.cols)) {
+    with_row_shape(a.cols, [&](auto nw, auto q) {
+      const int64_t rows = decltype(nw)::value == 1 ? 4 : 1;
+      const dim3 grid((unsigned)std::min<int64_t>((a.rows + rows - 1) / rows, kMaxBlocks));
+      const dim3 threads(kRowThreads<decltype(nw)::value>);
+      if (joint)
+        hipLaunchKernelGGL((norm_rows_kernel<decltype(nw)::value, decltype(q)::value, true>), grid, threads, 0,
+                           ctx->stream, a);
+      else
+        hipLaunchKernelGGL((norm_rows_kernel<decltype(nw)::value, decltype(q)::value, false>), grid, threads, 0,
+                           ctx->stream, a);
+    });
+  } else {
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, kMaxBlocks));
+    if (joint)
+      hipLaunchKernelGGL(norm_stream_kernel<true>, grid, dim3(kStream), 0, ctx->stream, a);
+    else
+      hipLaunchKernelGGL(norm_stream_kernel<false>, grid, dim3(kStream), 0, ctx->stream, a);
+  }
   ORCA_HIP_CHECK(hipGetLastError());
+}
+
+template <int NW, int Q>
+void launch_backward_rows(orca_hip_ctx* ctx, const NormBackward& a, bool block, unsigned blocks) {
+  const bool post = a.post.kind != ORCA_HIP_NORM_NONE;
+  const auto kernel = !block      ? a.du ? norm_backward_kernel<NW, Q, true, false, false>
+                                         : norm_backward_kernel<NW, Q, false, false, false>
+                      : a.du      ? post ? norm_backward_kernel<NW, Q, true, true, true>
+                                         : norm_backward_kernel<NW, Q, true, true, false>
+                      : post      ? norm_backward_kernel<NW, Q, false, true, true>
+                                  : norm_backward_kernel<NW, Q, false, true, false>;
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kRowThreads<NW>), 0, ctx->stream, a);
 }
 
 void launch_finish(orca_hip_ctx* ctx, const NormFinish& f) {
@@ -488,13 +854,14 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
   a.groups = a.gate_grouped ? a.rows / a.gate_rows : 1;
   a.group_rows = a.gate_grouped ? a.gate_rows : a.rows;
   const bool block = a.df || to[kSumGate] || to[kSumPostW] || to[kSumPostB];
-  const int64_t strips = (a.cols + kStream * 4 - 1) / (kStream * 4);
+  const bool registers = in_registers(a.cols);
+  const int64_t strips = registers ? 1 : (a.cols + kStream * 4 - 1) / (kStream * 4);
   int64_t blocks = std::max<int64_t>(1, 2 * ctx->num_cus / strips);
   if (a.groups >= blocks) {
     a.per_group = 1;
     a.piece_rows = a.group_rows;
   } else {
-    a.piece_rows = std::max<int64_t>(16, (a.group_rows * a.groups + blocks - 1) / blocks);
+    a.piece_rows = std::max<int64_t>(registers ? (a.cols <= 1024 ? 4 : 1) : 16, (a.group_rows * a.groups + blocks - 1) / blocks);
     a.per_group = (a.group_rows + a.piece_rows - 1) / a.piece_rows;
     blocks = a.groups * a.per_group;
   }
@@ -528,6 +895,14 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
       fin.from[fin.count] = p;
       fin.to[fin.count++] = out;
     }
+  }
+  if (registers) {
+    with_row_shape(a.cols, [&](auto nw, auto q) {
+      launch_backward_rows<decltype(nw)::value, decltype(q)::value>(ctx, a, block, (unsigned)blocks);
+    });
+    ORCA_HIP_CHECK(hipGetLastError());
+    if (!direct) launch_finish(ctx, fin);
+    return;
   }
   if (a.du || (block && a.post.kind != ORCA_HIP_NORM_NONE)) {
     stats = workspace(ctx, sizeof(float) * 8 * a.rows, op);
