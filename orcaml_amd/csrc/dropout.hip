@@ -10,32 +10,37 @@
 namespace orca_hip {
 namespace {
 
-constexpr int kDropRows = 4;  // rows of a thread, so that it has as many loads in flight
-
-// A thread takes four neighbouring columns of kDropRows rows; `across` threads of a block lie along a row, the
-// others below each other.  y may be x: a thread reads what it writes first.
+// A thread takes four neighbouring columns; `across` = 2^across_bits threads of a block lie along a row, the others
+// below each other.  y may be x: a thread reads what it writes first.
+//
+// Bound by HBM.  One quad a thread, blocks of up to 4 KiB of a row and non-temporal stores took 45 us at 8192 x 4096
+// (5.9 TB/s) where four rows a thread with ordinary stores took 67; at 1024 x 4096 6.3 and 8.4.  FAR: non-temporal
+// loads too: 43 us (6.3 TB/s) at 8192 x 4096, whose operands pass the 256 MiB of the memory-side cache, but 22.5 for
+// 20.7 at half of that, which it may hold from the operator before.
+template <bool FAR>
 __global__ void __launch_bounds__(256) dropout_kernel(const float* x, int64_t ldx, int64_t rows, int64_t cols, float* y,
                                                       int64_t ldy, int across_bits, Dropout d) {
-  const int64_t down = 256 >> across_bits;
   const int64_t quad = ((((int64_t)blockIdx.z * gridDim.y + blockIdx.y) << across_bits) +
                         (threadIdx.x & ((1 << across_bits) - 1)));
-  const int64_t r0 = (int64_t)blockIdx.x * down * kDropRows + (threadIdx.x >> across_bits);
+  const int64_t row = (int64_t)blockIdx.x * (256 >> across_bits) + (threadIdx.x >> across_bits);
   const Quad q = quad_of(quad * 4, cols);
-  floatx4 v[kDropRows];
+  const float* from = x + min(row, rows - 1) * ldx;
+  floatx4 v = FAR && q.n == 4 ? (floatx4)__builtin_nontemporal_load(reinterpret_cast<const floatx4_u*>(from + q.at))
+                              : load_quad(from, q);
+  settle(q, v);
+  if (d.on) {
+    const Words w = dropout_words(d, row, quad);
 #pragma unroll
-  for (int i = 0; i < kDropRows; ++i) v[i] = load_quad(x + min(r0 + i * down, rows - 1) * ldx, q);
-#pragma unroll
-  for (int i = 0; i < kDropRows; ++i) {
-    const int64_t row = r0 + i * down;
-    settle(q, v[i]);
-    if (d.on) {
-      const Words w = dropout_words(d, row, quad);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = dropout_keeps(d, w, j) ? v[i][j] * d.scale : 0.0f;
-    }
-    if (row < rows) store_quad(y + row * ldy, q, v[i]);
+    for (int j = 0; j < 4; ++j) v[j] = dropout_keeps(d, w, j) ? v[j] * d.scale : 0.0f;
   }
+  if (row >= rows) return;
+  if (q.have == 4)
+    __builtin_nontemporal_store((floatx4_u)v, reinterpret_cast<floatx4_u*>(y + row * ldy + q.c));
+  else
+    store_quad(y + row * ldy, q, v);
 }
+
+constexpr double kCacheBytes = 256.0 * (1 << 20);  // of the memory-side cache
 
 }  // namespace
 }  // namespace orca_hip
@@ -61,13 +66,14 @@ int orca_hip_dropout(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* x
     check_extent(ctx, y, ys.bytes(), "dropout (y)");
     const size_t quads = (cols + 3) / 4;
     int bits = 0;
-    while (bits < 6 && (size_t(1) << bits) < quads) ++bits;
+    while (bits < 8 && (size_t(1) << bits) < quads) ++bits;
     const size_t across = (quads + (size_t(1) << bits) - 1) >> bits, gy = std::min<size_t>(across, 32768),
-                 down = (size_t(256) >> bits) * kDropRows;
+                 down = size_t(256) >> bits;
     const dim3 grid((unsigned)((rows + down - 1) / down), (unsigned)gy, (unsigned)((across + gy - 1) / gy));
     ProfScope prof(ctx, op, (double)rows * cols, 8.0 * rows * cols);
-    hipLaunchKernelGGL(dropout_kernel, grid, dim3(256), 0, ctx->stream, x, (int64_t)ldx, (int64_t)rows, (int64_t)cols,
-                       y, (int64_t)ldy, bits, dropout_of(p, seed, offset));
+    hipLaunchKernelGGL(8.0 * rows * cols >= kCacheBytes ? dropout_kernel<true> : dropout_kernel<false>, grid, dim3(256), 0,
+                       ctx->stream, x, (int64_t)ldx, (int64_t)rows, (int64_t)cols, y, (int64_t)ldy, bits,
+                       dropout_of(p, seed, offset));
     ORCA_HIP_CHECK(hipGetLastError());
   });
 }

@@ -51,6 +51,7 @@ struct NormForward {
   int64_t ldgate, gate_rows;  // rows of f for each of the gate's
   float rs, bs;
   Dropout drop;
+  bool far;  // RowCols::load_row
 };
 
 // Sums over the rows that a backward gives.
@@ -80,6 +81,7 @@ struct NormBackward {
   // A block adds up whole pieces of rows: per_group pieces of piece_rows rows for each of `groups` groups of
   // group_rows (one group but where each row of the gate has its own sum).
   int64_t group_rows, groups, per_group, piece_rows;
+  bool far;           // RowCols::load_row
   bool gate_each;     // the gate's gradient row by row, without a sum
   bool gate_grouped;  // its sums are those of the groups
   float* sum[kSums];  // where a sum goes: the result itself (one block), or a block's first partial sum
@@ -412,9 +414,17 @@ struct RowCols {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = j < h ? v[j] : 0.0f;
   }
-  __device__ __forceinline__ void load_row(const float* row, floatx4 (&v)[Q]) const {
+  // far: the operands pass the memory-side cache, so that nothing of them is in it (kCacheBytes).
+  __device__ __forceinline__ void load_row(const float* row, floatx4 (&v)[Q], bool far) const {
+    if (far) {
 #pragma unroll
-    for (int i = 0; i < Q; ++i) v[i] = load(row, i);
+      for (int i = 0; i < Q; ++i)
+        v[i] = __builtin_nontemporal_load(
+            reinterpret_cast<const floatx4_u*>(reinterpret_cast<const char*>(row) + at[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) v[i] = load(row, i);
+    }
   }
   __device__ __forceinline__ void settle_row(floatx4 (&v)[Q]) const {
 #pragma unroll
@@ -427,14 +437,14 @@ struct RowCols {
       for (int i = 0; i < Q; ++i) v[i] = splat(none);
       return;
     }
-    load_row(w, v);
+    load_row(w, v, false);
     settle_row(v);
   }
   __device__ __forceinline__ void store(float* row, int i, floatx4 v) const {
     float* p = reinterpret_cast<float*>(reinterpret_cast<char*>(row) + 4u * (uint32_t)c(i));
     const int h = have(i);
     if (h >= 4) {
-      *reinterpret_cast<floatx4_u*>(p) = v;
+      __builtin_nontemporal_store((floatx4_u)v, reinterpret_cast<floatx4_u*>(p));
       return;
     }
 #pragma unroll
@@ -497,10 +507,10 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_rows_kernel(NormForward 
   const int64_t first = NW == 1 ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
   for (int64_t row = first; row < a.rows; row += (int64_t)gridDim.x * (NW == 1 ? 4 : 1)) {
     floatx4 v[Q], w[Q], b[Q];
-    rc.load_row(a.x + row * a.ldx, v);
+    rc.load_row(a.x + row * a.ldx, v, a.far);
     if (JOINT) {
       floatx4 f[Q];
-      rc.load_row(a.f + row * a.ldf, f);
+      rc.load_row(a.f + row * a.ldf, f, a.far);
       const uint32_t kept = rc.kept(a.drop, row);
       rc.settle_row(f);
       if (a.post.kind != ORCA_HIP_NORM_NONE) {
@@ -554,8 +564,8 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_rows_kernel(NormForward 
 }
 
 // The whole backward of the rows of a block's pieces: NEXT: a gradient through u; BLOCK: the gradients of the
-// block; POST: its output is normed.
-template <int NW, int Q, bool NEXT, bool BLOCK, bool POST>
+// block; POST: its output is normed; BIAS: a norm has a bias, or its gradient is wanted.
+template <int NW, int Q, bool NEXT, bool BLOCK, bool POST, bool BIAS>
 __global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBackward a) {
   constexpr int T = 64 * NW, TEAMS = kRowThreads<NW> / T;
   __shared__ float lds[2 * NW * 4];
@@ -596,16 +606,16 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBack
     for (int64_t row = r0 + tm; row < r1; row += TEAMS) {
       floatx4 g[Q], v[Q], d[Q], w[Q];
       if (a.dy)
-        rc.load_row(a.dy + row * a.lddy, g);
+        rc.load_row(a.dy + row * a.lddy, g, a.far);
       else
 #pragma unroll
         for (int i = 0; i < Q; ++i) g[i] = splat(0.0f);
       if (NEXT) {
-        rc.load_row(a.y + row * a.ldy, v);
-        rc.load_row(a.du + row * a.lddu, d);
+        rc.load_row(a.y + row * a.ldy, v, a.far);
+        rc.load_row(a.du + row * a.lddu, d, a.far);
       }
       floatx4 f[Q];
-      if (BLOCK && a.f) rc.load_row(a.f + row * a.ldf, f);
+      if (BLOCK && a.f) rc.load_row(a.f + row * a.ldf, f, a.far);
       if (a.dy) rc.settle_row(g);
       if (NEXT) {
         rc.settle_row(v);
@@ -619,7 +629,7 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBack
           for (int j = 0; j < 4; ++j) {
             v[i][j] = s.unit(v[i][j]);
             sum[kSumNextW][i][j] = fmaf(d[i][j], v[i][j], sum[kSumNextW][i][j]);
-            sum[kSumNextB][i][j] += d[i][j];
+            if (BIAS) sum[kSumNextB][i][j] += d[i][j];
             d[i][j] *= w[i][j];
             e[0] += d[i][j];
             e[1] = fmaf(d[i][j], v[i][j], e[1]);
@@ -650,7 +660,7 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBack
       if (POST) {
         s = row_stats<NW, Q>(a.post, f, rc, team);
         rc.load_weight(a.post.w, 1.0f, v);
-        rc.load_weight(a.post.b, 0.0f, d);
+        if (BIAS) rc.load_weight(a.post.b, 0.0f, d);
       }
 #pragma unroll
       for (int i = 0; i < Q; ++i) {
@@ -660,14 +670,14 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBack
         for (int j = 0; j < 4; ++j) {
           const bool on = (kept >> (4 * i + j) & 1) && j < h;
           if (POST) f[i][j] = s.unit(f[i][j]);
-          const float out = POST ? fmaf(f[i][j], v[i][j], d[i][j]) : f[i][j];
+          const float out = POST ? BIAS ? fmaf(f[i][j], v[i][j], d[i][j]) : f[i][j] * v[i][j] : f[i][j];
           float dv = on ? g[i][j] * k : 0.0f;
           each[j] = on ? dv * out : 0.0f;
           sum[kSumGate][i][j] += each[j];
           dv *= w[i][j];
           if (POST) {
             sum[kSumPostW][i][j] = fmaf(dv, f[i][j], sum[kSumPostW][i][j]);
-            sum[kSumPostB][i][j] += dv;
+            if (BIAS) sum[kSumPostB][i][j] += dv;
             dv *= v[i][j];
             e[0] += dv;
             e[1] = fmaf(dv, f[i][j], e[1]);
@@ -710,24 +720,40 @@ struct NormFinish {
   float* dgate;
   int64_t lddgate, groups, per_group;
 };
-// A block adds up 64 columns: 16 threads of four columns, 16 of each for every 16th partial sum.
-__global__ void __launch_bounds__(256) norm_finish_kernel(NormFinish a) {
-  __shared__ floatx4 lds[16][16];
-  const int q = threadIdx.x & 15, k = threadIdx.x >> 4;
-  const int64_t c = ((int64_t)blockIdx.x * 16 + q) * 4;
+// A block adds up 32 columns: a thread four columns of every 64th partial sum, eight of them in flight, then the
+// eight threads of a wave and the eight waves that have the same columns.
+__global__ void __launch_bounds__(512) norm_finish_kernel(NormFinish a) {
+  __shared__ floatx4 lds[8][8];
+  const int q = threadIdx.x & 7, k = threadIdx.x >> 3, wave = threadIdx.x >> 6;
+  const int64_t c = ((int64_t)blockIdx.x * 8 + q) * 4, at = max((int64_t)0, min(c, a.cols - 4));
   for (int64_t i = blockIdx.y; i < a.count + a.groups; i += gridDim.y) {
     const int64_t group = i - a.count;
     const float* from = group < 0 ? a.from[i] : a.gate_from + group * a.per_group * a.step;
     float* to = group < 0 ? a.to[i] : a.dgate + group * a.lddgate;
     const int64_t blocks = group < 0 ? a.blocks : a.per_group;
     floatx4 t = splat(0.0f);
-    if (c < a.cols)
-      for (int64_t b = k; b < blocks; b += 16) t += load4(from + b * a.step, c, a.cols);
-    lds[k][q] = t;
-    __syncthreads();
-    if (k == 0 && c < a.cols) {
+    for (int64_t b0 = k; b0 < blocks; b0 += 64 * 8) {
+      floatx4 v[8];
 #pragma unroll
-      for (int j = 1; j < 16; ++j) t += lds[j][q];
+      for (int u = 0; u < 8; ++u) {
+        const float* p = from + min(b0 + 64 * u, blocks - 1) * a.step;
+        v[u] = a.cols < 4 ? load4(p, c, a.cols) : *reinterpret_cast<const floatx4_u*>(p + at);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (b0 + 64 * u >= blocks) v[u] = splat(0.0f);
+      t += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+    if (a.cols >= 4) t = shift_down(t, (int)min((int64_t)3, c - at));  // what lies behind the row is not stored
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int d = 8; d < 64; d *= 2) t[j] += __shfl_xor(t[j], d);
+    if ((threadIdx.x & 63) < 8) lds[wave][q] = t;
+    __syncthreads();
+    if (threadIdx.x < 8 && c < a.cols) {
+#pragma unroll
+      for (int w = 1; w < 8; ++w) t += lds[w][q];
       store4(to, c, a.cols, t);
     }
     __syncthreads();
@@ -772,6 +798,7 @@ void check_operands(orca_hip_ctx* ctx, const char* op, std::initializer_list<Ope
     check_extent(ctx, o.span.p, o.span.bytes(), (std::string(op) + " (" + o.what + ")").c_str());
 }
 
+constexpr double kCacheBytes = 256.0 * (1 << 20);  // of the memory-side cache
 constexpr unsigned kMaxBlocks = 1u << 20;  // of 256 threads and more; the kernels step over the rest
 
 // Rows of up to 8192 values stay in registers; longer ones, and rows shorter than a quad, are gone over in passes.
@@ -784,12 +811,13 @@ void with_row_shape(int64_t cols, F f) {
   if (cols <= 512) return f(integral_constant<int, 1>(), integral_constant<int, 2>());
   if (cols <= 1024) return f(integral_constant<int, 1>(), integral_constant<int, 4>());
   if (cols <= 2048) return f(integral_constant<int, 4>(), integral_constant<int, 2>());
-  if (cols <= 4096) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
-  return f(integral_constant<int, 8>(), integral_constant<int, 4>());
+  if (cols <= 4096) return f(integral_constant<int, 8>(), integral_constant<int, 2>());
+  return f(integral_constant<int, 16>(), integral_constant<int, 2>());
 }
 bool in_registers(int64_t cols) { return cols >= 4 && cols <= kMaxRegisterRow; }
 
-void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
+void launch_forward(orca_hip_ctx* ctx, NormForward& a, bool joint) {
+  a.far = (joint ? 16.0 : 8.0) * a.rows * a.cols >= kCacheBytes;
   if (in_registers(a.cols)) {
     with_row_shape(a.cols, [&](auto nw, auto q) {
       const int64_t rows = decltype(nw)::value == 1 ? 4 : 1;
@@ -812,23 +840,26 @@ void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
   ORCA_HIP_CHECK(hipGetLastError());
 }
 
+template <int NW, int Q, bool BIAS>
+auto backward_kernel(bool next, bool block, bool post) {
+  if (!next) return post ? norm_backward_kernel<NW, Q, false, true, true, BIAS>
+                         : norm_backward_kernel<NW, Q, false, true, false, false>;
+  if (!block) return norm_backward_kernel<NW, Q, true, false, false, BIAS>;
+  return post ? norm_backward_kernel<NW, Q, true, true, true, BIAS> : norm_backward_kernel<NW, Q, true, true, false, BIAS>;
+}
 template <int NW, int Q>
 void launch_backward_rows(orca_hip_ctx* ctx, const NormBackward& a, bool block, unsigned blocks) {
-  const bool post = a.post.kind != ORCA_HIP_NORM_NONE;
-  const auto kernel = !block      ? a.du ? norm_backward_kernel<NW, Q, true, false, false>
-                                         : norm_backward_kernel<NW, Q, false, false, false>
-                      : a.du      ? post ? norm_backward_kernel<NW, Q, true, true, true>
-                                         : norm_backward_kernel<NW, Q, true, true, false>
-                      : post      ? norm_backward_kernel<NW, Q, false, true, true>
-                                  : norm_backward_kernel<NW, Q, false, true, false>;
+  const bool post = a.post.kind != ORCA_HIP_NORM_NONE, bias = a.post.b || a.sum[kSumPostB] || a.sum[kSumNextB];
+  const auto kernel = bias ? backward_kernel<NW, Q, true>(a.du, block, post)
+                           : backward_kernel<NW, Q, false>(a.du, block, post);
   hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kRowThreads<NW>), 0, ctx->stream, a);
 }
 
 void launch_finish(orca_hip_ctx* ctx, const NormFinish& f) {
   const int64_t outs = f.count + f.groups;
   if (!outs) return;
-  hipLaunchKernelGGL(norm_finish_kernel, dim3((unsigned)((f.cols + 63) / 64), (unsigned)std::min<int64_t>(outs, 32768)),
-                     dim3(256), 0, ctx->stream, f);
+  hipLaunchKernelGGL(norm_finish_kernel, dim3((unsigned)((f.cols + 31) / 32), (unsigned)std::min<int64_t>(outs, 32768)),
+                     dim3(512), 0, ctx->stream, f);
   ORCA_HIP_CHECK(hipGetLastError());
 }
 
@@ -846,6 +877,8 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
     }
     return launch_finish(ctx, fin);
   }
+  a.far = 4.0 * ((a.dy != nullptr) + 2 * (a.du != nullptr) + (a.f != nullptr) + (a.dx != nullptr) + (a.df != nullptr)) *
+              a.rows * a.cols >= kCacheBytes;
   a.gate_rows = gate_rows ? a.rows / gate_rows : a.rows;
   a.gate_each = to[kSumGate] && a.gate_rows == 1;
   const bool gate_sum = to[kSumGate] && !a.gate_each;
