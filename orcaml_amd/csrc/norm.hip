@@ -51,7 +51,6 @@ struct NormForward {
   int64_t ldgate, gate_rows;  // rows of f for each of the gate's
   float rs, bs;
   Dropout drop;
-  bool far;  // RowCols::load_row
 };
 
 // Sums over the rows that a backward gives.
@@ -78,15 +77,15 @@ struct NormBackward {
   int64_t lddf;
   float* dgate;
   int64_t lddgate;
-  // A block adds up whole pieces of rows: per_group pieces of piece_rows rows for each of `groups` groups of
-  // group_rows (one group but where each row of the gate has its own sum).
-  int64_t group_rows, groups, per_group, piece_rows;
-  bool far;           // RowCols::load_row
+  // The rows are in groups (one, but where each row of the gate has its own sum), and those in per_group pieces of
+  // every per_group-th row each, so that the blocks work on neighbouring rows at a time: 8192 x 4096 backward in 107 us,
+  // in 115 with successive rows to a block.  Unit i is piece i % per_group of group i / per_group.
+  int group_rows, groups, per_group;
   bool gate_each;     // the gate's gradient row by row, without a sum
   bool gate_grouped;  // its sums are those of the groups
   float* sum[kSums];  // where a sum goes: the result itself (one block), or a block's first partial sum
   int64_t sum_step;   // from one block's to the next one's
-  float* stats;       // [rows][8] (norm_stats_kernel)
+  float* stats;       // [rows][kRowStats] (norm_stats_kernel)
 };
 
 // ---------------------------------------------------------------- rows
@@ -117,11 +116,17 @@ struct Team {
   }
 };
 
-// unit = ((v - mean) - rest) r
+// unit = ((v - mean) - rest) r, off = -rest r
 struct Stats {
-  float mean, rest, r;
-  __device__ __forceinline__ float unit(float v) const { return ((v - mean) - rest) * r; }
+  float mean, off, r;
+  __device__ __forceinline__ float unit(float v) const { return fmaf(v - mean, r, off); }
 };
+// From the first mean and the sums of the differences to it and of their squares.
+__device__ __forceinline__ Stats stats_of(const Norm& n, float mean, float sum, float squares, float count) {
+  const float rest = n.kind == ORCA_HIP_NORM_LAYER ? sum / count : 0.0f;
+  const float var = fmaxf(fmaf(-rest, rest, squares / count), 0.0f), r = 1.0f / sqrtf(var + n.eps);
+  return Stats{mean, -rest * r, r};
+}
 
 __device__ __forceinline__ floatx4 splat(float v) { return floatx4{v, v, v, v}; }
 __device__ __forceinline__ floatx4 load4(const float* row, int64_t c, int64_t cols) {
@@ -149,7 +154,7 @@ __device__ __forceinline__ floatx4 weight4(const float* w, int64_t c, int64_t co
 constexpr int kStream = 256;  // threads of a block, 4 columns each at a time
 
 __device__ __forceinline__ Stats stream_stats(const Norm& n, const float* row, int64_t cols, Team<4>& team) {
-  Stats s{0.0f, 0.0f, 0.0f};
+  float mean = 0.0f;
   const float count = (float)cols;
   if (n.kind == ORCA_HIP_NORM_LAYER) {
     float t[1] = {0.0f};
@@ -158,26 +163,20 @@ __device__ __forceinline__ Stats stream_stats(const Norm& n, const float* row, i
       t[0] += (v.x + v.y) + (v.z + v.w);
     }
     team.sum(t);
-    s.mean = t[0] / count;
+    mean = t[0] / count;
   }
   float t[2] = {0.0f, 0.0f};
   for (int64_t c = threadIdx.x * 4; c < cols; c += kStream * 4) {
     const floatx4 v = load4(row, c, cols);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float d = c + j < cols ? v[j] - s.mean : 0.0f;
+      const float d = c + j < cols ? v[j] - mean : 0.0f;
       t[0] += d;
       t[1] = fmaf(d, d, t[1]);
     }
   }
   team.sum(t);
-  float var = t[1] / count;
-  if (n.kind == ORCA_HIP_NORM_LAYER) {
-    s.rest = t[0] / count;
-    var = fmaxf(fmaf(-s.rest, s.rest, var), 0.0f);
-  }
-  s.r = 1.0f / sqrtf(var + n.eps);
-  return s;
+  return stats_of(n, mean, t[0], t[1], count);
 }
 
 template <bool JOINT>
@@ -235,8 +234,8 @@ __global__ void __launch_bounds__(kStream) norm_stream_kernel(NormForward a) {
   }
 }
 
-// What a backward needs to know of each row: (mean, r, mean(e), mean(e unit)) of the next norm, then of the post
-// norm.
+// What a backward needs to know of each row: Stats, mean(e) and mean(e unit) of the next norm, then of the post norm.
+constexpr int kRowStats = 10;
 __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, bool block) {
   __shared__ float lds[2 * 4 * 4];
   Team<4> team{lds};
@@ -247,8 +246,6 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
     float c1 = 0.0f, c2 = 0.0f;
     if (a.du) {
       sy = stream_stats(a.next, y, a.cols, team);
-      sy.mean += sy.rest;
-      sy.rest = 0.0f;
       float t[2] = {0.0f, 0.0f};
       for (int64_t c = threadIdx.x * 4; c < a.cols; c += kStream * 4) {
         const floatx4 v = load4(y, c, a.cols), d = load4(du, c, a.cols), w = weight4(a.next.w, c, a.cols, 1.0f);
@@ -269,8 +266,6 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
     if (block && a.post.kind != ORCA_HIP_NORM_NONE) {
       const float *f = a.f + row * a.ldf, *gate = a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr;
       sf = stream_stats(a.post, f, a.cols, team);
-      sf.mean += sf.rest;
-      sf.rest = 0.0f;
       float t[2] = {0.0f, 0.0f};
       for (int64_t c = threadIdx.x * 4; c < a.cols; c += kStream * 4) {
         floatx4 g = splat(0.0f);
@@ -298,9 +293,10 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
       p2 = t[1] / count;
     }
     if (threadIdx.x == 0) {
-      floatx4* s = reinterpret_cast<floatx4*>(a.stats + row * 8);
-      s[0] = floatx4{sy.mean, sy.r, c1, c2};
-      s[1] = floatx4{sf.mean, sf.r, p1, p2};
+      float* s = a.stats + row * kRowStats;
+      const float v[kRowStats] = {sy.mean, sy.off, sy.r, c1, c2, sf.mean, sf.off, sf.r, p1, p2};
+#pragma unroll
+      for (int i = 0; i < kRowStats; ++i) s[i] = v[i];
     }
   }
 }
@@ -314,24 +310,23 @@ __global__ void __launch_bounds__(kStream) norm_strip_kernel(NormBackward a, boo
   const floatx4 bp = weight4(a.post.b, c, a.cols, 0.0f);
   const bool post = a.post.kind != ORCA_HIP_NORM_NONE;
   floatx4 sum[kSums] = {zero, zero, zero, zero, zero};
-  for (int64_t unit = blockIdx.y; unit < a.groups * a.per_group; unit += gridDim.y) {
-    const int64_t group = unit / a.per_group, r0 = group * a.group_rows + unit % a.per_group * a.piece_rows;
-    const int64_t r1 = min(r0 + a.piece_rows, (group + 1) * a.group_rows);
-    for (int64_t row = r0; row < r1; ++row) {
-      floatx4 s[2] = {zero, zero};
+  for (int unit = blockIdx.y; unit < a.groups * a.per_group; unit += gridDim.y) {
+    const int group = unit / a.per_group, r0 = group * a.group_rows;
+    for (int64_t row = r0 + unit % a.per_group; row < r0 + a.group_rows; row += a.per_group) {
+      float s[kRowStats] = {};
       if (a.stats) {
-        s[0] = reinterpret_cast<const floatx4*>(a.stats + row * 8)[0];
-        s[1] = reinterpret_cast<const floatx4*>(a.stats + row * 8)[1];
+#pragma unroll
+        for (int i = 0; i < kRowStats; ++i) s[i] = a.stats[row * kRowStats + i];
       }
       floatx4 g = zero;
       if (a.dy) g = load4(a.dy + row * a.lddy, c, a.cols);
       if (a.du) {
         const floatx4 v = load4(a.y + row * a.ldy, c, a.cols), d = load4(a.du + row * a.lddu, c, a.cols);
-        const Stats sy{s[0].x, 0.0f, s[0].y};
+        const Stats sy{s[0], s[1], s[2]};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float unit = sy.unit(v[j]);
-          g[j] += sy.r * (fmaf(-unit, s[0].w, d[j] * wn[j]) - s[0].z);
+          g[j] += sy.r * (fmaf(-unit, s[4], d[j] * wn[j]) - s[3]);
           sum[kSumNextW][j] = fmaf(d[j], unit, sum[kSumNextW][j]);
           sum[kSumNextB][j] += d[j];
         }
@@ -341,7 +336,7 @@ __global__ void __launch_bounds__(kStream) norm_strip_kernel(NormBackward a, boo
       floatx4 v = zero, unit = zero, dv, each;
       if (a.f) v = load4(a.f + row * a.ldf, c, a.cols);
       if (post) {
-        const Stats sf{s[1].x, 0.0f, s[1].y};
+        const Stats sf{s[5], s[6], s[7]};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           unit[j] = sf.unit(v[j]);
@@ -361,14 +356,14 @@ __global__ void __launch_bounds__(kStream) norm_strip_kernel(NormBackward a, boo
         sum[kSumPostB][j] += dv[j];
         if (post) {
           sum[kSumPostW][j] = fmaf(dv[j], unit[j], sum[kSumPostW][j]);
-          dv[j] = s[1].y * (fmaf(-unit[j], s[1].w, dv[j] * wp[j]) - s[1].z);
+          dv[j] = s[7] * (fmaf(-unit[j], s[9], dv[j] * wp[j]) - s[8]);
         }
       }
       if (a.gate_each) store4(a.dgate + row * a.lddgate, c, a.cols, each);
       if (a.df) store4(a.df + row * a.lddf, c, a.cols, dv);
     }
     if (a.gate_grouped && a.per_group == 1 && a.dgate) {
-      store4(a.dgate + group * a.lddgate, c, a.cols, sum[kSumGate]);
+      store4(a.dgate + (int64_t)group * a.lddgate, c, a.cols, sum[kSumGate]);
       sum[kSumGate] = zero;
     }
   }
@@ -414,17 +409,16 @@ struct RowCols {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = j < h ? v[j] : 0.0f;
   }
-  // far: the operands pass the memory-side cache, so that nothing of them is in it (kCacheBytes).
-  __device__ __forceinline__ void load_row(const float* row, floatx4 (&v)[Q], bool far) const {
-    if (far) {
+  // Zeros for what does not exist.
+  __device__ __forceinline__ void mask(floatx4& v, int i) const {
+    if (full) return;
+    const int h = have(i);
 #pragma unroll
-      for (int i = 0; i < Q; ++i)
-        v[i] = __builtin_nontemporal_load(
-            reinterpret_cast<const floatx4_u*>(reinterpret_cast<const char*>(row) + at[i]));
-    } else {
+    for (int j = 0; j < 4; ++j) v[j] = j < h ? v[j] : 0.0f;
+  }
+  __device__ __forceinline__ void load_row(const float* row, floatx4 (&v)[Q]) const {
 #pragma unroll
-      for (int i = 0; i < Q; ++i) v[i] = load(row, i);
-    }
+    for (int i = 0; i < Q; ++i) v[i] = load(row, i);
   }
   __device__ __forceinline__ void settle_row(floatx4 (&v)[Q]) const {
 #pragma unroll
@@ -437,7 +431,7 @@ struct RowCols {
       for (int i = 0; i < Q; ++i) v[i] = splat(none);
       return;
     }
-    load_row(w, v, false);
+    load_row(w, v);
     settle_row(v);
   }
   __device__ __forceinline__ void store(float* row, int i, floatx4 v) const {
@@ -456,11 +450,13 @@ struct RowCols {
     static_assert(Q <= 8, "a word has 32 bits");
     if (!d.on) return 0xffffffffu;
     uint32_t bits = 0;
+    Dropout o = d;
+    if (NW >= 8) asm volatile("" : "+s"(o.key[0]), "+s"(o.key[1]));  // or all rounds' keys stay in registers
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
-      const Words w = dropout_words(d, row, c(i) >> 2);
+      const Words w = dropout_words(o, row, c(i) >> 2);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bits |= (uint32_t)dropout_keeps(d, w, j) << (4 * i + j);
+      for (int j = 0; j < 4; ++j) bits |= (uint32_t)dropout_keeps(o, w, j) << (4 * i + j);
     }
     return bits;
   }
@@ -469,111 +465,155 @@ struct RowCols {
 template <int NW, int Q>
 __device__ __forceinline__ Stats row_stats(const Norm& n, const floatx4 (&v)[Q], const RowCols<NW, Q>& rc,
                                            Team<NW>& team) {
-  Stats s{0.0f, 0.0f, 0.0f};
   const float count = (float)rc.cols;
+  float mean = 0.0f, t[2] = {0.0f, 0.0f};
   if (n.kind == ORCA_HIP_NORM_LAYER) {
-    float t[1] = {0.0f};
+    float m[1] = {0.0f};
 #pragma unroll
-    for (int i = 0; i < Q; ++i) t[0] += (v[i].x + v[i].y) + (v[i].z + v[i].w);
-    team.sum(t);
-    s.mean = t[0] / count;
-  }
-  float t[2] = {0.0f, 0.0f};
+    for (int i = 0; i < Q; ++i) m[0] += (v[i].x + v[i].y) + (v[i].z + v[i].w);
+    team.sum(m);
+    mean = m[0] / count;
 #pragma unroll
-  for (int i = 0; i < Q; ++i) {
-    const int h = rc.have(i);
+    for (int i = 0; i < Q; ++i) {
+      floatx4 d = v[i] - mean;
+      rc.mask(d, i);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float d = j < h ? v[i][j] - s.mean : 0.0f;
-      t[0] += d;
-      t[1] = fmaf(d, d, t[1]);
+      for (int j = 0; j < 4; ++j) {
+        t[0] += d[j];
+        t[1] = fmaf(d[j], d[j], t[1]);
+      }
     }
+    team.sum(t);
+  } else {
+    float q[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[0] = fmaf(v[i][j], v[i][j], q[0]);
+    team.sum(q);
+    t[1] = q[0];
   }
-  team.sum(t);
-  float var = t[1] / count;
-  if (n.kind == ORCA_HIP_NORM_LAYER) {
-    s.rest = t[0] / count;
-    var = fmaxf(fmaf(-s.rest, s.rest, var), 0.0f);
-  }
-  s.r = 1.0f / sqrtf(var + n.eps);
-  return s;
+  return stats_of(n, mean, t[0], t[1], count);
 }
 
+// The forward.  A team takes every step-th row and has the loads of its next row in flight while it works on one:
+// the weights stay in registers, since a load behind those would have to wait for them.
 template <int NW, int Q, bool JOINT>
 __global__ void __launch_bounds__(kRowThreads<NW>) norm_rows_kernel(NormForward a) {
+  constexpr int TEAMS = kRowThreads<NW> / (64 * NW);
   __shared__ float lds[2 * NW * 4];
   Team<NW> team{lds};
   const RowCols<NW, Q> rc(a.cols);
-  const int64_t first = NW == 1 ? (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
-  for (int64_t row = first; row < a.rows; row += (int64_t)gridDim.x * (NW == 1 ? 4 : 1)) {
-    floatx4 v[Q], w[Q], b[Q];
-    rc.load_row(a.x + row * a.ldx, v, a.far);
+  const bool gates = JOINT && a.gate && a.gate_rows != a.rows;  // a gate for each row
+  int64_t row = (int64_t)blockIdx.x * TEAMS + (TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  const int64_t step = (int64_t)gridDim.x * TEAMS;
+  if (row >= a.rows) return;
+  floatx4 wp[Q], bp[Q], wn[Q], bn[Q], gate[Q];
+  floatx4 x1[Q], f1[Q];
+  rc.load_weight(a.next.w, 1.0f, wn);
+  rc.load_weight(a.next.b, 0.0f, bn);
+  if (JOINT) {
+    rc.load_weight(a.post.w, 1.0f, wp);
+    rc.load_weight(a.post.b, 0.0f, bp);
+    rc.load_weight(gates ? nullptr : a.gate, 1.0f, gate);
+  }
+  rc.load_row(a.x + row * a.ldx, x1);
+  if (JOINT) rc.load_row(a.f + row * a.ldf, f1);
+  while (true) {
+    floatx4 v[Q], f[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      v[i] = x1[i];
+      if (JOINT) f[i] = f1[i];
+    }
+    if (gates) rc.load_row(a.gate + (uint32_t)row / (uint32_t)a.gate_rows * a.ldgate, gate);
+    const int64_t after = row + step;
+    if (after < a.rows) {
+      rc.load_row(a.x + after * a.ldx, x1);
+      if (JOINT) rc.load_row(a.f + after * a.ldf, f1);
+    }
+    rc.settle_row(v);
     if (JOINT) {
-      floatx4 f[Q];
-      rc.load_row(a.f + row * a.ldf, f, a.far);
       const uint32_t kept = rc.kept(a.drop, row);
       rc.settle_row(f);
       if (a.post.kind != ORCA_HIP_NORM_NONE) {
-        rc.load_weight(a.post.w, 1.0f, w);
-        rc.load_weight(a.post.b, 0.0f, b);
         const Stats s = row_stats<NW, Q>(a.post, f, rc, team);
 #pragma unroll
         for (int i = 0; i < Q; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) f[i][j] = fmaf(s.unit(f[i][j]), w[i][j], b[i][j]);
+          for (int j = 0; j < 4; ++j) f[i][j] = fmaf(s.unit(f[i][j]), wp[i][j], bp[i][j]);
       }
-      rc.load_weight(a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr, 1.0f, w);
       const float k = a.bs * a.drop.scale;
 #pragma unroll
       for (int i = 0; i < Q; ++i) {
-        rc.settle(v[i], i);
+        floatx4 g = gate[i];
+        if (gates) rc.settle(g, i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float t = f[i][j] * (w[i][j] * k);
+          const float t = f[i][j] * (g[j] * k);
           v[i][j] = fmaf(a.rs, v[i][j], kept >> (4 * i + j) & 1 ? t : 0.0f);
         }
         rc.store(a.y + row * a.ldy, i, v[i]);
-        if (!rc.full) {  // zeros again behind the row, where a bias may have stood
-          const int h = rc.have(i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[i][j] = j < h ? v[i][j] : 0.0f;
-        }
+        rc.mask(v[i], i);  // a bias may have stood behind the row
       }
-    } else {
-      rc.settle_row(v);
     }
-    if (a.next.kind == ORCA_HIP_NORM_NONE) continue;
-    rc.load_weight(a.next.w, 1.0f, w);
-    rc.load_weight(a.next.b, 0.0f, b);
-    const Stats s = row_stats<NW, Q>(a.next, v, rc, team);
+    if (a.next.kind != ORCA_HIP_NORM_NONE) {
+      const Stats s = row_stats<NW, Q>(a.next, v, rc, team);
 #pragma unroll
-    for (int i = 0; i < Q; ++i) {
+      for (int i = 0; i < Q; ++i) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = fmaf(s.unit(v[i][j]), w[i][j], b[i][j]);
-      rc.store(a.u + row * a.ldu, i, v[i]);
-      if (a.u8.codes) {
-        const Quad q = quad_of(rc.c(i), a.cols);
-        const uint32_t byte = quad_byte(v[i], q);
-        if (q.have > 0) {
-          store_codes(a.u8.codes + row * a.u8.cols, q, v[i], byte);
-          if ((threadIdx.x & 7) == 0) a.u8.scales[q.group * a.u8.ld + row] = (uint8_t)byte;
+        for (int j = 0; j < 4; ++j) v[i][j] = fmaf(s.unit(v[i][j]), wn[i][j], bn[i][j]);
+        rc.store(a.u + row * a.ldu, i, v[i]);
+        if (a.u8.codes) {
+          const Quad q = quad_of(rc.c(i), a.cols);
+          const uint32_t byte = quad_byte(v[i], q);
+          if (q.have > 0) {
+            store_codes(a.u8.codes + row * a.u8.cols, q, v[i], byte);
+            if ((threadIdx.x & 7) == 0) a.u8.scales[q.group * a.u8.ld + row] = (uint8_t)byte;
+          }
         }
       }
     }
+    if (after >= a.rows) return;
+    row = after;
   }
 }
 
 // The whole backward of the rows of a block's pieces: NEXT: a gradient through u; BLOCK: the gradients of the
 // block; POST: its output is normed; BIAS: a norm has a bias, or its gradient is wanted.
+//
+// Two stages a row, each with the other one's loads in flight: the next norm (y, du), then the block (dy, f).  The
+// weights are in LDS: loads of theirs would wait for those of the rows, and registers go into the sums.
+//
+// Two blocks a CU are worth more than loads ahead: with both norms and biases, eight waves of a row keep to 128
+// registers without (8192 x 4096: 196 us; 210 with loads ahead and one block), and four waves, which do for the others,
+// to 256 (159 us without biases; 185 where more left one block).
 template <int NW, int Q, bool NEXT, bool BLOCK, bool POST, bool BIAS>
-__global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBackward a) {
+__global__ void __launch_bounds__(kRowThreads<NW>, NW == 8 && Q == 2 ? 4 : NW == 4 && Q == 4 ? 2 : 1)
+norm_backward_kernel(NormBackward a) {
+  constexpr bool PIPE = !(NEXT && BLOCK && POST && NW == 8);
   constexpr int T = 64 * NW, TEAMS = kRowThreads<NW> / T;
+  constexpr int WN = 0, WP = NEXT, BP = WP + POST, GATE = BP + (POST && BIAS), VECTORS = GATE + BLOCK;
   __shared__ float lds[2 * NW * 4];
+  __shared__ floatx4 weights[VECTORS * Q * T];
   __shared__ floatx4 sums_lds[TEAMS > 1 ? TEAMS * T * Q : 1];
   Team<NW> team{lds};
   const RowCols<NW, Q> rc(a.cols);
-  const int tm = NW == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, t = threadIdx.x % T;
+  const int tm = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, t = threadIdx.x % T;
   const float count = (float)a.cols, k = a.bs * a.drop.scale;
+  const bool gates = BLOCK && a.gate && a.gate_rows != a.rows;  // a gate for each row
+  // A thread reads only what it wrote (all teams write the same).
+  const auto put = [&](int n, const float* w, float none) {
+    floatx4 v[Q];
+    rc.load_weight(w, none, v);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) weights[(n * Q + i) * T + t] = v[i];
+  };
+  const auto weight = [&](int n, int i) { return weights[(n * Q + i) * T + t]; };
+  if (NEXT) put(WN, a.next.w, 1.0f);
+  if (POST) put(WP, a.post.w, 1.0f);
+  if (POST && BIAS) put(BP, a.post.b, 0.0f);
+  if (BLOCK) put(GATE, gates ? nullptr : a.gate, 1.0f);
   floatx4 sum[kSums][Q];
 #pragma unroll
   for (int n = 0; n < kSums; ++n)
@@ -600,85 +640,94 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBack
       for (int i = 0; i < Q; ++i) rc.store(out, i, v[i]);
     }
   };
-  for (int64_t unit = blockIdx.x; unit < a.groups * a.per_group; unit += gridDim.x) {
-    const int64_t group = unit / a.per_group, r0 = group * a.group_rows + unit % a.per_group * a.piece_rows;
-    const int64_t r1 = min(r0 + a.piece_rows, (group + 1) * a.group_rows);
-    for (int64_t row = r0 + tm; row < r1; row += TEAMS) {
-      floatx4 g[Q], v[Q], d[Q], w[Q];
-      if (a.dy)
-        rc.load_row(a.dy + row * a.lddy, g, a.far);
-      else
-#pragma unroll
-        for (int i = 0; i < Q; ++i) g[i] = splat(0.0f);
-      if (NEXT) {
-        rc.load_row(a.y + row * a.ldy, v, a.far);
-        rc.load_row(a.du + row * a.lddu, d, a.far);
-      }
-      floatx4 f[Q];
-      if (BLOCK && a.f) rc.load_row(a.f + row * a.ldf, f, a.far);
-      if (a.dy) rc.settle_row(g);
+  for (int unit = blockIdx.x; unit < a.groups * a.per_group; unit += gridDim.x) {
+    const int group = unit / a.per_group, r1 = (group + 1) * a.group_rows, step = a.per_group * TEAMS;
+    floatx4 v[Q], d[Q], g[Q], f[Q];
+    // The loads of a row's stages.
+    const auto load_next = [&](int64_t row) {
+      rc.load_row(a.y + row * a.ldy, v);
+      rc.load_row(a.du + row * a.lddu, d);
+    };
+    const auto load_block = [&](int64_t row) {
+      if (a.dy) rc.load_row(a.dy + row * a.lddy, g);
+      if (BLOCK && a.f) rc.load_row(a.f + row * a.ldf, f);
+    };
+    int64_t row = group * a.group_rows + unit % a.per_group * TEAMS + tm;
+    if (PIPE && NEXT && row < r1) load_next(row);
+    for (; row < r1; row += step) {
+      if (!PIPE && NEXT) load_next(row);
+      load_block(row);
+      const uint32_t kept = BLOCK ? rc.kept(a.drop, row) : 0;
+      Stats s{0.0f, 0.0f, 0.0f};
+      float c1 = 0.0f, c2 = 0.0f;
       if (NEXT) {
         rc.settle_row(v);
         rc.settle_row(d);
-        rc.load_weight(a.next.w, 1.0f, w);
-        Stats s = row_stats<NW, Q>(a.next, v, rc, team);
+        s = row_stats<NW, Q>(a.next, v, rc, team);
         float e[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
+          const floatx4 wn = weight(WN, i);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             v[i][j] = s.unit(v[i][j]);
             sum[kSumNextW][i][j] = fmaf(d[i][j], v[i][j], sum[kSumNextW][i][j]);
             if (BIAS) sum[kSumNextB][i][j] += d[i][j];
-            d[i][j] *= w[i][j];
+            d[i][j] *= wn[j];
             e[0] += d[i][j];
             e[1] = fmaf(d[i][j], v[i][j], e[1]);
           }
         }
         team.sum(e);
-        const float c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? e[0] / count : 0.0f, c2 = e[1] / count;
+        c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? e[0] / count : 0.0f;
+        c2 = e[1] / count;
+      }
 #pragma unroll
-        for (int i = 0; i < Q; ++i)
+      for (int i = 0; i < Q; ++i) {
+        if (a.dy)
+          rc.settle(g[i], i);
+        else
+          g[i] = splat(0.0f);
+        if (NEXT) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) g[i][j] = fmaf(s.r, fmaf(-v[i][j], c2, d[i][j]) - c1, g[i][j]);
+        }
+        if (a.dx) rc.store(a.dx + row * a.lddx, i, g[i] * a.rs);
       }
-      if (a.dx) {
-#pragma unroll
-        for (int i = 0; i < Q; ++i)
-          rc.store(a.dx + row * a.lddx, i, floatx4{g[i].x * a.rs, g[i].y * a.rs, g[i].z * a.rs, g[i].w * a.rs});
-      }
+      if (PIPE && NEXT && row + step < r1) load_next(row + step);
       if (!BLOCK) continue;
-      const uint32_t kept = rc.kept(a.drop, row);
-      rc.load_weight(a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr, 1.0f, w);
       if (a.f)
         rc.settle_row(f);
       else
 #pragma unroll
         for (int i = 0; i < Q; ++i) f[i] = splat(0.0f);
-      Stats s{0.0f, 0.0f, 0.0f};
+      if (POST) s = row_stats<NW, Q>(a.post, f, rc, team);
       float e[2] = {0.0f, 0.0f};
-      if (POST) {
-        s = row_stats<NW, Q>(a.post, f, rc, team);
-        rc.load_weight(a.post.w, 1.0f, v);
-        if (BIAS) rc.load_weight(a.post.b, 0.0f, d);
-      }
 #pragma unroll
       for (int i = 0; i < Q; ++i) {
-        floatx4 each;
-        const int h = rc.have(i);
+        floatx4 each, wp, bp, gate;
+        if (POST) wp = weight(WP, i);
+        if (POST && BIAS) bp = weight(BP, i);
+        if (gates) {
+          gate = rc.load(a.gate + (a.gate_rows == 1 ? row : group) * a.ldgate, i);
+          rc.settle(gate, i);
+        } else {
+          gate = weight(GATE, i);
+        }
+        rc.mask(g[i], i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool on = (kept >> (4 * i + j) & 1) && j < h;
+          const bool on = kept >> (4 * i + j) & 1;
           if (POST) f[i][j] = s.unit(f[i][j]);
-          const float out = POST ? BIAS ? fmaf(f[i][j], v[i][j], d[i][j]) : f[i][j] * v[i][j] : f[i][j];
+          const float out = POST ? BIAS ? fmaf(f[i][j], wp[j], bp[j]) : f[i][j] * wp[j] : f[i][j];
           float dv = on ? g[i][j] * k : 0.0f;
           each[j] = on ? dv * out : 0.0f;
           sum[kSumGate][i][j] += each[j];
-          dv *= w[i][j];
+          dv *= gate[j];
           if (POST) {
             sum[kSumPostW][i][j] = fmaf(dv, f[i][j], sum[kSumPostW][i][j]);
             if (BIAS) sum[kSumPostB][i][j] += dv;
-            dv *= v[i][j];
+            dv *= wp[j];
             e[0] += dv;
             e[1] = fmaf(dv, f[i][j], e[1]);
           }
@@ -688,7 +737,8 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBack
       }
       if (POST) {
         team.sum(e);
-        const float c1 = a.post.kind == ORCA_HIP_NORM_LAYER ? e[0] / count : 0.0f, c2 = e[1] / count;
+        c1 = a.post.kind == ORCA_HIP_NORM_LAYER ? e[0] / count : 0.0f;
+        c2 = e[1] / count;
 #pragma unroll
         for (int i = 0; i < Q; ++i)
 #pragma unroll
@@ -700,7 +750,7 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_backward_kernel(NormBack
       }
     }
     if (BLOCK && a.gate_grouped && a.per_group == 1 && a.dgate) {
-      flush(sum[kSumGate], a.dgate + group * a.lddgate);
+      flush(sum[kSumGate], a.dgate + (int64_t)group * a.lddgate);
 #pragma unroll
       for (int i = 0; i < Q; ++i) sum[kSumGate][i] = splat(0.0f);
     }
@@ -798,30 +848,32 @@ void check_operands(orca_hip_ctx* ctx, const char* op, std::initializer_list<Ope
     check_extent(ctx, o.span.p, o.span.bytes(), (std::string(op) + " (" + o.what + ")").c_str());
 }
 
-constexpr double kCacheBytes = 256.0 * (1 << 20);  // of the memory-side cache
 constexpr unsigned kMaxBlocks = 1u << 20;  // of 256 threads and more; the kernels step over the rest
 
 // Rows of up to 8192 values stay in registers; longer ones, and rows shorter than a quad, are gone over in passes.
 constexpr int64_t kMaxRegisterRow = 8192;
-// Calls f with the waves of a row and the quads of a thread, as template arguments.
+// Calls f with the waves of a row and the quads of a thread, as template arguments.  Rows of 2049 to 4096 values: four
+// waves, or eight (`many`) where four would have no registers left (kept quads and sums of both norms).
 template <class F>
-void with_row_shape(int64_t cols, F f) {
+void with_row_shape(int64_t cols, bool many, F f) {
   using std::integral_constant;
   if (cols <= 256) return f(integral_constant<int, 1>(), integral_constant<int, 1>());
   if (cols <= 512) return f(integral_constant<int, 1>(), integral_constant<int, 2>());
   if (cols <= 1024) return f(integral_constant<int, 1>(), integral_constant<int, 4>());
   if (cols <= 2048) return f(integral_constant<int, 4>(), integral_constant<int, 2>());
-  if (cols <= 4096) return f(integral_constant<int, 8>(), integral_constant<int, 2>());
-  return f(integral_constant<int, 16>(), integral_constant<int, 2>());
+  if (cols <= 4096 && many) return f(integral_constant<int, 8>(), integral_constant<int, 2>());
+  if (cols <= 4096) return f(integral_constant<int, 4>(), integral_constant<int, 4>());
+  return f(integral_constant<int, 8>(), integral_constant<int, 4>());
 }
+constexpr int kForwardBlocks = 4;  // a CU
 bool in_registers(int64_t cols) { return cols >= 4 && cols <= kMaxRegisterRow; }
 
-void launch_forward(orca_hip_ctx* ctx, NormForward& a, bool joint) {
-  a.far = (joint ? 16.0 : 8.0) * a.rows * a.cols >= kCacheBytes;
+void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
   if (in_registers(a.cols)) {
-    with_row_shape(a.cols, [&](auto nw, auto q) {
+    // joint 1024 x 4096: 14.2 us in eight waves, 15.4 in four; norm 6.9 in four, 7.6 in eight
+    with_row_shape(a.cols, joint, [&](auto nw, auto q) {
       const int64_t rows = decltype(nw)::value == 1 ? 4 : 1;
-      const dim3 grid((unsigned)std::min<int64_t>((a.rows + rows - 1) / rows, kMaxBlocks));
+      const dim3 grid((unsigned)std::min<int64_t>((a.rows + rows - 1) / rows, (int64_t)ctx->num_cus * kForwardBlocks));
       const dim3 threads(kRowThreads<decltype(nw)::value>);
       if (joint)
         hipLaunchKernelGGL((norm_rows_kernel<decltype(nw)::value, decltype(q)::value, true>), grid, threads, 0,
@@ -848,10 +900,11 @@ auto backward_kernel(bool next, bool block, bool post) {
   return post ? norm_backward_kernel<NW, Q, true, true, true, BIAS> : norm_backward_kernel<NW, Q, true, true, false, BIAS>;
 }
 template <int NW, int Q>
-void launch_backward_rows(orca_hip_ctx* ctx, const NormBackward& a, bool block, unsigned blocks) {
-  const bool post = a.post.kind != ORCA_HIP_NORM_NONE, bias = a.post.b || a.sum[kSumPostB] || a.sum[kSumNextB];
-  const auto kernel = bias ? backward_kernel<NW, Q, true>(a.du, block, post)
-                           : backward_kernel<NW, Q, false>(a.du, block, post);
+void launch_backward_rows(orca_hip_ctx* ctx, const NormBackward& a, bool block, bool bias, unsigned blocks) {
+  const bool post = a.post.kind != ORCA_HIP_NORM_NONE;
+  auto kernel = norm_backward_kernel<NW, Q, true, true, true, true>;
+  if constexpr (NW != 8 || Q != 2)  // the shape for this one alone (with_row_shape)
+    kernel = bias ? backward_kernel<NW, Q, true>(a.du, block, post) : backward_kernel<NW, Q, false>(a.du, block, post);
   hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kRowThreads<NW>), 0, ctx->stream, a);
 }
 
@@ -877,26 +930,23 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
     }
     return launch_finish(ctx, fin);
   }
-  a.far = 4.0 * ((a.dy != nullptr) + 2 * (a.du != nullptr) + (a.f != nullptr) + (a.dx != nullptr) + (a.df != nullptr)) *
-              a.rows * a.cols >= kCacheBytes;
   a.gate_rows = gate_rows ? a.rows / gate_rows : a.rows;
   a.gate_each = to[kSumGate] && a.gate_rows == 1;
   const bool gate_sum = to[kSumGate] && !a.gate_each;
   // by the gate's rows also where their gradient is not wanted: the other sums then have the same bits
   a.gate_grouped = a.gate_rows != 1 && a.gate_rows != a.rows;
-  a.groups = a.gate_grouped ? a.rows / a.gate_rows : 1;
-  a.group_rows = a.gate_grouped ? a.gate_rows : a.rows;
+  a.groups = a.gate_grouped ? (int)(a.rows / a.gate_rows) : 1;
+  a.group_rows = (int)(a.gate_grouped ? a.gate_rows : a.rows);
   const bool block = a.df || to[kSumGate] || to[kSumPostW] || to[kSumPostB];
   const bool registers = in_registers(a.cols);
   const int64_t strips = registers ? 1 : (a.cols + kStream * 4 - 1) / (kStream * 4);
   int64_t blocks = std::max<int64_t>(1, 2 * ctx->num_cus / strips);
   if (a.groups >= blocks) {
     a.per_group = 1;
-    a.piece_rows = a.group_rows;
   } else {
-    a.piece_rows = std::max<int64_t>(registers ? (a.cols <= 1024 ? 4 : 1) : 16, (a.group_rows * a.groups + blocks - 1) / blocks);
-    a.per_group = (a.group_rows + a.piece_rows - 1) / a.piece_rows;
-    blocks = a.groups * a.per_group;
+    const int64_t least = registers ? a.cols <= 1024 ? 4 : 1 : 16;  // rows of a piece
+    a.per_group = (int)std::min<int64_t>(blocks / a.groups, (a.group_rows + least - 1) / least);
+    blocks = (int64_t)a.groups * a.per_group;
   }
   // slots of the partial sums
   NormFinish fin{};
@@ -930,15 +980,17 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
     }
   }
   if (registers) {
-    with_row_shape(a.cols, [&](auto nw, auto q) {
-      launch_backward_rows<decltype(nw)::value, decltype(q)::value>(ctx, a, block, (unsigned)blocks);
+    const bool both = a.du && block && a.post.kind != ORCA_HIP_NORM_NONE;
+    const bool bias = a.post.b || a.sum[kSumPostB] || a.sum[kSumNextB];
+    with_row_shape(a.cols, both && bias, [&](auto nw, auto q) {
+      launch_backward_rows<decltype(nw)::value, decltype(q)::value>(ctx, a, block, bias, (unsigned)blocks);
     });
     ORCA_HIP_CHECK(hipGetLastError());
     if (!direct) launch_finish(ctx, fin);
     return;
   }
   if (a.du || (block && a.post.kind != ORCA_HIP_NORM_NONE)) {
-    stats = workspace(ctx, sizeof(float) * 8 * a.rows, op);
+    stats = workspace(ctx, sizeof(float) * kRowStats * a.rows, op);
     a.stats = stats->as<float>();
     hipLaunchKernelGGL(norm_stats_kernel, dim3((unsigned)std::min<int64_t>(a.rows, kMaxBlocks)), dim3(kStream), 0,
                        ctx->stream, a, block);
