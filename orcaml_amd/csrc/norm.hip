@@ -826,7 +826,7 @@ Norm norm_of(const orca_hip_norm_params& n) {
   r.b = n.bias;
   return r;
 }
-void check_block(const char* op, size_t rows, size_t cols, const orca_hip_residual_block& b) {
+void check_block(const char* op, const char* gate, size_t rows, size_t cols, const orca_hip_residual_block& b) {
   check_norm(op, b.post, true);
   check_norm(op, b.next, true);
   if (!(b.p >= 0.0 && b.p <= 1.0))
@@ -834,7 +834,7 @@ void check_block(const char* op, size_t rows, size_t cols, const orca_hip_residu
   if (!b.gate) return;
   if (!b.groups || b.groups >> kMaxSizeBits || rows % b.groups)
     fail_shape(op, "a number of gate rows that divides " + std::to_string(rows), std::to_string(b.groups));
-  check_ld((std::string(op) + " (gate)").c_str(), b.ldgate, cols);
+  check_ld(gate, b.ldgate, cols);
 }
 Span vector_span(const float* p, size_t cols) { return buffer_span(p, 4 * cols); }
 
@@ -844,8 +844,15 @@ struct Operand {
   const char* what;
 };
 void check_operands(orca_hip_ctx* ctx, const char* op, std::initializer_list<Operand> operands) {
-  for (const Operand& o : operands)
-    check_extent(ctx, o.span.p, o.span.bytes(), (std::string(op) + " (" + o.what + ")").c_str());
+  for (const Operand& o : operands) {
+    if (!o.span.p || !o.span.bytes()) continue;
+    size_t have = 0;
+    const auto where = ctx->alloc.locate(o.span.p, &have);
+    if (where == CachingAllocator::Where::kUnknown ||
+        (where == CachingAllocator::Where::kLive && o.span.bytes() <= have))
+      continue;
+    check_extent(ctx, o.span.p, o.span.bytes(), (std::string(op) + " (" + o.what + ")").c_str());  // fails
+  }
 }
 
 constexpr unsigned kMaxBlocks = 1u << 20;  // of 256 threads and more; the kernels step over the rest
@@ -892,6 +899,17 @@ void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
   ORCA_HIP_CHECK(hipGetLastError());
 }
 
+// Blocks of a backward.  Two a CU: fewer leave memory idle, more make more partial sums (8192 x 4096: 100 us with two a
+// CU, 114 with one, 109 with four).  One where a CU holds no more: rows of more than 4096 (4096 x 8192 111 for 119 us),
+// and a wave's rows of up to 1024 with both norms (2048 x 1024 with biases 22 for 29; 8192 x 1003 59 for 69, without
+// biases 54 for 51).  Up to four of the smallest rows, 16 rows a block at least (30000 x 200 26 for 29, but 8192 x 64
+// 14 for 13).
+int64_t backward_blocks(const orca_hip_ctx* ctx, int64_t rows, int64_t cols, bool both) {
+  if (cols > 4096 || (cols > 512 && cols <= 1024 && both)) return ctx->num_cus;
+  if (cols <= 256) return std::max<int64_t>(2 * ctx->num_cus, std::min<int64_t>(4 * ctx->num_cus, rows / 16));
+  return 2 * ctx->num_cus;
+}
+
 template <int NW, int Q, bool BIAS>
 auto backward_kernel(bool next, bool block, bool post) {
   if (!next) return post ? norm_backward_kernel<NW, Q, false, true, true, BIAS>
@@ -933,19 +951,24 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
   a.gate_rows = gate_rows ? a.rows / gate_rows : a.rows;
   a.gate_each = to[kSumGate] && a.gate_rows == 1;
   const bool gate_sum = to[kSumGate] && !a.gate_each;
-  // by the gate's rows also where their gradient is not wanted: the other sums then have the same bits
   a.gate_grouped = a.gate_rows != 1 && a.gate_rows != a.rows;
   a.groups = a.gate_grouped ? (int)(a.rows / a.gate_rows) : 1;
   a.group_rows = (int)(a.gate_grouped ? a.gate_rows : a.rows);
   const bool block = a.df || to[kSumGate] || to[kSumPostW] || to[kSumPostB];
   const bool registers = in_registers(a.cols);
+  // what the split of the rows and their shape go by: the parameters, and not which results are wanted
+  const bool both = a.du && a.post.kind != ORCA_HIP_NORM_NONE, heavy = both && (a.post.b || a.next.b);
   const int64_t strips = registers ? 1 : (a.cols + kStream * 4 - 1) / (kStream * 4);
-  int64_t blocks = std::max<int64_t>(1, 2 * ctx->num_cus / strips);
+  int64_t blocks = registers ? backward_blocks(ctx, a.rows, a.cols, both)
+                             : std::max<int64_t>(1, 2 * ctx->num_cus / strips);
   if (a.groups >= blocks) {
     a.per_group = 1;
   } else {
     const int64_t least = registers ? a.cols <= 1024 ? 4 : 1 : 16;  // rows of a piece
-    a.per_group = (int)std::min<int64_t>(blocks / a.groups, (a.group_rows + least - 1) / least);
+    const int64_t most = std::min<int64_t>(blocks / a.groups, (a.group_rows + least - 1) / least);
+    // no more pieces than the longest one's rows ask for: less to add up, and no later an end
+    const int64_t longest = (a.group_rows + least * most - 1) / (least * most) * least;
+    a.per_group = (int)((a.group_rows + longest - 1) / longest);
     blocks = (int64_t)a.groups * a.per_group;
   }
   // slots of the partial sums
@@ -980,9 +1003,8 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
     }
   }
   if (registers) {
-    const bool both = a.du && block && a.post.kind != ORCA_HIP_NORM_NONE;
-    const bool bias = a.post.b || a.sum[kSumPostB] || a.sum[kSumNextB];
-    with_row_shape(a.cols, both && bias, [&](auto nw, auto q) {
+    const bool bias = a.post.b || to[kSumPostB] || to[kSumNextB];
+    with_row_shape(a.cols, heavy, [&](auto nw, auto q) {
       launch_backward_rows<decltype(nw)::value, decltype(q)::value>(ctx, a, block, bias, (unsigned)blocks);
     });
     ORCA_HIP_CHECK(hipGetLastError());
@@ -1098,7 +1120,7 @@ int orca_hip_residual_norm(orca_hip_ctx* ctx, size_t rows, size_t cols, const fl
     check_sizes(op, {rows, cols});
     if (!block) fail(ORCA_HIP_ERR_INTERNAL, "residual_norm: null parameters");
     const orca_hip_residual_block& p = *block;
-    check_block(op, rows, cols, p);
+    check_block(op, "residual_norm (gate)", rows, cols, p);
     const bool next = p.next.kind != ORCA_HIP_NORM_NONE;
     check_ld("residual_norm (x)", ldx, cols);
     check_ld("residual_norm (f)", ldf, cols);
@@ -1159,7 +1181,7 @@ int orca_hip_residual_norm_backward(orca_hip_ctx* ctx, size_t rows, size_t cols,
     if (!block || !grads) fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: null parameters");
     const orca_hip_residual_block& p = *block;
     const orca_hip_residual_grads& o = *grads;
-    check_block(op, rows, cols, p);
+    check_block(op, "residual_norm_backward (gate)", rows, cols, p);
     const bool post = p.post.kind != ORCA_HIP_NORM_NONE;
     if (du && p.next.kind == ORCA_HIP_NORM_NONE)
       fail(ORCA_HIP_ERR_INTERNAL, "residual_norm_backward: du without a next norm");

@@ -109,6 +109,7 @@ int orca_hip_be_residual_norm_backward(orca_hip_backend* be, orca_hip_storage* d
                  {b.post_weight, cols, "residual_norm_backward (post weight)", true},
                  {b.post_bias, cols, "residual_norm_backward (post bias)", true},
                  {b.next_weight, cols, "residual_norm_backward (next weight)", true},
+                 {b.next_bias, cols, "residual_norm_backward (next bias)", true},
                  {b.gate, gn, "residual_norm_backward (gate)", true}},
                 {{mn, dx, true},
                  {mn, df, true},
@@ -118,7 +119,7 @@ int orca_hip_be_residual_norm_backward(orca_hip_backend* be, orca_hip_storage* d
                  {cols, dnext_weight, true},
                  {cols, dnext_bias, true}},
                 [&](orca_hip_ctx* ctx, float* const* i, float* const* o) {
-                  const orca_hip_residual_block p = block_of(b, i[4], i[5], i[6], nullptr, i[7], cols);
+                  const orca_hip_residual_block p = block_of(b, i[4], i[5], i[6], i[7], i[8], cols);
                   orca_hip_residual_grads g{};
                   g.dx = o[0];
                   g.df = o[1];

@@ -228,10 +228,26 @@ def test_joint_gates(ctx, m, groups, n):
     Joint(ctx, m + groups, m, n, "none", "none", groups, 0.0).check()
 
 
-@pytest.mark.parametrize("m,n", [(3000, 256), (1000, 1500), (2000, 4096)])
-def test_joint_large(ctx, m, n):
-    print(f"joint large {m} x {n}", flush=True)
-    Joint(ctx, m, m, n, "rms", "rms", 1, 0.1, bias=False).check()
+# more rows than the blocks take at once, in each length of row that has kernels of its own
+@pytest.mark.parametrize("m,n", [(3000, 256), (9000, 50), (2500, 400), (5000, 700), (1000, 1500), (2000, 4096), (1100, 2600),
+                                 (700, 6000)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_joint_large(ctx, m, n, bias):
+    print(f"joint large {m} x {n} bias {bias}", flush=True)
+    Joint(ctx, m, m, n, "rms", "rms", 1, 0.1, bias=bias).check()
+    if bias:
+        Joint(ctx, m + 1, m, n, "none", "layer", 0, 0.0, bias=bias).check()
+
+
+# each kernel: the lengths of a row that have one, the norms that are there, with biases and without
+@pytest.mark.parametrize("n", [200, 401, 1000, 1502, 3003, 6000])
+@pytest.mark.parametrize("post", NORMS)
+@pytest.mark.parametrize("next", NORMS)
+@pytest.mark.parametrize("bias", [False, True])
+def test_every_kernel(ctx, n, post, next, bias):
+    print(f"kernels {n} {post} {next} {bias}", flush=True)
+    for groups, p in ((0, 0.1), (1, 0.0), (3, 0.0), (9, 0.3)):
+        Joint(ctx, n + groups, 9, n, post, next, groups, p, bias=bias).check()
 
 
 def test_without_weights(ctx):
@@ -241,7 +257,7 @@ def test_without_weights(ctx):
 
 def test_gradients_of_one_side(ctx):
     """dy or du alone, and any part of the results alone, with the same bits."""
-    for n in (52, 1500):
+    for n in (52, 900, 1500, 4000, 8200):
         j = Joint(ctx, n, 40, n, "layer", "layer", 4, 0.25, rs=0.5)
         y = j.forward()["y"]
         full = j.backward(y)
