@@ -122,12 +122,18 @@ struct Stats {
   __device__ __forceinline__ float unit(float v) const { return fmaf(v - mean, r, off); }
 };
 // From the first mean and the sums of the differences to it and of their squares.
-__device__ __forceinline__ Stats stats_of(const Norm& n, float mean, float sum, float squares, float count) {
-  const float rest = n.kind == ORCA_HIP_NORM_LAYER ? sum / count : 0.0f;
-  const float var = fmaxf(fmaf(-rest, rest, squares / count), 0.0f), r = 1.0f / sqrtf(var + n.eps);
+// `share` is 1 / the number of values: a product with it costs a rounding more than a division, which takes ten
+// instructions a thread.
+__device__ __forceinline__ Stats stats_of(const Norm& n, float mean, float sum, float squares, float share) {
+  const float rest = n.kind == ORCA_HIP_NORM_LAYER ? sum * share : 0.0f;
+  const float var = fmaxf(fmaf(-rest, rest, squares * share), 0.0f), r = 1.0f / sqrtf(var + n.eps);
   return Stats{mean, -rest * r, r};
 }
 
+// v where bit n of `kept` is set, else 0.
+__device__ __forceinline__ float kept_or_zero(uint32_t kept, int n, float v) {
+  return __int_as_float(__float_as_int(v) & __builtin_amdgcn_sbfe((int)kept, n, 1));
+}
 __device__ __forceinline__ floatx4 splat(float v) { return floatx4{v, v, v, v}; }
 __device__ __forceinline__ floatx4 load4(const float* row, int64_t c, int64_t cols) {
   if (c + 4 <= cols) return *reinterpret_cast<const floatx4_u*>(row + c);
@@ -155,7 +161,7 @@ constexpr int kStream = 256;  // threads of a block, 4 columns each at a time
 
 __device__ __forceinline__ Stats stream_stats(const Norm& n, const float* row, int64_t cols, Team<4>& team) {
   float mean = 0.0f;
-  const float count = (float)cols;
+  const float share = 1.0f / (float)cols;
   if (n.kind == ORCA_HIP_NORM_LAYER) {
     float t[1] = {0.0f};
     for (int64_t c = threadIdx.x * 4; c < cols; c += kStream * 4) {
@@ -163,7 +169,7 @@ __device__ __forceinline__ Stats stream_stats(const Norm& n, const float* row, i
       t[0] += (v.x + v.y) + (v.z + v.w);
     }
     team.sum(t);
-    mean = t[0] / count;
+    mean = t[0] * share;
   }
   float t[2] = {0.0f, 0.0f};
   for (int64_t c = threadIdx.x * 4; c < cols; c += kStream * 4) {
@@ -176,7 +182,7 @@ __device__ __forceinline__ Stats stream_stats(const Norm& n, const float* row, i
     }
   }
   team.sum(t);
-  return stats_of(n, mean, t[0], t[1], count);
+  return stats_of(n, mean, t[0], t[1], share);
 }
 
 template <bool JOINT>
@@ -239,7 +245,7 @@ constexpr int kRowStats = 10;
 __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, bool block) {
   __shared__ float lds[2 * 4 * 4];
   Team<4> team{lds};
-  const float count = (float)a.cols;
+  const float share = 1.0f / (float)a.cols;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float *y = a.y + row * a.ldy, *du = a.du + row * a.lddu, *dy = a.dy + row * a.lddy;
     Stats sy{0.0f, 0.0f, 0.0f};
@@ -258,8 +264,8 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
         }
       }
       team.sum(t);
-      c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? t[0] / count : 0.0f;
-      c2 = t[1] / count;
+      c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? t[0] * share : 0.0f;
+      c2 = t[1] * share;
     }
     Stats sf{0.0f, 0.0f, 0.0f};
     float p1 = 0.0f, p2 = 0.0f;
@@ -289,8 +295,8 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
         }
       }
       team.sum(t);
-      p1 = a.post.kind == ORCA_HIP_NORM_LAYER ? t[0] / count : 0.0f;
-      p2 = t[1] / count;
+      p1 = a.post.kind == ORCA_HIP_NORM_LAYER ? t[0] * share : 0.0f;
+      p2 = t[1] * share;
     }
     if (threadIdx.x == 0) {
       float* s = a.stats + row * kRowStats;
@@ -465,14 +471,14 @@ struct RowCols {
 template <int NW, int Q>
 __device__ __forceinline__ Stats row_stats(const Norm& n, const floatx4 (&v)[Q], const RowCols<NW, Q>& rc,
                                            Team<NW>& team) {
-  const float count = (float)rc.cols;
+  const float share = 1.0f / (float)rc.cols;
   float mean = 0.0f, t[2] = {0.0f, 0.0f};
   if (n.kind == ORCA_HIP_NORM_LAYER) {
     float m[1] = {0.0f};
 #pragma unroll
     for (int i = 0; i < Q; ++i) m[0] += (v[i].x + v[i].y) + (v[i].z + v[i].w);
     team.sum(m);
-    mean = m[0] / count;
+    mean = m[0] * share;
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
       floatx4 d = v[i] - mean;
@@ -493,7 +499,7 @@ __device__ __forceinline__ Stats row_stats(const Norm& n, const floatx4 (&v)[Q],
     team.sum(q);
     t[1] = q[0];
   }
-  return stats_of(n, mean, t[0], t[1], count);
+  return stats_of(n, mean, t[0], t[1], share);
 }
 
 // The forward.  A team takes every step-th row and has the loads of its next row in flight while it works on one:
@@ -551,7 +557,7 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_rows_kernel(NormForward 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float t = f[i][j] * (g[j] * k);
-          v[i][j] = fmaf(a.rs, v[i][j], kept >> (4 * i + j) & 1 ? t : 0.0f);
+          v[i][j] = fmaf(a.rs, v[i][j], kept_or_zero(kept, 4 * i + j, t));
         }
         rc.store(a.y + row * a.ldy, i, v[i]);
         rc.mask(v[i], i);  // a bias may have stood behind the row
@@ -600,7 +606,7 @@ norm_backward_kernel(NormBackward a) {
   Team<NW> team{lds};
   const RowCols<NW, Q> rc(a.cols);
   const int tm = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, t = threadIdx.x % T;
-  const float count = (float)a.cols, k = a.bs * a.drop.scale;
+  const float share = 1.0f / (float)a.cols, k = a.bs * a.drop.scale;
   const bool gates = BLOCK && a.gate && a.gate_rows != a.rows;  // a gate for each row
   // A thread reads only what it wrote (all teams write the same).
   const auto put = [&](int n, const float* w, float none) {
@@ -679,8 +685,8 @@ norm_backward_kernel(NormBackward a) {
           }
         }
         team.sum(e);
-        c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? e[0] / count : 0.0f;
-        c2 = e[1] / count;
+        c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? e[0] * share : 0.0f;
+        c2 = e[1] * share;
       }
 #pragma unroll
       for (int i = 0; i < Q; ++i) {
@@ -717,11 +723,10 @@ norm_backward_kernel(NormBackward a) {
         rc.mask(g[i], i);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool on = kept >> (4 * i + j) & 1;
           if (POST) f[i][j] = s.unit(f[i][j]);
           const float out = POST ? BIAS ? fmaf(f[i][j], wp[j], bp[j]) : f[i][j] * wp[j] : f[i][j];
-          float dv = on ? g[i][j] * k : 0.0f;
-          each[j] = on ? dv * out : 0.0f;
+          float dv = kept_or_zero(kept, 4 * i + j, g[i][j] * k);
+          each[j] = kept_or_zero(kept, 4 * i + j, dv * out);
           sum[kSumGate][i][j] += each[j];
           dv *= gate[j];
           if (POST) {
@@ -737,8 +742,8 @@ norm_backward_kernel(NormBackward a) {
       }
       if (POST) {
         team.sum(e);
-        c1 = a.post.kind == ORCA_HIP_NORM_LAYER ? e[0] / count : 0.0f;
-        c2 = e[1] / count;
+        c1 = a.post.kind == ORCA_HIP_NORM_LAYER ? e[0] * share : 0.0f;
+        c2 = e[1] * share;
 #pragma unroll
         for (int i = 0; i < Q; ++i)
 #pragma unroll

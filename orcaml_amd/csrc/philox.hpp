@@ -4,8 +4,8 @@
 // A counter (col / 4, row, offset) gives the words of four neighbouring columns, which one thread holds.
 //
 // Cost: ten rounds of two 32 x 32 -> 64 bit products, which run at a quarter of the vector units' rate: 320 cycles
-// of a SIMD for a wave's 256 values, and about 160 for the rest.  A CU's share of HBM (21 GB/s) brings the 8 bytes
-// that a value's dropout moves no faster than 2.6 values a ns, and its four SIMDs draw 5.
+// of a SIMD for a wave's 256 values, and about 80 for the rest.  A CU's share of HBM (21 GB/s) brings the 8 bytes
+// that a value's dropout moves no faster than 2.6 values a ns, and its four SIMDs draw 6.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -42,12 +42,16 @@ namespace {
 struct Words {
   uint32_t v[4];
 };
+// a ^ b ^ c in one instruction (its truth table).
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
 __device__ __forceinline__ Words philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c0 = xor3((uint32_t)(b >> 32), c1, k0);
+    c2 = xor3((uint32_t)(a >> 32), c3, k1);
     c1 = (uint32_t)b;
     c3 = (uint32_t)a;
     k0 += 0x9E3779B9u;
