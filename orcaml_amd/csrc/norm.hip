@@ -451,6 +451,28 @@ struct RowCols {
     for (int j = 0; j < 3; ++j)
       if (j < h) p[j] = v[j];
   }
+  // A quad's codes of an 8-bit checkpoint; eight neighbouring threads share a step.
+  __device__ __forceinline__ void store_codes(const Act8& out, int64_t row, int i, floatx4 v) const {
+    mask(v, i);
+    uint32_t top = max(max(act8_magnitude(v.x), act8_magnitude(v.y)), max(act8_magnitude(v.z), act8_magnitude(v.w)));
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    const uint32_t byte = act8_byte(top);
+    const int h = have(i);
+    if (h <= 0) return;
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w |= ((uint32_t)act8_code(v[j], byte) & 255u) << (8 * j);
+    int8_t* p = out.codes + row * out.cols + (uint32_t)c(i);
+    if (h >= 4) {
+      *reinterpret_cast<word_u*>(p) = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+        if (j < h) p[j] = (int8_t)(w >> (8 * j));
+    }
+    if ((threadIdx.x & 7) == 0) out.scales[((uint32_t)c(i) >> 5) * out.ld + row] = (uint8_t)byte;
+  }
   // Bit 4 i + j: the dropout keeps column c(i) + j.
   __device__ __forceinline__ uint32_t kept(const Dropout& d, int64_t row) const {
     static_assert(Q <= 8, "a word has 32 bits");
@@ -570,14 +592,7 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_rows_kernel(NormForward 
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[i][j] = fmaf(s.unit(v[i][j]), wn[i][j], bn[i][j]);
         rc.store(a.u + row * a.ldu, i, v[i]);
-        if (a.u8.codes) {
-          const Quad q = quad_of(rc.c(i), a.cols);
-          const uint32_t byte = quad_byte(v[i], q);
-          if (q.have > 0) {
-            store_codes(a.u8.codes + row * a.u8.cols, q, v[i], byte);
-            if ((threadIdx.x & 7) == 0) a.u8.scales[q.group * a.u8.ld + row] = (uint8_t)byte;
-          }
-        }
+        if (a.u8.codes) rc.store_codes(a.u8, row, i, v[i]);
       }
     }
     if (after >= a.rows) return;
@@ -880,26 +895,27 @@ void with_row_shape(int64_t cols, bool many, F f) {
 constexpr int kForwardBlocks = 4;  // a CU
 bool in_registers(int64_t cols) { return cols >= 4 && cols <= kMaxRegisterRow; }
 
+template <int NW, int Q>
+void launch_forward_rows(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
+  constexpr int TEAMS = kRowThreads<NW> / (64 * NW);
+  const dim3 grid((unsigned)std::min<int64_t>((a.rows + TEAMS - 1) / TEAMS, (int64_t)ctx->num_cus * kForwardBlocks));
+  const auto kernel = joint ? norm_rows_kernel<NW, Q, true> : norm_rows_kernel<NW, Q, false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(kRowThreads<NW>), 0, ctx->stream, a);
+}
 void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
-  if (in_registers(a.cols)) {
+  if (!in_registers(a.cols)) {
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, kMaxBlocks));
+    hipLaunchKernelGGL(joint ? norm_stream_kernel<true> : norm_stream_kernel<false>, grid, dim3(kStream), 0, ctx->stream,
+                       a);
+  } else if (a.cols > 512 && a.cols <= 1024 && a.rows <= 4 * ctx->num_cus) {
+    // four waves a row where one a row would leave CUs without any (joint 777 x 1003: 8.4 us for 10.0, but
+    // 2048 x 1024 10.3 for 8.9)
+    launch_forward_rows<4, 1>(ctx, a, joint);
+  } else {
     // joint 1024 x 4096: 14.2 us in eight waves, 15.4 in four; norm 6.9 in four, 7.6 in eight
     with_row_shape(a.cols, joint, [&](auto nw, auto q) {
-      const int64_t rows = decltype(nw)::value == 1 ? 4 : 1;
-      const dim3 grid((unsigned)std::min<int64_t>((a.rows + rows - 1) / rows, (int64_t)ctx->num_cus * kForwardBlocks));
-      const dim3 threads(kRowThreads<decltype(nw)::value>);
-      if (joint)
-        hipLaunchKernelGGL((norm_rows_kernel<decltype(nw)::value, decltype(q)::value, true>), grid, threads, 0,
-                           ctx->stream, a);
-      else
-        hipLaunchKernelGGL((norm_rows_kernel<decltype(nw)::value, decltype(q)::value, false>), grid, threads, 0,
-                           ctx->stream, a);
+      launch_forward_rows<decltype(nw)::value, decltype(q)::value>(ctx, a, joint);
     });
-  } else {
-    const dim3 grid((unsigned)std::min<int64_t>(a.rows, kMaxBlocks));
-    if (joint)
-      hipLaunchKernelGGL(norm_stream_kernel<true>, grid, dim3(kStream), 0, ctx->stream, a);
-    else
-      hipLaunchKernelGGL(norm_stream_kernel<false>, grid, dim3(kStream), 0, ctx->stream, a);
   }
   ORCA_HIP_CHECK(hipGetLastError());
 }
