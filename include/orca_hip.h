@@ -779,8 +779,8 @@ int orca_hip_linear_act_backward(orca_hip_ctx* ctx, size_t M, size_t N, size_t K
  * unit(v) of a row v of n values:
  *   ORCA_HIP_NORM_LAYER  (v - mean) / sqrt(mean((v - mean)^2) + eps)
  *   ORCA_HIP_NORM_RMS    v / sqrt(mean(v^2) + eps)
- * and norm(v) = unit(v) * weight + bias.  A NaN or an infinity makes its row's outputs NaN or 0, as the
- * formula in fp32 does, and no other's; so do values whose squares overflow fp32 (beyond 2^63). */
+ * and norm(v) = unit(v) * weight + bias.  What a NaN, an infinity or squares whose sum overflows fp32 make of a row,
+ * as in the formula in fp32 (NaN, or unit(v) = 0), changes no other row; sums over rows have it. */
 #define ORCA_HIP_NORM_NONE 0
 #define ORCA_HIP_NORM_LAYER 1
 #define ORCA_HIP_NORM_RMS 2

@@ -556,10 +556,11 @@ class Module:
     """Parameter order: own parameters, then submodules in insertion order
     (python/orca/nn/module.py:32-44)."""
 
+    training = True
+
     def __init__(self):
         object.__setattr__(self, "_parameters", {})
         object.__setattr__(self, "_modules", {})
-        object.__setattr__(self, "training", True)
 
     def train(self, mode: bool = True) -> "Module":
         """Sets whether this module and those below it are in training (Dropout and ResidualNorm drop values then)."""
@@ -854,8 +855,9 @@ class ResidualNorm(Module):
 
     called as joint(x, f, gate) on the residual stream x and a block's output f; gives (y, u), or y alone without a
     next norm.  post and next are LayerNorm or RMSNorm modules over the same features, or None; next's `checkpoint`
-    goes for u.  The gate is a tensor of [..., features] whose leading dimensions have as many elements as x's, or
-    a divisor of that: each of its rows is for as many successive rows of x.  gate_weight gives the joint one row of
+    goes for u.  The gate is a tensor of x's shape with ones in the dimensions from some on, the last aside (a gate a
+    value, a sample, or one for all); for x [rows, features] it may be [groups, features], each row for as many
+    successive rows of x.  gate_weight gives the joint one row of
     its own, trained with it (a scale a channel), in place of the argument.  y.grad() is the whole gradient of y, with
     what came through u."""
 
@@ -890,9 +892,14 @@ class ResidualNorm(Module):
             gate = self.gate.tensor
         elif gate is not None:
             groups = _rows_cols(gate, N, op)[0]
-            if groups == 0 or M % groups:
-                raise OrcaError(f"Shape mismatch during {op}: expected a gate with a divisor of {M} rows, "
-                                f"got {list(gate.shape)}")
+            lead, same = gate.shape[:-1], 0
+            while same < len(lead) and len(lead) == len(x.shape) - 1 and lead[same] == x.shape[same]:
+                same += 1
+            # [..., 1, 1, features] broadcasts; with one leading dimension each, rows in groups are meant
+            fits = all(d == 1 for d in lead[same:]) or (len(lead) == 1 and len(x.shape) == 2)
+            if not fits or groups == 0 or M % groups:
+                raise OrcaError(f"Shape mismatch during {op}: expected a gate of {list(x.shape)} with ones from some "
+                                f"dimension on, got {list(gate.shape)}")
         post, nxt = self.post, self.next
         vectors = {k: _vector(p, N, op) for k, p in
                    (("post_weight", post and post.weight), ("post_bias", post and post.bias),

@@ -22,24 +22,28 @@ __global__ void __launch_bounds__(256) dropout_kernel(const float* x, int64_t ld
                                                       int64_t ldy, int across_bits, Dropout d) {
   const int64_t quad = ((((int64_t)blockIdx.z * gridDim.y + blockIdx.y) << across_bits) +
                         (threadIdx.x & ((1 << across_bits) - 1)));
-  const int64_t row = (int64_t)blockIdx.x * (256 >> across_bits) + (threadIdx.x >> across_bits);
+  const int64_t down = 256 >> across_bits;
   const Quad q = quad_of(quad * 4, cols);
-  const float* from = x + min(row, rows - 1) * ldx;
-  floatx4 v = FAR && q.n == 4 ? (floatx4)__builtin_nontemporal_load(reinterpret_cast<const floatx4_u*>(from + q.at))
-                              : load_quad(from, q);
-  settle(q, v);
-  if (d.on) {
-    const Words w = dropout_words(d, row, quad);
+  for (int64_t r0 = (int64_t)blockIdx.x * down; r0 < rows; r0 += (int64_t)gridDim.x * down) {
+    const int64_t row = r0 + (threadIdx.x >> across_bits);
+    const float* from = x + min(row, rows - 1) * ldx;
+    floatx4 v = FAR && q.n == 4 ? (floatx4)__builtin_nontemporal_load(reinterpret_cast<const floatx4_u*>(from + q.at))
+                                : load_quad(from, q);
+    settle(q, v);
+    if (d.on) {
+      const Words w = dropout_words(d, row, quad);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = dropout_keeps(d, w, j) ? v[j] * d.scale : 0.0f;
+      for (int j = 0; j < 4; ++j) v[j] = dropout_keeps(d, w, j) ? v[j] * d.scale : 0.0f;
+    }
+    if (row >= rows) continue;
+    if (q.have == 4)
+      __builtin_nontemporal_store((floatx4_u)v, reinterpret_cast<floatx4_u*>(y + row * ldy + q.c));
+    else
+      store_quad(y + row * ldy, q, v);
   }
-  if (row >= rows) return;
-  if (q.have == 4)
-    __builtin_nontemporal_store((floatx4_u)v, reinterpret_cast<floatx4_u*>(y + row * ldy + q.c));
-  else
-    store_quad(y + row * ldy, q, v);
 }
 
+constexpr size_t kMaxBlocks = size_t(1) << 23;  // in the first dimension, whose threads the runtime counts in 32 bits
 constexpr double kCacheBytes = 256.0 * (1 << 20);  // of the memory-side cache
 
 }  // namespace
@@ -69,7 +73,7 @@ int orca_hip_dropout(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* x
     while (bits < 8 && (size_t(1) << bits) < quads) ++bits;
     const size_t across = (quads + (size_t(1) << bits) - 1) >> bits, gy = std::min<size_t>(across, 32768),
                  down = size_t(256) >> bits;
-    const dim3 grid((unsigned)((rows + down - 1) / down), (unsigned)gy, (unsigned)((across + gy - 1) / gy));
+    const dim3 grid((unsigned)std::min((rows + down - 1) / down, kMaxBlocks), (unsigned)gy, (unsigned)((across + gy - 1) / gy));
     ProfScope prof(ctx, op, (double)rows * cols, 8.0 * rows * cols);
     hipLaunchKernelGGL(8.0 * rows * cols >= kCacheBytes ? dropout_kernel<true> : dropout_kernel<false>, grid, dim3(256), 0,
                        ctx->stream, x, (int64_t)ldx, (int64_t)rows, (int64_t)cols, y, (int64_t)ldy, bits,

@@ -126,7 +126,9 @@ struct Stats {
 // instructions a thread.
 __device__ __forceinline__ Stats stats_of(const Norm& n, float mean, float sum, float squares, float share) {
   const float rest = n.kind == ORCA_HIP_NORM_LAYER ? sum * share : 0.0f;
-  const float var = fmaxf(fmaf(-rest, rest, squares * share), 0.0f), r = 1.0f / sqrtf(var + n.eps);
+  float var = fmaf(-rest, rest, squares * share);
+  var = var < 0.0f ? 0.0f : var;  // a NaN stays one
+  const float r = 1.0f / sqrtf(var + n.eps);
   return Stats{mean, -rest * r, r};
 }
 
@@ -899,7 +901,9 @@ template <int NW, int Q>
 void launch_forward_rows(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
   constexpr int TEAMS = kRowThreads<NW> / (64 * NW);
   const dim3 grid((unsigned)std::min<int64_t>((a.rows + TEAMS - 1) / TEAMS, (int64_t)ctx->num_cus * kForwardBlocks));
-  const auto kernel = joint ? norm_rows_kernel<NW, Q, true> : norm_rows_kernel<NW, Q, false>;
+  auto kernel = norm_rows_kernel<NW, Q, NW == 8 && Q == 2>;  // of with_row_shape's two for 2049 to 4096 values
+  if constexpr (!(NW == 8 && Q == 2) && !(NW == 4 && Q == 4))
+    kernel = joint ? norm_rows_kernel<NW, Q, true> : norm_rows_kernel<NW, Q, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(kRowThreads<NW>), 0, ctx->stream, a);
 }
 void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {

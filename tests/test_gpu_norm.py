@@ -305,7 +305,7 @@ def test_in_place(ctx):
         np.testing.assert_array_equal(outs[0], outs[1])
 
 
-@pytest.mark.parametrize("m,n", [(5, 8), (17, 33), (40, 1003), (16, 1024), (3, 4100), (2, 9001)])
+@pytest.mark.parametrize("m,n", [(3, 1), (4, 3), (5, 8), (17, 33), (40, 1003), (16, 1024), (3, 4100), (2, 9001)])
 def test_checkpoint_of_the_output(ctx, m, n):
     """The checkpoint is that of the values written, and writing it changes none of them."""
     rng = np.random.default_rng(n)
@@ -347,6 +347,32 @@ def test_bad_rows_keep_to_themselves(ctx, n):
     np.testing.assert_array_equal(back["df"], clean_back["df"])  # without a post norm f is no part of it
     np.testing.assert_array_equal(back["dgate"][rows], clean_back["dgate"][rows])
     assert (back["dgate"][dropped] == 0).all()
+
+
+@pytest.mark.parametrize("n", [7, 300, 1000, 2000, 4000, 8000, 9000])
+def test_what_a_bad_value_makes_of_its_row(ctx, n):
+    """As the formulas in fp32: NaN throughout, but 0 at the finite values of an rms row with an infinity."""
+    rng = np.random.default_rng(n)
+    x, w, b = stream(rng, 6, n), (1 + rng.random(n)).astype(np.float32), rng.standard_normal(n).astype(np.float32)
+    x[1, 3], x[3, n - 1], x[4, 0] = np.nan, np.inf, -np.inf
+    mx, my, dy, dx = Matrix(ctx, 6, n, x), Matrix(ctx, 6, n), Matrix(ctx, 6, n, stream(rng, 6, n)), Matrix(ctx, 6, n)
+    ws = ctx.upload(w), ctx.upload(b)
+    for kind in ("layer", "rms"):
+        p = params(kind, *ws)
+        _lib.call("orca_hip_norm", ctx.handle, 6, n, mx.ptr, n, ctypes.byref(p), my.ptr, n, None)
+        got = my.read()
+        assert np.isnan(got[1]).all() and np.isfinite(got[[0, 2, 5]]).all()
+        for row, col in ((3, n - 1), (4, 0)):
+            rest = np.arange(n) != col
+            assert np.isnan(got[row, col])
+            if kind == "layer":
+                assert np.isnan(got[row]).all()
+            else:
+                np.testing.assert_array_equal(got[row][rest], b[rest])
+        _lib.call("orca_hip_norm_backward", ctx.handle, 6, n, dy.ptr, n, mx.ptr, n, ctypes.byref(p), None, 0, dx.ptr, n,
+                  None, None)
+        got = dx.read()
+        assert np.isnan(got[1]).all() and np.isfinite(got[[0, 2, 5]]).all()
 
 
 def test_rows_of_one_value(ctx):

@@ -361,7 +361,9 @@ def test_refusals(hb):
         A.ResidualNorm(ad, 8, post=A.RMSNorm(ad, 9))
     joint = A.ResidualNorm(ad, 8)
     for x, f, g in ((ones(6, 8), ones(6, 7), None), (ones(6, 8), ones(3, 8), None), (ones(6, 8), ones(6, 8), ones(4, 8)),
-                    (ones(6, 8), ones(6, 8), ones(6, 7)), (ones(6, 7), ones(6, 7), None)):
+                    (ones(6, 8), ones(6, 8), ones(6, 7)), (ones(6, 7), ones(6, 7), None),
+                    (ones(4, 6, 8), ones(4, 6, 8), ones(1, 6, 8)), (ones(4, 4, 8), ones(4, 4, 8), ones(4, 8)),
+                    (ones(4, 6, 8), ones(4, 6, 8), ones(2, 1, 8))):
         with pytest.raises(ValueError, match="Shape mismatch"):
             joint(x, f, g)
     with pytest.raises(ValueError, match="no other|takes no"):

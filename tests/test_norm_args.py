@@ -153,3 +153,8 @@ def test_null_parameters():
                  ("orca_hip_be_residual_norm_backward", None, None, None, None, None, 4, 16, None) + (None,) * 7):
         rc, msg = _call(*args)
         assert rc == INTERNAL and "null parameters" in msg, msg
+
+
+def test_the_rust_struct_matches_the_header():
+    from tests.test_rust_binding import _c_struct, _rust_struct
+    assert _rust_struct("OrcaHipBeResidualBlock") == _c_struct("orca_hip_be_residual_block")
