@@ -121,7 +121,8 @@ class Autodiff:
 
     def custom_pair(self, primals, inputs, backward):
         """custom() for a node with two outputs, which later nodes read independently: backward((g0, g1), backend)
-        gets None for an output that no gradient reached and runs unless that is both."""
+        gets None for an output that no gradient reached (it runs unless that is both) and returns the inputs'
+        gradients and the first output's own with what came through the second, which the tape then holds for it."""
         outs = [AdStorage(p) for p in primals]
         if not self.grad_enabled:
             return outs
@@ -134,7 +135,8 @@ class Autodiff:
             g = [tape.grads.get(i) for i in ids]
             if all(v is None for v in g):
                 return
-            for i, gi in zip(wanted, backward(g, be)):
+            grads, tape.grads[ids[0]] = backward(g, be)
+            for i, gi in zip(wanted, grads):
                 if i is not None and gi is not None:
                     tape.accumulate(i, gi, be)
         self.tape.push_node(run)
@@ -807,7 +809,8 @@ class RMSNorm(_Norm):
 
 class _Draws:
     """The numbers of a layer's dropout: every call in training takes the next offset under the layer's seed, so
-    that a run repeats from its seeds and no two calls share a mask.  Layers take different seeds."""
+    that a run repeats from its seeds and no two calls share a mask.  Layers take different seeds.  `calls` is the
+    place in the sequence: a run that goes on from a checkpoint sets it."""
 
     def __init__(self, seed: int):
         if not 0 <= seed < 2 ** 64:
@@ -921,22 +924,23 @@ class ResidualNorm(Module):
         want = tuple(k for k, s in inputs.items() if s.node_id is not None)
         reads_f = any(k in want for k in ("dgate", "dpost_weight", "dpost_bias")) or ("df" in want and post is not None)
         fp, yp = f.storage.primal if reads_f else None, y if nxt is not None else None
-        rs, names, node = self.residual_scale, tuple(inputs), {}  # the node holds no more of the operands than that
+        rs, names = self.residual_scale, tuple(inputs)  # the node holds no more of the operands than that
 
-        def backward(gy, gu, be):
-            asked = want if gu is not None else tuple(k for k in want if not k.startswith("dnext"))
-            # dx is asked for in any case: it is y's own gradient, scaled
-            out = be.residual_norm_backward(gy, gu, fp, yp, M, N, block, want=tuple({*asked, "dx"}))
-            total = out["dx"] if rs == 1.0 else be.mul_scalar(out["dx"], 1.0 / rs, (M, N))
-            ad.tape.grads[node["y"]] = total
-            return [out.get(k) if k in want else None for k in names]
+        def gradients(gy, gu, be, asked):
+            return be.residual_norm_backward(gy, gu, fp, yp, M, N, block, want=asked)
 
         if nxt is None:
-            ys = ad.custom(y, list(inputs.values()), lambda g, be: backward(g, None, be))
-            node["y"] = ys.node_id
-            return Tensor(ad, ys, x.shape)
-        ys, us = ad.custom_pair((y, u), list(inputs.values()), lambda g, be: backward(*g, be))
-        node["y"] = ys.node_id
+            def backward(g, be):
+                out = gradients(g, None, be, want)
+                return [out.get(k) for k in names]
+            return Tensor(ad, ad.custom(y, list(inputs.values()), backward), x.shape)
+
+        def backward(g, be):
+            asked = want if g[1] is not None else tuple(k for k in want if not k.startswith("dnext"))
+            out = gradients(*g, be, tuple({*asked, "dx"}))  # dx in any case: it is y's own gradient, scaled
+            whole = out["dx"] if rs == 1.0 else be.mul_scalar(out["dx"], 1.0 / rs, (M, N))
+            return [out.get(k) if k in want else None for k in names], whole
+        ys, us = ad.custom_pair((y, u), list(inputs.values()), backward)
         ty, tu = Tensor(ad, ys, x.shape), Tensor(ad, us, x.shape)
         if u8 is not None:
             tu.checkpoint, tu.checkpoint_of = u8, weakref.ref(u)

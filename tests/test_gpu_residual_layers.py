@@ -214,6 +214,24 @@ def test_the_joint_keeps_what_its_backward_reads(hb):
     ad.tape.clear()
 
 
+def test_nodes_hold_no_cycle(hb):
+    """A tape that is dropped releases its storages at once."""
+    gc.collect()
+    gc.disable()
+    try:
+        before = hb.ctx.mem_stats()["live"]
+        ad = A.Autodiff(hb)
+        x, f = (A.Tensor.from_numpy(ad, np.ones((64, 128)), requires_grad=True) for _ in range(2))
+        joint = A.ResidualNorm(ad, 128, A.RMSNorm(ad, 128), A.LayerNorm(ad, 128), p=0.1)
+        y, u = joint(A.Dropout(0.5)(A.LayerNorm(ad, 128)(x)), f)
+        (y.sum() + u.sum()).backward()
+        assert hb.ctx.mem_stats()["live"] > before
+        del ad, x, f, joint, y, u
+        assert hb.ctx.mem_stats()["live"] == before
+    finally:
+        gc.enable()
+
+
 class Block:
     """norm, up, down, joint: two residual feed-forward blocks with everything there is."""
 
