@@ -457,6 +457,52 @@ def test_nothing_to_do(ctx):
             assert (t.read() == 0).all()
 
 
+def test_operands_that_are_too_small_or_freed(ctx):
+    """Found on the host, before any launch (blocks are whole multiples of 256 bytes)."""
+    small, big, p = ctx.alloc(256), ctx.alloc(512), params("rms", None, None)
+    with pytest.raises(_lib.OrcaHipError, match=r"norm \(x\)"):
+        _lib.call("orca_hip_norm", ctx.handle, 8, 16, small.ptr, 16, ctypes.byref(p), big.ptr, 16, None)
+    with pytest.raises(_lib.OrcaHipError, match=r"norm \(y\)"):
+        _lib.call("orca_hip_norm", ctx.handle, 8, 16, big.ptr, 16, ctypes.byref(p), small.ptr, 16, None)
+    with pytest.raises(_lib.OrcaHipError, match=r"dropout \(y\)"):
+        _lib.call("orca_hip_dropout", ctx.handle, 8, 16, big.ptr, 16, 0.5, 0, 0, small.ptr, 16)
+    b = _lib.ResidualBlock(next=p, gate=small.ptr, groups=8, ldgate=16, residual_scale=1.0, block_scale=1.0)
+    others = [ctx.alloc(512) for _ in range(4)]
+    with pytest.raises(_lib.OrcaHipError, match=r"residual_norm \(gate\)"):
+        _lib.call("orca_hip_residual_norm", ctx.handle, 8, 16, big.ptr, 16, others[0].ptr, 16, ctypes.byref(b),
+                  others[1].ptr, 16, others[2].ptr, 16, None)
+    ptr = others.pop().ptr
+    ctx.release_dropped()
+    with pytest.raises(_lib.OrcaHipError, match="freed"):
+        _lib.call("orca_hip_norm", ctx.handle, 8, 16, ptr, 16, ctypes.byref(p), big.ptr, 16, None)
+
+
+def test_on_the_side_stream(ctx):
+    """A forward runs there; a backward that needs a workspace is refused, and one block's, which needs none, runs."""
+    j = Joint(ctx, 11, 600, 300, "rms", "layer", 1, 0.2)
+    one = Joint(ctx, 12, 6, 300, "rms", "layer", 1, 0.2)
+    want, want_one = j.forward(), one.backward(one.host["x"])
+    d, y, u, dw = j.dev, j.matrix(), j.matrix(), j.matrix(rows=1)
+    od, ody, odx = one.dev, one.matrix(one.host["x"]), one.matrix()
+    ctx.sync()
+    ctx.use_side_stream(-1)
+    try:
+        _lib.call("orca_hip_residual_norm", ctx.handle, j.m, j.n, d["x"].ptr, j.n, d["f"].ptr, j.n, ctypes.byref(j.block),
+                  y.ptr, j.n, u.ptr, j.n, None)
+        g = _lib.ResidualGrads(dx=odx.ptr, lddx=one.n)
+        _lib.call("orca_hip_residual_norm_backward", ctx.handle, one.m, one.n, od["dy"].ptr, one.n, od["du"].ptr, one.n,
+                  od["f"].ptr, one.n, ody.ptr, one.n, ctypes.byref(one.block), ctypes.byref(g))
+        with pytest.raises(_lib.OrcaHipError, match="side stream"):
+            _lib.call("orca_hip_norm_backward", ctx.handle, j.m, j.n, d["dy"].ptr, j.n, d["x"].ptr, j.n,
+                      ctypes.byref(j.block.next), None, 0, None, 0, dw.ptr, None)
+    finally:
+        ctx.use_side_stream(0)
+    ctx.sync()
+    for k, m in (("y", y), ("u", u)):
+        np.testing.assert_array_equal(m.read(), want[k])
+    np.testing.assert_array_equal(odx.read(), want_one["dx"])
+
+
 def test_another_context_on_its_own_stream(ctx):
     """Two contexts, so two streams, at once: each gives what it gives alone."""
     from orcaml_amd.device import Context

@@ -158,3 +158,15 @@ def test_null_parameters():
 def test_the_rust_struct_matches_the_header():
     from tests.test_rust_binding import _c_struct, _rust_struct
     assert _rust_struct("OrcaHipBeResidualBlock") == _c_struct("orca_hip_be_residual_block")
+
+
+def test_layers_need_a_backend_that_has_them():
+    from orcaml_amd import autodiff as A
+    ad = A.Autodiff(object())
+    for layer in (A.LayerNorm, A.RMSNorm, A.ResidualNorm):
+        with pytest.raises(A.OrcaError, match="needs a backend"):
+            layer(ad, 4)
+    x = A.Tensor(ad, A.AdStorage(None), (2, 4))
+    with pytest.raises(A.OrcaError, match="needs a backend"):
+        A.Dropout(0.5)(x)
+    assert A.Dropout(0.5).eval()(x) is x
