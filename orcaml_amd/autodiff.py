@@ -22,6 +22,7 @@ the HIP backend exactly as they would:
 from __future__ import annotations
 
 import contextlib
+import itertools
 import math
 import weakref
 from typing import Iterable
@@ -809,10 +810,15 @@ class RMSNorm(_Norm):
 
 class _Draws:
     """The numbers of a layer's dropout: every call in training takes the next offset under the layer's seed, so
-    that a run repeats from its seeds and no two calls share a mask.  Layers take different seeds.  `calls` is the
-    place in the sequence: a run that goes on from a checkpoint sets it."""
+    that a run repeats from its seeds and no two calls share a mask.  Layers that are given seeds take different ones;
+    those without get the next of the process's, from 2^63 on.  `calls` is the place in the sequence: a run that goes
+    on from a checkpoint sets it."""
 
-    def __init__(self, seed: int):
+    _seeds = itertools.count(2 ** 63)
+
+    def __init__(self, seed: int | None):
+        if seed is None:
+            seed = next(self._seeds)
         if not 0 <= seed < 2 ** 64:
             raise ValueError(f"a dropout's seed must be a number of 64 bits, got {seed}")
         self.seed, self.calls = seed, 0
@@ -833,7 +839,7 @@ class Dropout(Module):
     The mask is drawn from (seed, number of the call, place of the value) in the forward and again in the backward,
     and never stored."""
 
-    def __init__(self, p: float = 0.5, seed: int = 0):
+    def __init__(self, p: float = 0.5, seed: int | None = None):
         super().__init__()
         self.p, self.draws = _check_p(p), _Draws(seed)
 
@@ -865,8 +871,8 @@ class ResidualNorm(Module):
     what came through u."""
 
     def __init__(self, ad: Autodiff, features: int, post: _Norm | None = None, next: _Norm | None = None,
-                 gate_weight: np.ndarray | None = None, p: float = 0.0, seed: int = 0, residual_scale: float = 1.0,
-                 block_scale: float = 1.0):
+                 gate_weight: np.ndarray | None = None, p: float = 0.0, seed: int | None = None,
+                 residual_scale: float = 1.0, block_scale: float = 1.0):
         super().__init__()
         if not hasattr(ad.inner, "residual_norm"):
             raise OrcaError("ResidualNorm needs a backend with residual_norm")

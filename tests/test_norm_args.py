@@ -170,3 +170,15 @@ def test_layers_need_a_backend_that_has_them():
     with pytest.raises(A.OrcaError, match="needs a backend"):
         A.Dropout(0.5)(x)
     assert A.Dropout(0.5).eval()(x) is x
+
+
+def test_layers_without_a_seed_draw_apart():
+    from orcaml_amd import autodiff as A
+
+    class Backend:
+        residual_norm = None
+
+    ad = A.Autodiff(Backend())
+    layers = [A.Dropout(0.5), A.Dropout(0.5), A.ResidualNorm(ad, 4, p=0.5), A.ResidualNorm(ad, 4, p=0.5)]
+    assert len({layer.draws.seed for layer in layers}) == len(layers)
+    assert A.Dropout(0.5, seed=0).draws.seed == 0 and A.ResidualNorm(ad, 4, p=0.5, seed=7).draws.seed == 7
