@@ -880,8 +880,10 @@ class ResidualNorm(Module):
             if n is not None and n.features != features:
                 raise OrcaError(f"Shape mismatch during residual_norm: expected norms of {features} features, "
                                 f"got {n.features}")
-        if not (math.isfinite(residual_scale) and residual_scale != 0.0 and math.isfinite(block_scale)):
-            raise ValueError("a joint's scales must be finite, and residual_scale not 0")
+        # y's gradient is dx over residual_scale: it and its inverse are floats of full precision
+        largest = float(np.finfo(np.float32).max)
+        if not (2.0 ** -126 <= abs(residual_scale) <= 2.0 ** 126 and abs(block_scale) <= largest):
+            raise ValueError("a joint's scales must be floats of 32 bits, residual_scale from 2^-126 to 2^126 in size")
         self.features, self.p, self.draws = features, _check_p(p), _Draws(seed)
         self.residual_scale, self.block_scale = residual_scale, block_scale
         self.post, self.next = post, next

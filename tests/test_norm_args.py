@@ -3,6 +3,7 @@ come before any work, so they need no GPU."""
 from __future__ import annotations
 
 import ctypes
+import math
 
 import pytest
 
@@ -182,3 +183,22 @@ def test_layers_without_a_seed_draw_apart():
     layers = [A.Dropout(0.5), A.Dropout(0.5), A.ResidualNorm(ad, 4, p=0.5), A.ResidualNorm(ad, 4, p=0.5)]
     assert len({layer.draws.seed for layer in layers}) == len(layers)
     assert A.Dropout(0.5, seed=0).draws.seed == 0 and A.ResidualNorm(ad, 4, p=0.5, seed=7).draws.seed == 7
+
+
+def test_scales_a_float_cannot_hold():
+    """y's gradient is dx over the residual's scale, so the scale and its inverse are floats of full precision."""
+    from orcaml_amd import autodiff as A
+
+    class Backend:
+        residual_norm = None
+
+    ad = A.Autodiff(Backend())
+    for bad in ({"residual_scale": 1e-50}, {"residual_scale": 1e-40}, {"residual_scale": -1e-40}, {"residual_scale": 1e39},
+                {"residual_scale": 3e38}, {"residual_scale": 0.0}, {"residual_scale": math.nan}, {"block_scale": 1e39},
+                {"block_scale": 2.0 ** 128 * (1 - 2.0 ** -30)},
+                {"block_scale": -math.inf}):
+        with pytest.raises(ValueError, match="scale"):
+            A.ResidualNorm(ad, 4, **bad)
+    for good in ({"residual_scale": 2.0 ** -126}, {"residual_scale": -2.0 ** 126}, {"block_scale": 0.0},
+                 {"block_scale": 1e-50}):
+        A.ResidualNorm(ad, 4, **good)
