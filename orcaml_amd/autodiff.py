@@ -848,7 +848,7 @@ class Dropout(Module):
             return x
         if not hasattr(x.ad.inner, "dropout"):
             raise OrcaError("Dropout needs a backend with dropout")
-        M, N = _numel(x.shape[:-1]), x.shape[-1]
+        M, N = (_numel(x.shape[:-1]), x.shape[-1]) if x.shape else (1, 1)
         p, seed, offset = self.p, self.draws.seed, self.draws.next()
         y = x.ad.inner.dropout(x.storage.primal, M, N, p, seed, offset)
 

@@ -202,3 +202,16 @@ def test_scales_a_float_cannot_hold():
     for good in ({"residual_scale": 2.0 ** -126}, {"residual_scale": -2.0 ** 126}, {"block_scale": 0.0},
                  {"block_scale": 1e-50}):
         A.ResidualNorm(ad, 4, **good)
+
+
+@pytest.mark.parametrize("shape,sizes", [((), (1, 1)), ((5,), (1, 5)), ((0,), (1, 0)), ((3, 0), (3, 0)), ((2, 3, 4), (6, 4))])
+def test_dropout_takes_every_shape(shape, sizes):
+    from orcaml_amd import autodiff as A
+
+    class Backend:
+        def dropout(self, x, rows, cols, p, seed, offset):
+            assert (rows, cols) == sizes and (p, seed, offset) == (0.5, 3, 0)
+            return x
+
+    ad = A.Autodiff(Backend())
+    assert A.Dropout(0.5, seed=3)(A.Tensor(ad, A.AdStorage(None), shape)).shape == shape
