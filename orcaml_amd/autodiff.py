@@ -880,7 +880,7 @@ class ResidualNorm(Module):
             if n is not None and n.features != features:
                 raise OrcaError(f"Shape mismatch during residual_norm: expected norms of {features} features, "
                                 f"got {n.features}")
-        # y's gradient is dx over residual_scale: it and its inverse are floats of full precision
+        # neither a subnormal scale, which is not the number that was given, nor one that few gradients survive
         largest = float(np.finfo(np.float32).max)
         if not (2.0 ** -126 <= abs(residual_scale) <= 2.0 ** 126 and abs(block_scale) <= largest):
             raise ValueError("a joint's scales must be floats of 32 bits, residual_scale from 2^-126 to 2^126 in size")
@@ -943,10 +943,18 @@ class ResidualNorm(Module):
                 return [out.get(k) for k in names]
             return Tensor(ad, ad.custom(y, list(inputs.values()), backward), x.shape)
 
+        # y's whole gradient is the kernel's dx at a scale of 1 (nothing else of a backward depends on the scale), and
+        # x's is that times the scale, rounded once
+        block.residual_scale = 1.0
+
         def backward(g, be):
-            asked = want if g[1] is not None else tuple(k for k in want if not k.startswith("dnext"))
-            out = gradients(*g, be, tuple({*asked, "dx"}))  # dx in any case: it is y's own gradient, scaled
-            whole = out["dx"] if rs == 1.0 else be.mul_scalar(out["dx"], 1.0 / rs, (M, N))
+            gy, gu = g
+            asked = tuple(k for k in want if k != "dx" and (gu is not None or not k.startswith("dnext")))
+            if gu is not None:
+                asked += ("dx",)
+            out = gradients(gy, gu, be, asked) if asked else {}
+            whole = out["dx"] if gu is not None else gy
+            out["dx"] = whole if rs == 1.0 else be.mul_scalar(whole, rs, (M, N)) if "dx" in want else None
             return [out.get(k) if k in want else None for k in names], whole
         ys, us = ad.custom_pair((y, u), list(inputs.values()), backward)
         ty, tu = Tensor(ad, ys, x.shape), Tensor(ad, us, x.shape)
