@@ -314,16 +314,19 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
   }
 }
 
-// The gradients, a block for 1024 columns (blockIdx.x) and a piece of rows, from the rows' statistics.
+// The gradients, a block for 1024 columns (a strip) and a piece of rows, from the rows' statistics.  The strips of a piece
+// follow each other.
 __global__ void __launch_bounds__(kStream) norm_strip_kernel(NormBackward a, bool block) {
-  const int64_t c = ((int64_t)blockIdx.x * kStream + threadIdx.x) * 4;
+  const unsigned strips = (unsigned)((a.cols + kStream * 4 - 1) / (kStream * 4));
+  const unsigned strip = blockIdx.x % strips, first = blockIdx.x / strips, blocks = gridDim.x / strips;
+  const int64_t c = ((int64_t)strip * kStream + threadIdx.x) * 4;
   if (c >= a.cols) return;
   const floatx4 zero = splat(0.0f);
   const floatx4 wn = weight4(a.next.w, c, a.cols, 1.0f), wp = weight4(a.post.w, c, a.cols, 1.0f);
   const floatx4 bp = weight4(a.post.b, c, a.cols, 0.0f);
   const bool post = a.post.kind != ORCA_HIP_NORM_NONE;
   floatx4 sum[kSums] = {zero, zero, zero, zero, zero};
-  for (int unit = blockIdx.y; unit < a.groups * a.per_group; unit += gridDim.y) {
+  for (int unit = first; unit < a.groups * a.per_group; unit += blocks) {
     const int group = unit / a.per_group, r0 = group * a.group_rows;
     for (int64_t row = r0 + unit % a.per_group; row < r0 + a.group_rows; row += a.per_group) {
       float s[kRowStats] = {};
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(kStream) norm_strip_kernel(NormBackward a, boo
   }
 #pragma unroll
   for (int i = 0; i < kSums; ++i)
-    if (a.sum[i]) store4(a.sum[i] + blockIdx.y * a.sum_step, c, a.cols, sum[i]);
+    if (a.sum[i]) store4(a.sum[i] + first * a.sum_step, c, a.cols, sum[i]);
 }
 
 // ---------------------------------------------------------------- rows in registers
@@ -965,6 +968,11 @@ int64_t backward_blocks(const orca_hip_ctx* ctx, int64_t rows, int64_t cols, boo
   return 2 * ctx->num_cus;
 }
 
+// Each of a block's teams adds up its rows one after the other: so many at most, and up to twice as many in whole groups
+// (2^25 rows of four columns, of one value each: off by up to 7e-6, and by 1.2e-4 in chains of 8192).  Beyond the usual
+// blocks times that many rows there are more blocks; a vector of partial sums takes 1 / 512 of an operand's bytes then.
+constexpr int64_t kMaxChain = 512;
+
 template <int NW, int Q, bool BIAS>
 auto backward_kernel(bool next, bool block, bool post) {
   if (!next) return post ? norm_backward_kernel<NW, Q, false, true, true, BIAS>
@@ -1017,13 +1025,17 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
   int64_t blocks = registers ? backward_blocks(ctx, a.rows, a.cols, both)
                              : std::max<int64_t>(1, 2 * ctx->num_cus / strips);
   const bool few = registers && a.groups == 1 && a.rows <= (a.cols <= 1024 ? 8 : 2);
+  const int64_t span = kMaxChain * (registers && a.cols <= 1024 ? 4 : 1);  // rows that a block adds up
+  const int64_t least_pieces = (a.group_rows + span - 1) / span;
   if (few) {  // one block, without a launch for partial sums (norm 8 x 512: 5.9 us for 9.9, 4 x 4096 10.9 for 10.2)
     blocks = a.per_group = 1;
-  } else if (a.groups >= blocks) {
+  } else if (a.groups >= blocks && least_pieces == 1) {
     a.per_group = 1;
+    blocks = std::max(blocks, (a.rows + span - 1) / span);
   } else {
     const int64_t least = registers ? a.cols <= 1024 ? 4 : 1 : 16;  // rows of a piece
-    const int64_t most = std::min<int64_t>(blocks / a.groups, (a.group_rows + least - 1) / least);
+    const int64_t most =
+        std::max(least_pieces, std::min<int64_t>(blocks / a.groups, (a.group_rows + least - 1) / least));
     // no more pieces than the longest one's rows ask for: less to add up, and no later an end
     const int64_t longest = (a.group_rows + least * most - 1) / (least * most) * least;
     a.per_group = (int)((a.group_rows + longest - 1) / longest);
@@ -1076,8 +1088,7 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
                        ctx->stream, a, block);
     ORCA_HIP_CHECK(hipGetLastError());
   }
-  hipLaunchKernelGGL(norm_strip_kernel, dim3((unsigned)strips, (unsigned)blocks), dim3(kStream), 0, ctx->stream, a,
-                     block);
+  hipLaunchKernelGGL(norm_strip_kernel, dim3((unsigned)(strips * blocks)), dim3(kStream), 0, ctx->stream, a, block);
   ORCA_HIP_CHECK(hipGetLastError());
   if (!direct) launch_finish(ctx, fin);
 }
