@@ -166,20 +166,39 @@ __device__ __forceinline__ floatx4 weight4(const float* w, int64_t c, int64_t co
 // ---------------------------------------------------------------- rows of any length
 constexpr int kStream = 256;  // threads of a block, 4 columns each at a time
 
+// Sums along a row: quad(c, t) adds what the row's columns c .. c + 3 give.  A thread adds up runs of 64 quads and those
+// to each other: of a row of n values a term goes through 256 + n / 65536 additions of a thread's, not through n / 256
+// (the squares of a row of 2^24 values all alike: the deviation is off by up to 3e-6, and was by 7e-5).
+constexpr int64_t kRun = 64 * kStream * 4;
+template <int N, class F>
+__device__ __forceinline__ void row_sums(int64_t cols, Team<4>& team, float (&t)[N], F quad) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) t[i] = 0.0f;
+  int c = threadIdx.x * 4, end = (int)min(cols, kRun);
+  for (; c < end; c += kStream * 4) quad(c, t);
+  while (end < cols) {
+    end = (int)min(cols, end + kRun);
+    float run[N] = {};
+    for (; c < end; c += kStream * 4) quad(c, run);
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] += run[i];
+  }
+  team.sum(t);
+}
+
 __device__ __forceinline__ Stats stream_stats(const Norm& n, const float* row, int64_t cols, Team<4>& team) {
   float mean = 0.0f;
   const float share = 1.0f / (float)cols;
   if (n.kind == ORCA_HIP_NORM_LAYER) {
-    float t[1] = {0.0f};
-    for (int64_t c = threadIdx.x * 4; c < cols; c += kStream * 4) {
+    float t[1];
+    row_sums(cols, team, t, [&](int64_t c, float (&t)[1]) {
       const floatx4 v = load4(row, c, cols);
       t[0] += (v.x + v.y) + (v.z + v.w);
-    }
-    team.sum(t);
+    });
     mean = t[0] * share;
   }
-  float t[2] = {0.0f, 0.0f};
-  for (int64_t c = threadIdx.x * 4; c < cols; c += kStream * 4) {
+  float t[2];
+  row_sums(cols, team, t, [&](int64_t c, float (&t)[2]) {
     const floatx4 v = load4(row, c, cols);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -187,8 +206,7 @@ __device__ __forceinline__ Stats stream_stats(const Norm& n, const float* row, i
       t[0] += d;
       t[1] = fmaf(d, d, t[1]);
     }
-  }
-  team.sum(t);
+  });
   return stats_of(n, mean, t[0], t[1], share);
 }
 
@@ -259,8 +277,8 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
     float c1 = 0.0f, c2 = 0.0f;
     if (a.du) {
       sy = stream_stats(a.next, y, a.cols, team);
-      float t[2] = {0.0f, 0.0f};
-      for (int64_t c = threadIdx.x * 4; c < a.cols; c += kStream * 4) {
+      float t[2];
+      row_sums(a.cols, team, t, [&](int64_t c, float (&t)[2]) {
         const floatx4 v = load4(y, c, a.cols), d = load4(du, c, a.cols), w = weight4(a.next.w, c, a.cols, 1.0f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -269,8 +287,7 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
           t[0] += e;
           t[1] = fmaf(e, sy.unit(v[j]), t[1]);
         }
-      }
-      team.sum(t);
+      });
       c1 = a.next.kind == ORCA_HIP_NORM_LAYER ? t[0] * share : 0.0f;
       c2 = t[1] * share;
     }
@@ -279,8 +296,8 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
     if (block && a.post.kind != ORCA_HIP_NORM_NONE) {
       const float *f = a.f + row * a.ldf, *gate = a.gate ? a.gate + row / a.gate_rows * a.ldgate : nullptr;
       sf = stream_stats(a.post, f, a.cols, team);
-      float t[2] = {0.0f, 0.0f};
-      for (int64_t c = threadIdx.x * 4; c < a.cols; c += kStream * 4) {
+      float t[2];
+      row_sums(a.cols, team, t, [&](int64_t c, float (&t)[2]) {
         floatx4 g = splat(0.0f);
         if (a.dy) g = load4(dy, c, a.cols);
         if (a.du) {
@@ -300,8 +317,7 @@ __global__ void __launch_bounds__(kStream) norm_stats_kernel(NormBackward a, boo
           t[0] += e;
           t[1] = fmaf(e, sf.unit(v[j]), t[1]);
         }
-      }
-      team.sum(t);
+      });
       p1 = a.post.kind == ORCA_HIP_NORM_LAYER ? t[0] * share : 0.0f;
       p2 = t[1] * share;
     }
