@@ -807,8 +807,9 @@ int orca_hip_norm_backward(orca_hip_ctx* ctx, size_t rows, size_t cols, const fl
  * high word) under the key (seed's low and high word) is at least rint(p 2^32); 1 - p above is the share of
  * words that keep.  The mask depends on the seed, the offset and the place alone (not on leading dimensions), so the
  * gradient of x is the same call on the gradient of y, and no mask is stored.  Calls that are to be independent
- * take different offsets; a captured graph draws its capture's mask at every replay.  0 <= p <= 1; y may be x itself
- * (ldx = ldy). */
+ * take different offsets; a captured graph draws its capture's mask at every replay.  r is the row of this call: processes
+ * or calls that each take a part of a batch need seeds of their own, or they draw one mask for different rows, and
+ * a batch taken in parts does not draw the mask of the whole.  0 <= p <= 1; y may be x itself (ldx = ldy). */
 int orca_hip_dropout(orca_hip_ctx* ctx, size_t rows, size_t cols, const float* x, size_t ldx, double p, uint64_t seed,
                      uint64_t offset, float* y, size_t ldy);
 

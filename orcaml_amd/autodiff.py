@@ -811,8 +811,9 @@ class RMSNorm(_Norm):
 class _Draws:
     """The numbers of a layer's dropout: every call in training takes the next offset under the layer's seed, so
     that a run repeats from its seeds and no two calls share a mask.  Layers that are given seeds take different ones;
-    those without get the next of the process's, from 2^63 on.  `calls` is the place in the sequence: a run that goes
-    on from a checkpoint sets it."""
+    those without get the next of the process's, from 2^63 on in every process: processes that share a batch give
+    their layers seeds, each its own, or they draw equal masks for their different rows.  `calls` is the place in the
+    sequence: a run that goes on from a checkpoint sets it."""
 
     _seeds = itertools.count(2 ** 63)
 
@@ -837,7 +838,7 @@ def _check_p(p: float) -> float:
 class Dropout(Module):
     """In training x / (1 - p) where a value is kept and 0 elsewhere, after eval() x itself (orca_hip_dropout).
     The mask is drawn from (seed, number of the call, place of the value) in the forward and again in the backward,
-    and never stored."""
+    and never stored.  The last dimension, and the others together, are below 2^27."""
 
     def __init__(self, p: float = 0.5, seed: int | None = None):
         super().__init__()
