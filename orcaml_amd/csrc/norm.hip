@@ -994,13 +994,17 @@ auto backward_kernel(bool next, bool block, bool post) {
   if (!next) return post ? norm_backward_kernel<NW, Q, false, true, true, BIAS>
                          : norm_backward_kernel<NW, Q, false, true, false, false>;
   if (!block) return norm_backward_kernel<NW, Q, true, false, false, BIAS>;
-  return post ? norm_backward_kernel<NW, Q, true, true, true, BIAS> : norm_backward_kernel<NW, Q, true, true, false, BIAS>;
+  constexpr bool EIGHT = BIAS && NW == 4 && Q == 4;  // both norms with biases: with_row_shape's eight waves
+  return post ? norm_backward_kernel<NW, Q, true, true, true, BIAS && !EIGHT>
+              : norm_backward_kernel<NW, Q, true, true, false, BIAS>;
 }
 template <int NW, int Q>
 void launch_backward_rows(orca_hip_ctx* ctx, const NormBackward& a, bool block, bool bias, unsigned blocks) {
   const bool post = a.post.kind != ORCA_HIP_NORM_NONE;
-  auto kernel = norm_backward_kernel<NW, Q, true, true, true, true>;
-  if constexpr (NW != 8 || Q != 2)  // the shape for this one alone (with_row_shape)
+  void (*kernel)(NormBackward);
+  if constexpr (NW == 8 && Q == 2)  // the shape for this one alone (with_row_shape)
+    kernel = norm_backward_kernel<NW, Q, true, true, true, true>;
+  else
     kernel = bias ? backward_kernel<NW, Q, true>(a.du, block, post) : backward_kernel<NW, Q, false>(a.du, block, post);
   hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kRowThreads<NW>), 0, ctx->stream, a);
 }
@@ -1035,8 +1039,10 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
   a.group_rows = (int)(a.gate_grouped ? a.gate_rows : a.rows);
   const bool block = a.df || to[kSumGate] || to[kSumPostW] || to[kSumPostB];
   const bool registers = in_registers(a.cols);
-  // what the split of the rows and their shape go by: the parameters, and not which results are wanted
-  const bool both = a.du && a.post.kind != ORCA_HIP_NORM_NONE, heavy = both && (a.post.b || a.next.b);
+  // What the split of the rows and their shape go by: the parameters, and not which results are wanted, but for a
+  // bias's gradient of norms that have none: four waves would spill 36 registers on it (8192 x 4096: 198 us for 180).
+  const bool both = a.du && a.post.kind != ORCA_HIP_NORM_NONE,
+             heavy = both && (a.post.b || a.next.b || to[kSumPostB] || to[kSumNextB]);
   const int64_t strips = registers ? 1 : (a.cols + kStream * 4 - 1) / (kStream * 4);
   int64_t blocks = registers ? backward_blocks(ctx, a.rows, a.cols, both)
                              : std::max<int64_t>(1, 2 * ctx->num_cus / strips);
