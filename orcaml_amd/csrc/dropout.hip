@@ -13,10 +13,11 @@ namespace {
 // A thread takes four neighbouring columns; `across` = 2^across_bits threads of a block lie along a row, the others
 // below each other.  y may be x: a thread reads what it writes first.
 //
-// Bound by HBM.  One quad a thread, blocks of up to 4 KiB of a row and non-temporal stores took 45 us at 8192 x 4096
-// (5.9 TB/s) where four rows a thread with ordinary stores took 67; at 1024 x 4096 6.3 and 8.4.  FAR: non-temporal
-// loads too: 43 us (6.3 TB/s) at 8192 x 4096, whose operands pass the 256 MiB of the memory-side cache, but 22.5 for
-// 20.7 at half of that, which it may hold from the operator before.
+// Bound by HBM: 42 to 45 us at 8192 x 4096 by the box (6.3 to 6.0 TB/s), 6.6 at 1024 x 4096.  One quad a thread, blocks
+// of up to 4 KiB of a row and non-temporal stores (four rows a thread with ordinary stores, its first form, took 67 and
+// 8.4).  FAR: non-temporal loads too: 44.7 us for 46.0 at 8192 x 4096, whose operands pass the 256 MiB of the
+// memory-side cache, but 22.8 for 22.2 at half of that and 7.8 for 6.6 at an eighth, which it may hold from the operator
+// before.
 template <bool FAR>
 __global__ void __launch_bounds__(256) dropout_kernel(const float* x, int64_t ldx, int64_t rows, int64_t cols, float* y,
                                                       int64_t ldy, int across_bits, Dropout d) {

@@ -14,7 +14,7 @@
 // atomics, the same bits every time.
 //
 // Bound by HBM where there are many rows: 8192 x 4096 (134 MB an operand), rms without biases: norm backward 99 us
-// (5.4 TB/s), joint forward 98 us (5.5), joint backward 158 us (5.1; 25 MB of partial sums and a launch of 8 us on
+// (5.4 TB/s), joint forward 98 us (5.5), joint backward 159 us (5.1; 25 MB of partial sums and a launch of 8 us on
 // top), where a copy of 1 GiB runs at 5.0.  Few rows take the latency of a row's chain of sums: 777 x 1501 backward
 // 24 us, of which the partial sums take 5.  Registers decide the rest: see norm_backward_kernel.
 #include <algorithm>
@@ -83,8 +83,8 @@ struct NormBackward {
   float* dgate;
   int64_t lddgate;
   // The rows are in groups (one, but where each row of the gate has its own sum), and those in per_group pieces of
-  // every per_group-th row each, so that the blocks work on neighbouring rows at a time: 8192 x 4096 backward in 107 us,
-  // in 115 with successive rows to a block.  Unit i is piece i % per_group of group i / per_group.
+  // every per_group-th row each, so that the blocks work on neighbouring rows at a time: norm backward of 8192 x 4096 in
+  // 99 us, in 107 with successive rows to a block.  Unit i is piece i % per_group of group i / per_group.
   int group_rows, groups, per_group;
   bool gate_each;     // the gate's gradient row by row, without a sum
   bool gate_grouped;  // its sums are those of the groups
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_rows_kernel(NormForward 
   if (row >= a.rows) return;
   floatx4 wp[Q], bp[Q], wn[Q], bn[Q], gate[Q];
   floatx4 x1[Q], f1[Q];
-  // the weights first, one after the other: with all loads under way together 777 x 1501 took 11.0 us for 9.7
+  // the weights first, one after the other (with all loads under way together the same: joint 777 x 1501 10.4 us)
   const auto load_weight = [&](const float* w, float none, floatx4 (&v)[Q]) {
     rc.load_weight(w, none, v);
     if (w) rc.settle_row(v);
@@ -636,9 +636,13 @@ __global__ void __launch_bounds__(kRowThreads<NW>) norm_rows_kernel(NormForward 
 // Two stages a row, each with the other one's loads in flight: the next norm (y, du), then the block (dy, f).  The
 // weights are in LDS: loads of theirs would wait for those of the rows, and registers go into the sums.
 //
-// Two blocks a CU are worth more than loads ahead: with both norms and biases, eight waves of a row keep to 128
-// registers without (8192 x 4096: 196 us; 210 with loads ahead and one block), and four waves, which do for the others,
-// to 256 (159 us without biases; 185 where more left one block).
+// Two blocks a CU are worth about as much as loads ahead: with both norms and biases, eight waves of a row keep to 128
+// registers without (8192 x 4096: layer norms 166 us, 180 with loads ahead and one block; rms norms, gate and dropout
+// 185 and 177), and four waves, which do for the others, to 256 (159 us without biases; 178 where more left one block).
+//
+// Spills (the compiler's report): every kernel with BLOCK keeps 34 to 108 scalar registers in lanes of vector ones and
+// takes them back inside the row loop (<4, 4, 1, 1, 1, 0>, the large joint's: 97).  <8, 2, 1, 1, 1, 1> spills nine vector
+// registers to memory, <8, 4, 1, 1, 1, 1> two.
 template <int NW, int Q, bool NEXT, bool BLOCK, bool POST, bool BIAS>
 __global__ void __launch_bounds__(kRowThreads<NW>, NW == 8 && Q == 2 ? 4 : NW == 4 && Q == 4 ? 2 : 1)
 norm_backward_kernel(NormBackward a) {
@@ -961,11 +965,12 @@ void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
     hipLaunchKernelGGL(joint ? norm_stream_kernel<true> : norm_stream_kernel<false>, grid, dim3(kStream), 0, ctx->stream,
                        a);
   } else if (a.cols > 512 && a.cols <= 1024 && a.rows <= 4 * ctx->num_cus) {
-    // four waves a row where one a row would leave CUs without any (joint 777 x 1003: 8.4 us for 10.0, but
-    // 2048 x 1024 10.3 for 8.9)
+    // four waves a row where one a row would leave CUs without any (joint 777 x 1003: 7.8 us for 9.4, but
+    // 2048 x 1024 8.9 for 8.4)
     launch_forward_rows<4, 1>(ctx, a, joint);
   } else {
-    // joint 1024 x 4096: 14.2 us in eight waves, 15.4 in four; norm 6.9 in four, 7.6 in eight
+    // joint 300 x 3000: 9.4 us in eight waves, 9.8 in four, 8192 x 2100 73 and 77; norm 1024 x 4096 7.0 in four, 8.5 in
+    // eight
     with_row_shape(a.cols, joint, [&](auto nw, auto q) {
       launch_forward_rows<decltype(nw)::value, decltype(q)::value>(ctx, a, joint);
     });
@@ -973,11 +978,11 @@ void launch_forward(orca_hip_ctx* ctx, const NormForward& a, bool joint) {
   ORCA_HIP_CHECK(hipGetLastError());
 }
 
-// Blocks of a backward.  Two a CU: fewer leave memory idle, more make more partial sums (8192 x 4096: 100 us with two a
-// CU, 114 with one, 109 with four).  One where a CU holds no more: rows of more than 4096 (4096 x 8192 111 for 119 us),
-// and a wave's rows of up to 1024 with both norms (2048 x 1024 with biases 22 for 29; 8192 x 1003 59 for 69, without
-// biases 54 for 51).  Up to four of the smallest rows, 16 rows a block at least (30000 x 200 26 for 29, but 8192 x 64
-// 14 for 13).
+// Blocks of a backward.  Two a CU: fewer leave memory idle, more make more partial sums (norm 8192 x 4096: 99 us with two
+// a CU, 111 with one, 107 with four).  One where a CU holds no more: rows of more than 4096 (4096 x 8192 105 us, 107 with
+// two), and a wave's rows of 513 to 1024 with both norms (2048 x 1024 with biases 22 for 30, without 20 for 27; 8192 x 1003
+// 58 for 70 and 56 for 66).  Up to four of the smallest rows, 16 rows a block at least (131072 x 64 51 us, 71 with two;
+// 131072 x 256 80 and 86; joint 30000 x 200 43 and 48).
 int64_t backward_blocks(const orca_hip_ctx* ctx, int64_t rows, int64_t cols, bool both) {
   if (cols > 4096 || (cols > 512 && cols <= 1024 && both)) return ctx->num_cus;
   if (cols <= 256) return std::max<int64_t>(2 * ctx->num_cus, std::min<int64_t>(4 * ctx->num_cus, rows / 16));
@@ -1049,7 +1054,9 @@ void launch_backward(orca_hip_ctx* ctx, NormBackward& a, float* const (&to)[kSum
   const bool few = registers && a.groups == 1 && a.rows <= (a.cols <= 1024 ? 8 : 2);
   const int64_t span = kMaxChain * (registers && a.cols <= 1024 ? 4 : 1);  // rows that a block adds up
   const int64_t least_pieces = (a.group_rows + span - 1) / span;
-  if (few) {  // one block, without a launch for partial sums (norm 8 x 512: 5.9 us for 9.9, 4 x 4096 10.9 for 10.2)
+  if (few) {
+    // one block, without a launch for partial sums (norm 8 x 512: 6.1 us for 9.0, 2 x 4096 6.9 for 8.9; but 4 x 4096 10.4
+    // for 8.5, joint 16 x 1000 25 for 16)
     blocks = a.per_group = 1;
   } else if (a.groups >= blocks && least_pieces == 1) {
     a.per_group = 1;
