@@ -909,7 +909,7 @@ class ResidualNorm(Module):
                 same += 1
             # [..., 1, 1, features] broadcasts; with one leading dimension each, rows in groups are meant
             fits = all(d == 1 for d in lead[same:]) or (len(lead) == 1 and len(x.shape) == 2)
-            if not fits or groups == 0 or M % groups:
+            if not fits or (M % groups if groups else M):
                 raise OrcaError(f"Shape mismatch during {op}: expected a gate of {list(x.shape)} with ones from some "
                                 f"dimension on, got {list(gate.shape)}")
         post, nxt = self.post, self.next
@@ -920,7 +920,7 @@ class ResidualNorm(Module):
         p = self.p if self.training else 0.0
         block = be.ResidualBlock(post=post.kind if post else "none", post_eps=post.eps if post else 0.0,
                                  next=nxt.kind if nxt else "none", next_eps=nxt.eps if nxt else 0.0,
-                                 gate=gate.storage.primal if gate is not None else None, groups=groups,
+                                 gate=gate.storage.primal if gate is not None and groups else None, groups=groups,
                                  residual_scale=self.residual_scale, block_scale=self.block_scale, p=p,
                                  seed=self.draws.seed, offset=self.draws.next() if p else 0,
                                  **{k: s.primal if s is not None else None for k, s in vectors.items()})
@@ -935,8 +935,14 @@ class ResidualNorm(Module):
         fp, yp = f.storage.primal if reads_f else None, y if nxt is not None else None
         rs, names = self.residual_scale, tuple(inputs)  # the node holds no more of the operands than that
 
+        gate_shape = gate.shape if gate is not None else None
+
         def gradients(gy, gu, be, asked):
-            return be.residual_norm_backward(gy, gu, fp, yp, M, N, block, want=asked)
+            read = tuple(k for k in asked if k != "dgate" or groups)
+            out = be.residual_norm_backward(gy, gu, fp, yp, M, N, block, want=read)
+            if len(read) < len(asked):  # a gate of no rows, for none
+                out["dgate"] = be.zeros(gate_shape)
+            return out
 
         if nxt is None:
             def backward(g, be):
